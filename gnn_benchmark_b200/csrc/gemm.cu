@@ -27,13 +27,12 @@
 //               under the MMAs of the next.
 // Every wait is bounded (about a second); on a time-out the kernel records a code in the status
 // word of the workspace, drains its own copies and MMAs, frees tensor memory and returns.
-#include <cuda.h>
-
-#include <mutex>
-
-#include "common.cuh"
+#include "tc.cuh"
 
 namespace gnnagg {
+
+StallTest g_stall;
+
 namespace {
 
 constexpr int BM = 128;                 // rows of A per tile = UMMA M = TMEM lanes
@@ -58,99 +57,8 @@ constexpr int BIAS_BYTES = kMaxN * 4;
 constexpr int kNumBarriers = 3 * kStages + 4 + 1;
 constexpr int SMEM_BYTES = 1024 + kStages * STAGE_BYTES + EPI_BYTES + BIAS_BYTES + 256;
 constexpr int kThreads = 320;
-constexpr unsigned long long kWaitLimitNs = 1000ull * 1000ull * 1000ull;  // every launch but the stall test's
-constexpr int kStatusBytes = 256;
 
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
-
-__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-__device__ __forceinline__ unsigned long long globaltimer_ns() {
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive_expect_tx(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-        "selp.u32 %0, 1, 0, p;\n"
-        "}\n"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-
-// Bounded wait.  Returns false when another role has raised `abort_flag` or when this wait ran out
-// of time (it then raises the flag and leaves `code` in the status word, first writer wins).
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *status,
-                                          int code, unsigned long long limit_ns) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const unsigned long long t0 = globaltimer_ns();
-    uint32_t n = 0;
-    while (!mbar_try_wait(bar, parity)) {
-        if ((++n & 31u) == 0) {
-            if (*abort_flag != 0) return false;
-            if (globaltimer_ns() - t0 > limit_ns) {
-                *abort_flag = 1;
-                atomicCAS(status, 0, code);
-                return false;
-            }
-        }
-    }
-    return true;
-}
-
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
-        "l"(map), "r"(bar), "r"(x), "r"(y)
-        : "memory");
-}
-__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap *map, int x, int y) {
-    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
-}
-
-// Shared -> global tile store / add through the tensor map (rows and columns outside the tensor are clipped).
-__device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, uint32_t src, int x, int y) {
-    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(src),
-                 "r"(x), "r"(y)
-                 : "memory");
-}
-__device__ __forceinline__ void tma_reduce_add_2d(const CUtensorMap *map, uint32_t src, int x, int y) {
-    asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map),
-                 "r"(src), "r"(x), "r"(y)
-                 : "memory");
-}
-__device__ __forceinline__ void tma_store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-template <int kPending>
-__device__ __forceinline__ void tma_store_wait_read() {
-    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kPending) : "memory");
-}
-__device__ __forceinline__ void tma_store_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
-
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_generic_to_async_smem() {
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-}
-
-__device__ __forceinline__ void tc_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
 
 __device__ __forceinline__ void tc_mma_tf32(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                             uint32_t accumulate) {
@@ -162,22 +70,6 @@ __device__ __forceinline__ void tc_mma_tf32(uint32_t tmem_d, uint64_t adesc, uin
         "}\n" ::"r"(tmem_d),
         "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
-}
-
-// 32 lanes x 32 columns of fp32: thread t of the warp receives columns [c, c+32) of TMEM lane
-// (lane base of the address) + t.
-__device__ __forceinline__ void tc_ld_32x32(uint32_t taddr, uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr)
-        : "memory");
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
 __device__ __forceinline__ float tf32_rna(float x) {
@@ -198,19 +90,6 @@ __device__ __forceinline__ float lo_of_truncated(float x) {
     const float hi = __uint_as_float(__float_as_uint(x) & 0xFFFFE000u);
     const float rest = x - hi;  // exact
     return (fabsf(hi) <= 3.402823466e38f) ? tf32_rna(rest) : 0.0f;
-}
-
-// Shared-memory matrix descriptor of a K-major tile whose rows are 128 bytes, 128-byte-swizzled (what
-// TMA writes for a {32 fp32, rows} box): start address, 8-row group stride 1024 bytes, descriptor
-// version 1 (sm_100), layout type 2 (128-byte swizzle).
-__device__ __forceinline__ uint64_t make_smem_desc(uint32_t smem_addr) {
-    uint64_t d = 0;
-    d |= (uint64_t)((smem_addr & 0x3FFFFu) >> 4);       // bits [0,14)
-    d |= (uint64_t)1 << 16;                              // leading byte offset (unused for swizzled K-major)
-    d |= (uint64_t)(1024 >> 4) << 32;                    // stride byte offset
-    d |= (uint64_t)1 << 46;                              // descriptor version
-    d |= (uint64_t)2 << 61;                              // SWIZZLE_128B
-    return d;
 }
 
 // Instruction descriptor of kind::tf32: fp32 accumulator, TF32 A and B, both K-major, M = 128.
@@ -832,23 +711,6 @@ __global__ void split_weight_kernel(const float *__restrict__ W, int64_t ldb, in
     }
 }
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn() {
-    static EncodeTiledFn fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void *ptr = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeTiledFn>(ptr);
-    });
-    return fn;
-}
-
 // 2-D fp32 tensor map: `cols` contiguous elements per row, `rows` rows of stride ld elements;
 // box = {box_cols, box_rows} with box_cols * 4 bytes = the swizzle span; out-of-range elements read
 // as zero and are not written.
@@ -868,14 +730,6 @@ int make_map(CUtensorMap *map, const float *base, int64_t rows, int64_t cols, in
     if (r != CUDA_SUCCESS) return fail(GNNAGG_ERR_CUDA, "dense: cuTensorMapEncodeTiled failed with code %d", (int)r);
     return GNNAGG_OK;
 }
-
-// Stall test: the launches that follow announce `tx_excess` bytes that never arrive, so their first wait for a
-// load runs out after `wait_ns` and the kernel takes its abort path.  Zero in normal operation.
-struct StallTest {
-    unsigned long long wait_ns = kWaitLimitNs;
-    uint32_t tx_excess = 0;
-};
-StallTest g_stall;
 
 inline int round_up(int v, int m) { return (v + m - 1) / m * m; }
 inline size_t piece_bytes(int N, int K) { return ((size_t)N * round_up(K, 4) * 4 + 255) / 256 * 256; }

@@ -3,7 +3,9 @@
 #include <stdarg.h>
 #include <string.h>
 
-#include "common.cuh"
+#include <mutex>
+
+#include "tc.cuh"
 
 namespace gnnagg {
 
@@ -23,6 +25,19 @@ int check_launch(const char *what) {
     const cudaError_t e = cudaGetLastError();
     if (e == cudaSuccess) return GNNAGG_OK;
     return fail(GNNAGG_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+}
+
+EncodeTiledFn encode_fn() {
+    static EncodeTiledFn fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void *ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeTiledFn>(ptr);
+    });
+    return fn;
 }
 
 __global__ void cast_f32_bf16_kernel(const float *__restrict__ src, __nv_bfloat16 *__restrict__ dst, int64_t n) {
