@@ -62,7 +62,28 @@ SIGNATURES = {
     "gnnagg_relu_dropout_bwd": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i32, ctypes.c_float, _vp, _i64, _vp]),
     "gnnagg_dropout_ln_relu_bwd": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i32, ctypes.c_float,
                                                   _vp, _i64, _vp, _sz, _vp, _vp, _vp]),
+    "gnnagg_rms_norm_fwd": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i32, _i64, _i32, _i32, ctypes.c_float, _vp, _i64,
+                                           _vp, _i64, _vp, _vp]),
+    "gnnagg_rms_norm_fp8": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i32, _i64, _i32, _i32, ctypes.c_float, _vp, _i64,
+                                           _vp, _i64, _vp, _i64, _vp]),
+    "gnnagg_rms_norm_partial_bytes": (_sz, [_i64, _i32, _i32]),
+    "gnnagg_rms_norm_bwd": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i32, _i64, _i32, _i32, _vp, _i64,
+                                           _vp, _vp, _sz, _vp]),
+    "gnnagg_fp8_quantize": (ctypes.c_int, [_vp, _i64, _i64, _i64, _i32, _i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64,
+                                           _vp]),
+    "gnnagg_fp8_matmul_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "gnnagg_fp8_matmul": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i64, _i32, _vp, _i64, _vp, _i64, _i64, _i32, _i64, _i64,
+                                         _i64, _vp, _i32, _vp, _i64, _i32, _vp, _sz, _vp]),
+    "gnnagg_fp8_matmul_status": (ctypes.c_int, [_vp]),
+    "gnnagg_fp8_matmul_status_clear": (ctypes.c_int, [_vp]),
+    "gnnagg_adamw_scalars_bytes": (_sz, []),
+    "gnnagg_adamw_tick": (ctypes.c_int, [_vp, _vp] + [ctypes.c_double] * 5 + [_vp, _vp]),
+    "gnnagg_adamw_step": (ctypes.c_int, [_vp, _i64, _i32, _i32] + [ctypes.c_double] * 5 + [_i64, _vp, _vp]),
 }
+
+# element types of the low-precision entry points
+F32, BF16, F16 = 0, 1, 2
+TYPES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
 
 
 def lib():
@@ -98,6 +119,33 @@ def stream_ptr(device=None) -> int:
 def ptr(t) -> int:
     """Device address of a tensor, 0 for None."""
     return 0 if t is None else t.data_ptr()
+
+
+class device_of:
+    """Makes a tensor's device current for a launch (kernels go to the current device) and puts the caller's
+    back; free where it is current already."""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, t):
+        self.index = t.device.index
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
+
+
+def empty_codes(rows: int, cols: int, device):
+    """Uninitialised e4m3 codes (rows, cols) whose rows start on 16 bytes, and their scales, one per row and 128
+    columns, (rows, ceil(cols / 128)) lying column by column."""
+    codes = torch.empty((rows, (cols + 15) // 16 * 16), dtype=torch.float8_e4m3fn, device=device)
+    scales = torch.empty(((cols + 127) // 128, rows), dtype=torch.float32, device=device)
+    return codes[:, :cols], scales.t()
 
 
 def require_cuda(*tensors) -> None:

@@ -19,6 +19,7 @@ NVCC_FLAGS = [
     "-lineinfo",
     "-Xcompiler", "-fPIC",
     "--shared",
+    "--threads", "0",  # as many files at once as the machine has cores
     "-ccbin", "/usr/bin/g++",
 ]
 

@@ -1,0 +1,99 @@
+// Element types of the low-precision path: 16-byte vectors of fp32 / bf16 / fp16 as fp32 registers, and the
+// e4m3 blocks that the 8-bit operands and optimiser moments are held in.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace gnnagg {
+
+// Block scaling: a = max |u| over the block, at least 2^-96 (so that its reciprocal stays finite);
+// code = e4m3(u * (448 * (1 / a))), value = code * (a * (1 / 448)).  Every step is rounded to nearest on its
+// own, so that the codes are the same however a caller computes them.
+constexpr float kE4m3Max = 448.0f;
+constexpr float kBlockTiny = 1.262177448e-29f;  // 2^-96
+static_assert(kBlockTiny == 1.0f / 79228162514264337593543950336.0f, "2^-96");
+
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
+// Largest magnitudes are compared as bit patterns: the order of |x|, with NaN above infinity, so a block that
+// holds a NaN or an infinity gets a NaN or infinite scale and reads back as NaN instead of losing it.
+__device__ __forceinline__ float block_amax(uint32_t bits) {
+    return __uint_as_float(max(bits, __float_as_uint(kBlockTiny)));
+}
+__device__ __forceinline__ float block_factor(float amax) { return __fmul_rn(__frcp_rn(amax), kE4m3Max); }
+__device__ __forceinline__ float block_scale(float amax) { return __fmul_rn(amax, 1.0f / kE4m3Max); }
+
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+    return lo | (hi << 16);
+}
+__device__ __forceinline__ float4 from_e4m3x4(uint32_t v) {
+    const __half2 lo(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(v & 0xFFFFu), __NV_E4M3));
+    const __half2 hi(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(v >> 16), __NV_E4M3));
+    const float2 a = __half22float2(lo), b = __half22float2(hi);
+    return make_float4(a.x, a.y, b.x, b.y);
+}
+
+enum : int { kTypeF32 = GNNAGG_F32, kTypeBf16 = GNNAGG_BF16, kTypeF16 = GNNAGG_F16 };
+
+inline int type_size(int type) { return type == kTypeF32 ? 4 : (type == kTypeBf16 || type == kTypeF16 ? 2 : 0); }
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+
+template <typename T>
+struct Vec {
+    static constexpr int N = 16 / (int)sizeof(T);  // elements of one 16-byte access
+};
+
+template <typename T>
+__device__ __forceinline__ void unpack16(const uint4 &u, float (&f)[Vec<T>::N]) {
+    const T *e = reinterpret_cast<const T *>(&u);
+#pragma unroll
+    for (int i = 0; i < Vec<T>::N; ++i) f[i] = to_f32(e[i]);
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack16(const float (&f)[Vec<T>::N]) {
+    uint4 u;
+    T *e = reinterpret_cast<T *>(&u);
+#pragma unroll
+    for (int i = 0; i < Vec<T>::N; ++i) e[i] = from_f32<T>(f[i]);
+    return u;
+}
+
+// Vec<T>::N consecutive elements at p, of which `valid` exist (the others read as zero).  VEC: one 16-byte
+// access (p aligned, all valid); otherwise element by element.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_chunk(const T *p, int valid, float (&f)[Vec<T>::N]) {
+    if (VEC) {
+        unpack16<T>(__ldcs(reinterpret_cast<const uint4 *>(p)), f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < Vec<T>::N; ++i) f[i] = i < valid ? to_f32(p[i]) : 0.0f;
+    }
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void store_chunk(T *p, int valid, const float (&f)[Vec<T>::N]) {
+    if (VEC) {
+        *reinterpret_cast<uint4 *>(p) = pack16<T>(f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < Vec<T>::N; ++i)
+            if (i < valid) p[i] = from_f32<T>(f[i]);
+    }
+}
+
+}  // namespace gnnagg

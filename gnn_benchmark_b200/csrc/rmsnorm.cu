@@ -1,0 +1,472 @@
+// Root-mean-square norm with the residual's addition, its gradients, and its output as e4m3 codes.
+//
+//     h = x + residual (rounded to the stream's type: h is an output, and the norm is of what is stored)
+//     y = h * r * w,   r = rsqrt(mean(h^2) + eps)
+//     dh = gh + r * (w gy - hat * mean(w gy hat)),  hat = h r;   dw = sum over rows of gy hat
+//
+// Forward is one pass: a row stays in registers between the sum of squares and the scaling.  A row of up to
+// 128 16-byte chunks belongs to a warp (eight rows a block), a longer one to a block.  Backward reads h and the
+// two gradients once, writes dh once and keeps the column sums of dw in registers over all rows of a
+// persistent block; a second kernel adds the blocks' sums in a fixed order (no atomics).
+//
+// As codes: with t = h w and a = max |t| over 128 columns, code = e4m3(t * (448 / a)) and scale = a / 448 * r.
+// The row's statistic enters the scale alone, so the codes are ready before the sum of squares is, and do not
+// depend on its order of summation.
+#include "lowp.cuh"
+
+namespace gnnagg {
+namespace {
+
+constexpr int kRowThreads = 256;             // block of the warp-per-row and the block-per-row forms
+constexpr int kWideThreads = 1024;           // block of the widest rows
+constexpr int kMaxWidth = 16384;
+
+template <int GT>
+struct Shape {
+    static constexpr int kThreads = GT == 32 ? kRowThreads : GT;
+    static constexpr int kRows = kThreads / GT;  // rows a block works on at once
+};
+
+// Sum over the GT threads of a row; every thread gets it.  `red` holds a value per warp.
+template <int GT>
+__device__ __forceinline__ float row_sum(float v, float *red) {
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(kFullMask, v, off);
+    if (GT == 32) return v;
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < GT / 32; ++i) s += red[i];
+    return s;
+}
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_weight(const void *w, bool w_f32, int col, int valid, float (&f)[Vec<T>::N]) {
+    constexpr int V = Vec<T>::N;
+    if (VEC && !w_f32) {
+        unpack16<T>(__ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(w) + col)), f);
+    } else if (VEC) {
+#pragma unroll
+        for (int i = 0; i < V; i += 4) {
+            const float4 v = __ldg(reinterpret_cast<const float4 *>(static_cast<const float *>(w) + col + i));
+            f[i] = v.x, f[i + 1] = v.y, f[i + 2] = v.z, f[i + 3] = v.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            f[i] = i < valid ? (w_f32 ? __ldg(static_cast<const float *>(w) + col + i)
+                                      : to_f32(static_cast<const T *>(w)[col + i]))
+                             : 0.0f;
+    }
+}
+
+struct FwdParams {
+    const void *x, *residual, *w;
+    void *h, *y;      // y: the stream's type, or codes
+    float *scales, *rstd;
+    int64_t ldx, ldr, ldh, ldy, lds;
+    int64_t rows;
+    int F, w_f32;
+    float eps;
+};
+
+template <typename T, int GT, int NV, bool VEC, bool FP8>
+__global__ void __launch_bounds__(Shape<GT>::kThreads) rms_norm_fwd_kernel(const FwdParams p) {
+    constexpr int V = Vec<T>::N;
+    __shared__ float red[32];
+    const int lane = threadIdx.x % GT;
+    const int64_t row = (int64_t)blockIdx.x * Shape<GT>::kRows + threadIdx.x / GT;
+    if (GT == 32 && row >= p.rows) return;  // whole warps; a wider row's block has a row of its own
+    const T *x = static_cast<const T *>(p.x) + row * p.ldx;
+    const T *res = static_cast<const T *>(p.residual) + row * p.ldr;
+    float v[NV][V];
+    float ss = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int col = (lane + GT * j) * V, valid = p.F - col;
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[j][i] = 0.0f;
+        if (valid > 0) {
+            load_chunk<T, VEC>(x + col, valid, v[j]);
+            if (p.residual != nullptr) {
+                float r[V];
+                load_chunk<T, VEC>(res + col, valid, r);
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[j][i] = to_f32(from_f32<T>(v[j][i] + r[i]));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) ss = fmaf(v[j][i], v[j][i], ss);
+    }
+    const float rstd = rsqrtf(row_sum<GT>(ss, red) / (float)p.F + p.eps);
+    if (lane == 0 && p.rstd != nullptr) p.rstd[row] = rstd;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int col = (lane + GT * j) * V, valid = p.F - col;
+        float w[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) w[i] = 0.0f;
+        if (valid > 0) {
+            if (p.residual != nullptr)
+                store_chunk<T, VEC>(static_cast<T *>(p.h) + row * p.ldh + col, valid, v[j]);
+            load_weight<T, VEC>(p.w, p.w_f32 != 0, col, valid, w);
+        }
+        if (!FP8) {
+            if (valid > 0) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[j][i] = v[j][i] * rstd * w[i];
+                store_chunk<T, VEC>(static_cast<T *>(p.y) + row * p.ldy + col, valid, v[j]);
+            }
+        } else {
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                v[j][i] = __fmul_rn(v[j][i], w[i]);
+                m = max(m, abs_bits(v[j][i]));
+            }
+            // 128 columns are 128 / V neighbouring threads: a whole or half a warp
+#pragma unroll
+            for (int off = 64 / V; off > 0; off >>= 1) m = max(m, __shfl_xor_sync(kFullMask, m, off));
+            const float a = block_amax(m), f = block_factor(a);
+            if (valid > 0) {
+                // code rows are padded to 16 bytes, so a whole chunk always fits; columns from F on are zeros
+                uint32_t c[V / 4];
+#pragma unroll
+                for (int i = 0; i < V / 4; ++i)
+                    c[i] = e4m3x4(v[j][4 * i] * f, v[j][4 * i + 1] * f, v[j][4 * i + 2] * f, v[j][4 * i + 3] * f);
+                uint32_t *dst = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(p.y) + row * p.ldy + col);
+                if (V == 8)
+                    *reinterpret_cast<uint2 *>(dst) = make_uint2(c[0], c[V / 4 - 1]);
+                else
+                    *dst = c[0];
+                if ((col & 127) == 0) p.scales[(int64_t)(col >> 7) * p.lds + row] = block_scale(a) * rstd;
+            }
+        }
+    }
+}
+
+struct BwdParams {
+    const void *gy, *gh, *h, *w;
+    const float *rstd;
+    void *gx;
+    float *partial;   // [blocks][F]
+    int64_t ldgy, ldgh, ldh, ldgx;
+    int64_t rows;
+    int F, w_f32;
+};
+
+template <typename T, int GT, int NV, bool VEC>
+__global__ void __launch_bounds__(Shape<GT>::kThreads) rms_norm_bwd_kernel(const BwdParams p) {
+    constexpr int V = Vec<T>::N;
+    constexpr int kRows = Shape<GT>::kRows;
+    __shared__ float red[2][32];
+    __shared__ float cols[GT == 32 ? kRows * 32 * V : 1];
+    const int lane = threadIdx.x % GT, slot = threadIdx.x / GT;
+    const float inv_f = 1.0f / (float)p.F;
+    float w[NV][V], dw[NV][V];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int col = (lane + GT * j) * V, valid = p.F - col;
+#pragma unroll
+        for (int i = 0; i < V; ++i) w[j][i] = 0.0f, dw[j][i] = 0.0f;
+        if (valid > 0) load_weight<T, VEC>(p.w, p.w_f32 != 0, col, valid, w[j]);
+    }
+    int turn = 0;
+    for (int64_t row = (int64_t)blockIdx.x * kRows + slot; row < p.rows; row += (int64_t)gridDim.x * kRows, turn ^= 1) {
+        const float rstd = __ldg(p.rstd + row);
+        float hat[NV][V], g[NV][V], gh[NV][V];
+        float s = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int col = (lane + GT * j) * V, valid = p.F - col;
+#pragma unroll
+            for (int i = 0; i < V; ++i) hat[j][i] = 0.0f, g[j][i] = 0.0f, gh[j][i] = 0.0f;
+            if (valid > 0) {
+                load_chunk<T, VEC>(static_cast<const T *>(p.h) + row * p.ldh + col, valid, hat[j]);
+                load_chunk<T, VEC>(static_cast<const T *>(p.gy) + row * p.ldgy + col, valid, g[j]);
+                if (p.gh != nullptr)
+                    load_chunk<T, VEC>(static_cast<const T *>(p.gh) + row * p.ldgh + col, valid, gh[j]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                hat[j][i] *= rstd;
+                dw[j][i] = fmaf(g[j][i], hat[j][i], dw[j][i]);
+                g[j][i] *= w[j][i];
+                s = fmaf(g[j][i], hat[j][i], s);
+            }
+        const float c = row_sum<GT>(s, red[turn]) * inv_f;  // two buffers: a warp may be a row ahead of another
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int col = (lane + GT * j) * V, valid = p.F - col;
+            if (valid > 0) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) gh[j][i] = fmaf(rstd, g[j][i] - hat[j][i] * c, gh[j][i]);
+                store_chunk<T, VEC>(static_cast<T *>(p.gx) + row * p.ldgx + col, valid, gh[j]);
+            }
+        }
+    }
+    float *out = p.partial + (int64_t)blockIdx.x * p.F;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int col = (lane + GT * j) * V;
+        if (GT == 32) {  // the block's warps add up in warp order
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < V; ++i) cols[(slot * V + i) * 32 + lane] = dw[j][i];
+            __syncthreads();
+            for (int e = threadIdx.x; e < 32 * V; e += kRowThreads) {
+                float s = 0.0f;
+#pragma unroll
+                for (int r = 0; r < kRows; ++r) s += cols[r * 32 * V + e];
+                const int c = ((e & 31) + 32 * j) * V + (e >> 5);
+                if (c < p.F) out[c] = s;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (col + i < p.F) out[col + i] = dw[j][i];
+        }
+    }
+}
+
+// Rows too wide for the registers of a block: two sweeps over the row (the second finds it in L1 / L2), and the
+// column sums of dw in shared memory, where every thread adds to columns of its own.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kWideThreads) rms_norm_bwd_wide_kernel(const BwdParams p) {
+    constexpr int V = Vec<T>::N;
+    extern __shared__ float dw[];  // [V][chunks]
+    __shared__ float red[2][32];
+    const int chunks = (p.F + V - 1) / V;
+    const float inv_f = 1.0f / (float)p.F;
+    for (int i = threadIdx.x; i < chunks * V; i += kWideThreads) dw[i] = 0.0f;
+    __syncthreads();
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
+        const float rstd = __ldg(p.rstd + row);
+        const T *h = static_cast<const T *>(p.h) + row * p.ldh, *gy = static_cast<const T *>(p.gy) + row * p.ldgy;
+        float s = 0.0f;
+        for (int k = threadIdx.x; k < chunks; k += kWideThreads) {
+            const int col = k * V, valid = p.F - col;
+            float hat[V], g[V], w[V];
+            load_chunk<T, VEC>(h + col, valid, hat);
+            load_chunk<T, VEC>(gy + col, valid, g);
+            load_weight<T, VEC>(p.w, p.w_f32 != 0, col, valid, w);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                hat[i] *= rstd;
+                dw[i * chunks + k] = fmaf(g[i], hat[i], dw[i * chunks + k]);
+                s = fmaf(g[i] * w[i], hat[i], s);
+            }
+        }
+        const float c = row_sum<kWideThreads>(s, red[turn]) * inv_f;
+        for (int k = threadIdx.x; k < chunks; k += kWideThreads) {
+            const int col = k * V, valid = p.F - col;
+            float hat[V], g[V], w[V], gh[V];
+            load_chunk<T, VEC>(h + col, valid, hat);
+            load_chunk<T, VEC>(gy + col, valid, g);
+            load_weight<T, VEC>(p.w, p.w_f32 != 0, col, valid, w);
+#pragma unroll
+            for (int i = 0; i < V; ++i) gh[i] = 0.0f;
+            if (p.gh != nullptr) load_chunk<T, VEC>(static_cast<const T *>(p.gh) + row * p.ldgh + col, valid, gh);
+#pragma unroll
+            for (int i = 0; i < V; ++i) gh[i] = fmaf(rstd, g[i] * w[i] - hat[i] * rstd * c, gh[i]);
+            store_chunk<T, VEC>(static_cast<T *>(p.gx) + row * p.ldgx + col, valid, gh);
+        }
+    }
+    float *out = p.partial + (int64_t)blockIdx.x * p.F;
+    for (int k = threadIdx.x; k < chunks; k += kWideThreads)
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (k * V + i < p.F) out[k * V + i] = dw[i * chunks + k];
+}
+
+// dw[c] = sum of partial[b][c] over the blocks, in a fixed order: 16 threads take every 16th block of a column.
+template <typename T>
+__global__ void __launch_bounds__(512) rms_norm_dw_kernel(const float *__restrict__ partial, int blocks, int F, T *dw) {
+    __shared__ float red[16][33];
+    const int c = blockIdx.x * 32 + threadIdx.x;
+    float s = 0.0f;
+    if (c < F) {
+#pragma unroll 8
+        for (int b = threadIdx.y; b < blocks; b += 16) s += partial[(int64_t)b * F + c];
+    }
+    red[threadIdx.y][threadIdx.x] = s;
+    __syncthreads();
+    if (threadIdx.y == 0 && c < F) {
+#pragma unroll
+        for (int i = 1; i < 16; ++i) s += red[i][threadIdx.x];
+        dw[c] = from_f32<T>(s);
+    }
+}
+
+// How a row of F elements of `size` bytes is spread: threads per row and 16-byte chunks per thread.
+struct Spread {
+    int gt, nv;
+};
+Spread spread_of(int F, int size) {
+    const int chunks = (int)div_up(F, 16 / size);
+    if (chunks <= 32) return {32, 1};
+    if (chunks <= 64) return {32, 2};
+    if (chunks <= 128) return {32, 4};
+    if (chunks <= 256) return {256, 1};
+    if (chunks <= 512) return {256, 2};
+    if (chunks <= 1024) return {256, 4};
+    return {kWideThreads, 4};
+}
+
+int bwd_blocks(int64_t rows, int F, int size) {
+    const Spread s = spread_of(F, size);
+    const int64_t need = div_up(rows, s.gt == 32 ? kRowThreads / 32 : 1);
+    const int64_t cap = (int64_t)kNumSMs * (s.gt == kWideThreads ? 2 : 4);
+    return (int)(need < cap ? need : cap);
+}
+
+template <typename F32, typename BF16, typename F16>
+int by_type(int type, F32 a, BF16 b, F16 c) {
+    return type == kTypeF32 ? a() : type == kTypeBf16 ? b() : c();
+}
+
+template <typename T, bool VEC, bool FP8>
+int launch_fwd(const FwdParams &p, cudaStream_t st) {
+    const Spread s = spread_of(p.F, (int)sizeof(T));
+    const int64_t blocks = s.gt == 32 ? div_up(p.rows, kRowThreads / 32) : p.rows;
+    const dim3 grid((unsigned)blocks);
+#define RMS_LAUNCH(GT, NV) rms_norm_fwd_kernel<T, GT, NV, VEC, FP8><<<grid, Shape<GT>::kThreads, 0, st>>>(p)
+    if (s.gt == 32 && s.nv == 1) RMS_LAUNCH(32, 1);
+    else if (s.gt == 32 && s.nv == 2) RMS_LAUNCH(32, 2);
+    else if (s.gt == 32) RMS_LAUNCH(32, 4);
+    else if (s.gt == 256 && s.nv == 1) RMS_LAUNCH(256, 1);
+    else if (s.gt == 256 && s.nv == 2) RMS_LAUNCH(256, 2);
+    else if (s.gt == 256) RMS_LAUNCH(256, 4);
+    else RMS_LAUNCH(kWideThreads, 4);
+#undef RMS_LAUNCH
+    return check_launch("rms_norm_fwd_kernel");
+}
+
+template <typename T, bool VEC>
+int launch_bwd(const BwdParams &p, int blocks, cudaStream_t st) {
+    const Spread s = spread_of(p.F, (int)sizeof(T));
+#define RMS_LAUNCH(GT, NV) rms_norm_bwd_kernel<T, GT, NV, VEC><<<blocks, Shape<GT>::kThreads, 0, st>>>(p)
+    if (s.gt == 32 && s.nv == 1) RMS_LAUNCH(32, 1);
+    else if (s.gt == 32 && s.nv == 2) RMS_LAUNCH(32, 2);
+    else if (s.gt == 32) RMS_LAUNCH(32, 4);
+    else if (s.gt == 256 && s.nv == 1) RMS_LAUNCH(256, 1);
+    else if (s.gt == 256 && s.nv == 2) RMS_LAUNCH(256, 2);
+    else if (s.gt == 256) RMS_LAUNCH(256, 4);
+    else {
+        static PerDeviceOnce attr_done;
+        const cudaError_t e = attr_done.run([] {
+            return cudaFuncSetAttribute(rms_norm_bwd_wide_kernel<T, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        kMaxWidth * (int)sizeof(float));
+        });
+        if (e != cudaSuccess) return fail(GNNAGG_ERR_CUDA, "rms_norm_bwd: %s", cudaGetErrorString(e));
+        const size_t smem = (size_t)div_up(p.F, Vec<T>::N) * Vec<T>::N * sizeof(float);
+        rms_norm_bwd_wide_kernel<T, VEC><<<blocks, kWideThreads, smem, st>>>(p);
+    }
+#undef RMS_LAUNCH
+    return check_launch("rms_norm_bwd_kernel");
+}
+
+template <typename T>
+int launch_dw(const float *partial, int blocks, int F, void *dw, cudaStream_t st) {
+    rms_norm_dw_kernel<T><<<(unsigned)div_up(F, 32), dim3(32, 16), 0, st>>>(partial, blocks, F, static_cast<T *>(dw));
+    return check_launch("rms_norm_dw_kernel");
+}
+
+// 16-byte accesses of rows at p with a stride of ld elements
+bool vec_rows(const void *p, int64_t ld, int size) { return aligned16(p) && (ld * size) % 16 == 0; }
+
+int check_common(const char *what, int type, int w_type, int64_t rows, int F) {
+    if (type_size(type) == 0) return fail(GNNAGG_ERR_ARG, "%s: unknown element type %d", what, type);
+    if (w_type != kTypeF32 && w_type != type)
+        return fail(GNNAGG_ERR_ARG, "%s: the weight is fp32 or of the rows' type", what);
+    if (rows < 0 || F <= 0) return fail(GNNAGG_ERR_ARG, "%s: negative or zero size", what);
+    if (F > kMaxWidth || rows > 0x7FFFFFFF)
+        return fail(GNNAGG_ERR_UNSUPPORTED, "%s: at most %d columns and 2^31 - 1 rows", what, kMaxWidth);
+    return GNNAGG_OK;
+}
+
+int fwd(const char *what, bool fp8, const void *x, int64_t ldx, const void *residual, int64_t ldr, const void *w,
+        int w_type, int64_t rows, int F, int type, float eps, void *h, int64_t ldh, void *y, int64_t ldy, float *scales,
+        int64_t lds, float *rstd, void *stream) {
+    int rc = check_common(what, type, w_type, rows, F);
+    if (rc != GNNAGG_OK) return rc;
+    if (rows == 0) return GNNAGG_OK;
+    if (x == nullptr || w == nullptr || y == nullptr || (fp8 && scales == nullptr))
+        return fail(GNNAGG_ERR_ARG, "%s: null pointer", what);
+    if ((residual == nullptr) != (h == nullptr))
+        return fail(GNNAGG_ERR_ARG, "%s: the residual and the sum's output come together", what);
+    if (ldx < F || ldy < F || (residual != nullptr && (ldr < F || ldh < F)) || (fp8 && lds < rows))
+        return fail(GNNAGG_ERR_ARG, "%s: a stride is smaller than its rows", what);
+    if (fp8 && (!aligned16(y) || ldy % 16 != 0))
+        return fail(GNNAGG_ERR_UNSUPPORTED, "%s: code rows start on 16 bytes", what);
+    const int size = type_size(type);
+    bool vec = F % (16 / size) == 0 && vec_rows(x, ldx, size) && aligned16(w) && (fp8 || vec_rows(y, ldy, size));
+    if (residual != nullptr) vec = vec && vec_rows(residual, ldr, size) && vec_rows(h, ldh, size);
+    const FwdParams p{x, residual, w, h, y, scales, rstd, ldx, ldr, ldh, ldy, lds, rows, F, w_type == kTypeF32, eps};
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+#define RMS_TYPE(T)                                                                                       \
+    [&] {                                                                                                 \
+        return fp8 ? (vec ? launch_fwd<T, true, true>(p, st) : launch_fwd<T, false, true>(p, st))         \
+                   : (vec ? launch_fwd<T, true, false>(p, st) : launch_fwd<T, false, false>(p, st));      \
+    }
+    return by_type(type, RMS_TYPE(float), RMS_TYPE(__nv_bfloat16), RMS_TYPE(__half));
+#undef RMS_TYPE
+}
+
+}  // namespace
+}  // namespace gnnagg
+
+using namespace gnnagg;
+
+extern "C" int gnnagg_rms_norm_fwd(const void *x, int64_t ldx, const void *residual, int64_t ldr, const void *w,
+                                   int32_t w_type, int64_t rows, int32_t F, int32_t type, float eps, void *h,
+                                   int64_t ldh, void *y, int64_t ldy, float *rstd, void *stream) {
+    return fwd("rms_norm_fwd", false, x, ldx, residual, ldr, w, w_type, rows, F, type, eps, h, ldh, y, ldy, nullptr, 0,
+               rstd, stream);
+}
+
+extern "C" int gnnagg_rms_norm_fp8(const void *x, int64_t ldx, const void *residual, int64_t ldr, const void *w,
+                                   int32_t w_type, int64_t rows, int32_t F, int32_t type, float eps, void *h,
+                                   int64_t ldh, uint8_t *codes, int64_t ldc, float *scales, int64_t lds, void *stream) {
+    return fwd("rms_norm_fp8", true, x, ldx, residual, ldr, w, w_type, rows, F, type, eps, h, ldh, codes, ldc, scales,
+               lds, nullptr, stream);
+}
+
+extern "C" size_t gnnagg_rms_norm_partial_bytes(int64_t rows, int32_t F, int32_t type) {
+    if (type_size(type) == 0 || rows < 0 || F <= 0 || F > kMaxWidth) return 0;
+    return (size_t)bwd_blocks(rows, F, type_size(type)) * (size_t)F * sizeof(float);
+}
+
+extern "C" int gnnagg_rms_norm_bwd(const void *gy, int64_t ldgy, const void *gh, int64_t ldgh, const void *h, int64_t ldh,
+                                   const float *rstd, const void *w, int32_t w_type, int64_t rows, int32_t F,
+                                   int32_t type, void *gx, int64_t ldgx, void *dw, float *partial, size_t partial_bytes,
+                                   void *stream) {
+    int rc = check_common("rms_norm_bwd", type, w_type, rows, F);
+    if (rc != GNNAGG_OK) return rc;
+    if (dw == nullptr || w == nullptr || (rows > 0 && (gy == nullptr || h == nullptr || rstd == nullptr || gx == nullptr ||
+                                                       partial == nullptr)))
+        return fail(GNNAGG_ERR_ARG, "rms_norm_bwd: null pointer");
+    if (rows > 0 && (ldgy < F || ldh < F || ldgx < F || (gh != nullptr && ldgh < F)))
+        return fail(GNNAGG_ERR_ARG, "rms_norm_bwd: a stride is smaller than its rows");
+    const int size = type_size(type), blocks = bwd_blocks(rows, F, size);
+    if (partial_bytes < gnnagg_rms_norm_partial_bytes(rows, F, type))
+        return fail(GNNAGG_ERR_SCRATCH, "rms_norm_bwd: partial-sum scratch too small");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (rows > 0) {
+        const bool vec = F % (16 / size) == 0 && vec_rows(gy, ldgy, size) && vec_rows(h, ldh, size) &&
+                         vec_rows(gx, ldgx, size) && (gh == nullptr || vec_rows(gh, ldgh, size)) && aligned16(w);
+        const BwdParams p{gy, gh, h, w, rstd, gx, partial, ldgy, ldgh, ldh, ldgx, rows, F, w_type == kTypeF32};
+#define RMS_TYPE(T) [&] { return vec ? launch_bwd<T, true>(p, blocks, st) : launch_bwd<T, false>(p, blocks, st); }
+        rc = by_type(type, RMS_TYPE(float), RMS_TYPE(__nv_bfloat16), RMS_TYPE(__half));
+#undef RMS_TYPE
+        if (rc != GNNAGG_OK) return rc;
+    }
+    return by_type(w_type, [&] { return launch_dw<float>(partial, blocks, F, dw, st); },
+                   [&] { return launch_dw<__nv_bfloat16>(partial, blocks, F, dw, st); },
+                   [&] { return launch_dw<__half>(partial, blocks, F, dw, st); });
+}

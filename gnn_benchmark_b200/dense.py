@@ -11,6 +11,11 @@ autograd nodes the models use; `wgrad(g, x)` is the weight gradient G^T X (a red
 into a small matrix) on the same tensor-core scheme.  Shapes the kernels do not take (more than 256
 output columns, operand rows not 16-byte aligned) go to cuBLAS: `supported()` / `wgrad_supported()`
 say which.
+
+The 8-bit form: `quantize_fp8` gives e4m3 codes with an fp32 scale for each block of 128 (1 x 128 or 128 x 128),
+`matmul_fp8` multiplies two such operands, `linear_fp8` is a differentiable linear layer whose three products
+(output, input gradient, weight gradient) all run that way.  `MODE = "fp8"` routes the models' transforms through
+the same products.
 """
 import warnings
 
@@ -19,15 +24,17 @@ import torch
 from . import _lib
 
 MAX_N = 256
-# "tf32x3": the tensor-core kernels wherever `supported()`.  Tests and the epoch benchmark set
-# "cublas" (torch's fp32 matmul) to have the library call the kernels replace measured beside them.
+# "tf32x3": the tensor-core kernels wherever `supported()`.  "fp8": the same transforms with operands rounded to
+# e4m3 in blocks of 128 (any width).  Tests and the epoch benchmark set "cublas" (torch's fp32 matmul) to have the
+# library call the kernels replace measured beside them.
 MODE = "tf32x3"
 
 _workspaces = {}
+_fp8_devices = set()  # devices that have run an 8-bit product, whose status check_status reads
 
 
 def enabled() -> bool:
-    return MODE == "tf32x3"
+    return MODE in ("tf32x3", "fp8")
 
 
 _warned = set()
@@ -124,6 +131,8 @@ def wgrad(g: torch.Tensor, x: torch.Tensor, out: torch.Tensor = None) -> torch.T
 
 def _matmul_tn(g: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
     """g.T @ x, tensor-core kernel when it takes the shapes, cuBLAS otherwise."""
+    if MODE == "fp8":
+        return matmul_fp8(*_quantize(g, 1, False, True)[2:], *_quantize(x, 1, False, True)[2:], out_dtype=torch.float32)
     if enabled() and wgrad_supported(g, x):
         return wgrad(g, x)
     _library_path("wgrad", (g.size(1), x.size(1)))
@@ -141,6 +150,15 @@ def check_status(device=None) -> None:
             raise RuntimeError(f"dense kernel (N={n}, K={k}) reported status {code}: "
                                + ("a bounded wait inside the kernel ran out" if code > 0 else
                                   _lib.lib().gnnagg_error_string(code).decode()))
+    for dev in sorted(_fp8_devices):
+        if device is not None and torch.device(device).index not in (None, dev):
+            continue
+        with torch.cuda.device(dev):
+            code = _lib.lib().gnnagg_fp8_matmul_status(_lib.stream_ptr())
+        if code != 0:
+            raise RuntimeError(f"8-bit product on device {dev} reported status {code}: "
+                               + ("a bounded wait inside the kernel ran out" if code > 0 else
+                                  _lib.lib().gnnagg_error_string(code).decode()))
 
 
 def clear_status(device=None) -> None:
@@ -149,6 +167,10 @@ def clear_status(device=None) -> None:
         if device is not None and torch.device(device).index not in (None, key[0]):
             continue
         _lib.check(_lib.lib().gnnagg_dense_status_clear(ws.data_ptr(), _lib.stream_ptr(ws.device)), "dense_status_clear")
+    for dev in sorted(_fp8_devices):
+        if device is None or torch.device(device).index in (None, dev):
+            with torch.cuda.device(dev):
+                _lib.check(_lib.lib().gnnagg_fp8_matmul_status_clear(_lib.stream_ptr()), "fp8_matmul_status_clear")
 
 
 def scale_rows(x: torch.Tensor, s: torch.Tensor, divide: bool = False, out: torch.Tensor = None,
@@ -188,6 +210,9 @@ class RowDivide_(torch.autograd.Function):
 
 def _matmul_nt(a: torch.Tensor, w: torch.Tensor, bias=None, out=None, accumulate=False) -> torch.Tensor:
     """a @ w.T (+bias), tensor-core kernel when it takes the shape, cuBLAS otherwise."""
+    if MODE == "fp8":
+        return matmul_fp8(*quantize_fp8(a), *quantize_fp8(w, (128, 128)), bias=bias, out=out, out_dtype=torch.float32,
+                          accumulate=accumulate)
     if enabled() and supported(a, w.size(0)):
         return linear(a, w, bias, out, accumulate)
     _library_path("linear", (w.size(0), a.size(1)))
@@ -207,7 +232,7 @@ def _tma_rows(g: torch.Tensor) -> torch.Tensor:
     """`g` itself when its rows are 16-byte addressable, else a copy whose rows are padded with zero
     columns to a multiple of 4 (an upstream gradient of 47 columns has 188-byte rows, which TMA cannot
     address; the extra columns meet zero rows of the weight / are dropped from the weight gradient)."""
-    if not enabled() or not g.is_cuda or g.dim() != 2 or g.size(1) % 4 == 0 or g.size(1) > MAX_N - 3:
+    if MODE != "tf32x3" or not g.is_cuda or g.dim() != 2 or g.size(1) % 4 == 0 or g.size(1) > MAX_N - 3:
         return g
     pad = torch.zeros(g.size(0), (g.size(1) + 3) // 4 * 4, dtype=g.dtype, device=g.device)
     pad[:, :g.size(1)] = g
@@ -285,3 +310,153 @@ class SageDense(torch.autograd.Function):
         if ctx.needs_input_grad[3]:
             g_ws = _weight_grad(g, x, n_out)
         return g_aggr, g_x, g_wn, g_ws, g_b
+
+
+# ---------------------------------------------------------------------------------------------- 8-bit products
+
+FP8 = torch.float8_e4m3fn
+FP8_BLOCK = 128
+
+
+def _quantize(x: torch.Tensor, block_rows: int, rows: bool, cols: bool):
+    """(codes, scales, codes_t, scales_t) of x from one read; the pair that is not asked for is None, None."""
+    if x.dim() != 2 or x.dtype not in _lib.TYPES:
+        raise RuntimeError(f"quantize_fp8: x must be a float32, bfloat16 or float16 matrix, not {tuple(x.shape)} {x.dtype}")
+    _lib.require_cuda(x)
+    m, k = x.shape
+    if x.stride(1) != 1 or x.stride(0) < k:
+        x = x.contiguous()
+    high = (m + 127) // 128 if block_rows == 128 else m
+    wide = (k + 127) // 128 if block_rows == 128 else k
+    codes = scales = codes_t = scales_t = None
+    args, args_t = (0, 0, 0, 0), (0, 0, 0, 0)
+    if rows:
+        codes, scales = _lib.empty_codes(m, k, x.device)
+        scales = scales if high == m else torch.empty(((k + 127) // 128, high), dtype=torch.float32, device=x.device).t()
+        args = (codes.data_ptr(), codes.stride(0), scales.data_ptr(), high)
+    if cols:
+        codes_t, scales_t = _lib.empty_codes(k, m, x.device)
+        scales_t = scales_t if wide == k else torch.empty(((m + 127) // 128, wide), dtype=torch.float32, device=x.device).t()
+        args_t = (codes_t.data_ptr(), codes_t.stride(0), scales_t.data_ptr(), wide)
+    with _lib.device_of(x):
+        rc = _lib.lib().gnnagg_fp8_quantize(x.data_ptr(), max(x.stride(0), k), m, k, _lib.TYPES[x.dtype], block_rows, *args, *args_t,
+                                            _lib.stream_ptr(x.device))
+    _lib.check(rc, "fp8_quantize")
+    return codes, scales, codes_t, scales_t
+
+
+def quantize_fp8(x: torch.Tensor, block=(1, 128), transpose: bool = False):
+    """(codes, scales) of x (rows, cols) float32, bfloat16 or float16.
+
+    codes: float8_e4m3fn of x's shape, rows padded to 16 bytes in memory.  scales: float32, one for each block of
+    (1, 128) elements, shape (rows, ceil(cols / 128)), or of (128, 128), shape (ceil(rows / 128), ceil(cols / 128)).
+    An element's value is code * scale.  scale = a * (1 / 448) with a the block's largest magnitude (at least 2^-96),
+    code = e4m3(x * (448 * (1 / a))).  transpose=True gives the codes and scales of x.T without forming it.  A block
+    that holds a NaN or an infinity reads back as NaN."""
+    if tuple(block) not in ((1, 128), (128, 128)):
+        raise RuntimeError(f"quantize_fp8: block must be (1, 128) or (128, 128), not {block}")
+    r = _quantize(x, block[0], not transpose, transpose)
+    return r[2:] if transpose else r[:2]
+
+
+def _operand(name: str, codes: torch.Tensor, scales: torch.Tensor, device):
+    """(rows that a scale covers, row stride) of a checked operand."""
+    if codes.dim() != 2 or codes.dtype != FP8 or codes.device != device:
+        raise RuntimeError(f"matmul_fp8: {name} must be a float8_e4m3fn matrix on the operands' device")
+    rows, k = codes.shape
+    ld = codes.stride(0) if rows > 1 and k > 0 else (k + 15) // 16 * 16 + 16
+    if rows > 0 and k > 0 and (codes.stride(1) != 1 and k > 1 or ld < k or ld % 16 != 0 or codes.data_ptr() % 16 != 0):
+        raise RuntimeError(f"matmul_fp8: {name}'s rows must be contiguous and start on 16 bytes (as quantize_fp8 lays them)")
+    kb = (k + 127) // 128
+    if scales.dim() != 2 or scales.dtype != torch.float32 or scales.device != device or scales.size(1) != kb \
+            or scales.size(0) not in (rows, (rows + 127) // 128):
+        raise RuntimeError(f"matmul_fp8: {name}'s scales must be float32 ({rows} or {(rows + 127) // 128}, {kb}), "
+                           f"not {tuple(scales.shape)} {scales.dtype}")
+    return (1 if scales.size(0) == rows else 128), ld
+
+
+def matmul_fp8(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor,
+               bias: torch.Tensor = None, out: torch.Tensor = None, out_dtype: torch.dtype = torch.bfloat16,
+               accumulate: bool = False) -> torch.Tensor:
+    """out (M, N) (+)= (a * a_scales) @ (b * b_scales).T (+ bias): a (M, K) and b (N, K) float8_e4m3fn with float32
+    scales for each block of 128 along K, one per row, (rows, ceil(K / 128)), or per 128 rows.  out_dtype float32,
+    bfloat16 or float16 (out's type when out is given); bias float32 (N,); accumulate needs a float32 out."""
+    _lib.require_cuda(a, a_scales, b, b_scales, bias, out)
+    device = a.device
+    a_block, lda = _operand("a", a, a_scales, device)
+    b_block, ldb = _operand("b", b, b_scales, device)
+    m, k = a.shape
+    n = b.size(0)
+    if b.size(1) != k:
+        raise RuntimeError(f"matmul_fp8: shape mismatch a={tuple(a.shape)} b={tuple(b.shape)}")
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,) or not bias.is_contiguous()
+                             or bias.device != device):
+        raise RuntimeError("matmul_fp8: bias must be a contiguous float32 vector of N elements on the operands' device")
+    if out is None:
+        if accumulate:
+            raise RuntimeError("matmul_fp8: accumulate needs an output to accumulate into")
+        if out_dtype not in _lib.TYPES:
+            raise RuntimeError("matmul_fp8: out_dtype must be float32, bfloat16 or float16")
+        out = torch.empty((m, n), dtype=out_dtype, device=device)
+    elif out.shape != (m, n) or out.dtype not in _lib.TYPES or out.device != device \
+            or (out.numel() > 0 and (out.stride(1) != 1 and n > 1 or out.stride(0) < n)):
+        raise RuntimeError("matmul_fp8: out must be (M, N) float32, bfloat16 or float16 with contiguous rows")
+    if accumulate and out.dtype != torch.float32:
+        raise RuntimeError("matmul_fp8: accumulate needs a float32 output")
+    lib = _lib.lib()
+    ws_bytes = lib.gnnagg_fp8_matmul_workspace_bytes(m, n, k)
+    # from the caching allocator at every call: ordered with the stream, and a captured graph has its own
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes else None
+    _fp8_devices.add(device.index)
+    with _lib.device_of(a):
+        rc = lib.gnnagg_fp8_matmul(a.data_ptr(), lda, a_scales.data_ptr(), a_scales.stride(0), a_scales.stride(1),
+                                   a_block, b.data_ptr(), ldb, b_scales.data_ptr(), b_scales.stride(0),
+                                   b_scales.stride(1), b_block, m, n, k, _lib.ptr(bias), 1 if accumulate else 0,
+                                   out.data_ptr(), max(out.stride(0), n), _lib.TYPES[out.dtype], _lib.ptr(ws), ws_bytes,
+                                   _lib.stream_ptr(device))
+    _lib.check(rc, "fp8_matmul")
+    return out
+
+
+class LinearFP8(torch.autograd.Function):
+    """y = x @ W^T (+ b) with e4m3 operands in all three products.  x and the output's gradient are rounded in blocks
+    of 1 x 128 along the sum they enter (columns for y and the input gradient, rows for the weight gradient), the
+    weight in blocks of 128 x 128.  What is kept for the backward is 8-bit: x's transposed codes and the weight's."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+        xq, xs, xt, xts = _quantize(x, 1, True, need_w)
+        wq, ws, wt, wts = _quantize(weight, 128, True, need_x)
+        ctx.save_for_backward(xt, xts, wt, wts)
+        ctx.types = x.dtype, weight.dtype, None if bias is None else bias.dtype
+        return matmul_fp8(xq, xs, wq, ws, bias=None if bias is None else bias.float(), out_dtype=x.dtype)
+
+    @staticmethod
+    def backward(ctx, g):
+        xt, xts, wt, wts = ctx.saved_tensors
+        x_type, w_type, b_type = ctx.types
+        need_x, need_w, need_b = ctx.needs_input_grad
+        gx = gw = gb = None
+        if need_b:
+            gb = g.sum(0, dtype=torch.float32).to(b_type)
+        if need_x or need_w:
+            gq, gs, gt, gts = _quantize(g, 1, need_x, need_w)
+        if need_x:
+            gx = matmul_fp8(gq, gs, wt, wts, out_dtype=x_type)
+        if need_w:
+            gw = matmul_fp8(gt, gts, xt, xts, out_dtype=w_type)
+        return gx, gw, gb
+
+
+def linear_fp8(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor = None) -> torch.Tensor:
+    """x (M, K) @ weight (N, K).T (+ bias (N,)) with operands rounded to e4m3 in blocks of 128, in the forward and in
+    both gradients; sums in float32, the output in x's type.  float32, bfloat16 or float16."""
+    _lib.require_cuda(x, weight, bias)
+    if x.dim() != 2 or weight.dim() != 2 or x.size(1) != weight.size(1):
+        raise RuntimeError(f"linear_fp8: shape mismatch x={tuple(x.shape)} weight={tuple(weight.shape)}")
+    if x.dtype not in _lib.TYPES or weight.dtype not in _lib.TYPES or weight.device != x.device:
+        raise RuntimeError("linear_fp8: x and weight must be float32, bfloat16 or float16 on one device")
+    if bias is not None and (bias.shape != (weight.size(0),) or bias.dtype not in _lib.TYPES or bias.device != x.device):
+        raise RuntimeError("linear_fp8: bias must be a float32, bfloat16 or float16 vector of N elements on x's device")
+    return LinearFP8.apply(x, weight, bias)

@@ -16,7 +16,7 @@ import torch.nn.functional as F
 from torch import Tensor
 from torch.nn import LayerNorm, Linear, Parameter
 
-from . import dense, norm
+from . import dense, norm, optim
 from .aggregator import Aggregator
 
 
@@ -168,7 +168,9 @@ class DistGCN(torch.nn.Module):
 
 def create_model_and_optimizer(config: dict, device=None):
     """model/utils.py:8-29 of the reference: build, reset_parameters, DDP when world_size > 1, Adam.
-    Weights are drawn on the CPU (so a seed gives the reference's initial weights) and then moved."""
+    Weights are drawn on the CPU (so a seed gives the reference's initial weights) and then moved.
+    config["optimizer"]: "adam" (the reference's, the default) or "adamw" (`optim.AdamW`, with
+    config["optimizer_state_bits"] 32 or 8)."""
     cls = {"sage": DistSAGE, "gcn": DistGCN}.get(config["model_name"])
     if cls is None:
         return None, None
@@ -179,7 +181,14 @@ def create_model_and_optimizer(config: dict, device=None):
         model = model.to(device)
     if dist.is_available() and dist.is_initialized() and dist.get_world_size() > 1:
         model = torch.nn.parallel.DistributedDataParallel(model)
-    optimizer = torch.optim.Adam(model.parameters(), lr=config["lr"], weight_decay=config["weight_decay"])
+    kind = config.get("optimizer", "adam")
+    if kind == "adam":
+        optimizer = torch.optim.Adam(model.parameters(), lr=config["lr"], weight_decay=config["weight_decay"])
+    elif kind == "adamw":
+        optimizer = optim.AdamW(model.parameters(), lr=config["lr"], weight_decay=config["weight_decay"],
+                                state_bits=config.get("optimizer_state_bits", 32))
+    else:
+        raise ValueError(f"unknown optimizer {kind!r}: adam or adamw")
     return model, optimizer
 
 

@@ -1,0 +1,201 @@
+"""AdamW over many tensors at once, with moments in 32 or 8 bits.
+
+The reference trains with torch.optim.Adam (self_benchmark/a64fx/model/utils.py:24), a loop of element-wise passes
+over every parameter.  Here one kernel launch updates up to 500 tensors: `adamw_step` is the plain call on lists of
+tensors, `AdamW` the torch.optim.Optimizer around it.
+
+8-bit moments (`state_bits=8`) take 2.03 bytes a parameter instead of 8: e4m3 codes of the first moment and of the
+second moment's square root, in blocks of 256 elements with an fp32 scale each.
+"""
+import ctypes
+
+import torch
+
+from . import _lib
+
+STATE_BLOCK = 256
+FP8 = torch.float8_e4m3fn
+
+
+class _Tensor(ctypes.Structure):
+    _fields_ = [("param", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("exp_avg", ctypes.c_void_p),
+                ("exp_avg_sq", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("master", ctypes.c_void_p),
+                ("n", ctypes.c_int64)]
+
+
+def _check(what, i, t, n, dtype, device):
+    if t.numel() != n or t.dtype != dtype or t.device != device or not t.is_contiguous():
+        raise RuntimeError(f"adamw_step: {what} {i} must be a contiguous {dtype} tensor of {n} elements on the "
+                           f"parameters' device, not {tuple(t.shape)} {t.dtype} on {t.device}")
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr: float, betas=(0.9, 0.999), eps: float = 1e-8,
+               weight_decay: float = 1e-2, scales=None, masters=None, device_scalars: torch.Tensor = None) -> None:
+    """One AdamW step over lists of tensors, in place:
+
+        m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2
+        p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+
+    params, grads: one type (float32, bfloat16 or float16), contiguous, on one device.  exp_avgs, exp_avg_sqs:
+    float32, or float8_e4m3fn codes of m and of sqrt(v) with `scales`, (ceil(n / 256), 2) float32 per tensor.
+    masters: for 16-bit parameters, float32 copies (None where there is none) that are updated and that the
+    parameters are rounded from.  step: t, from 1.  device_scalars: what `AdamW(capturable=True)` keeps on the device
+    instead of step and lr.  No two tensors may overlap."""
+    count = len(params)
+    if not (len(grads) == len(exp_avgs) == len(exp_avg_sqs) == count) or (scales is not None and len(scales) != count) \
+            or (masters is not None and len(masters) != count):
+        raise RuntimeError("adamw_step: the lists must have one entry per parameter")
+    b1, b2 = betas
+    if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
+        raise RuntimeError(f"adamw_step: betas must be in [0, 1), not {betas}")
+    if device_scalars is None and step < 1:
+        raise RuntimeError("adamw_step: the first step is 1")
+    if count == 0:
+        return
+    device, dtype = params[0].device, params[0].dtype
+    _lib.require_cuda(params[0])
+    if dtype not in _lib.TYPES:
+        raise RuntimeError(f"adamw_step: parameters must be float32, bfloat16 or float16, not {dtype}")
+    state = torch.float32 if scales is None else FP8
+    rows = []
+    for i in range(count):
+        p, g, m, v = params[i], grads[i], exp_avgs[i], exp_avg_sqs[i]
+        n = p.numel()
+        _check("parameter", i, p, n, dtype, device)
+        _check("gradient", i, g, n, dtype, device)
+        _check("exp_avg", i, m, n, state, device)
+        _check("exp_avg_sq", i, v, n, state, device)
+        s = w = 0
+        if scales is not None:
+            _check("scales", i, scales[i], (n + STATE_BLOCK - 1) // STATE_BLOCK * 2, torch.float32, device)
+            s = scales[i].data_ptr()
+        if masters is not None and masters[i] is not None:
+            _check("master", i, masters[i], n, torch.float32, device)
+            w = masters[i].data_ptr()
+        rows.append((p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), s, w, n))
+    table = (_Tensor * count)(*rows)
+    with _lib.device_of(params[0]):
+        rc = _lib.lib().gnnagg_adamw_step(table, count, _lib.TYPES[dtype], 32 if scales is None else 8, lr, b1, b2, eps,
+                                          weight_decay, step, _lib.ptr(device_scalars), _lib.stream_ptr(device))
+    _lib.check(rc, "adamw_step")
+
+
+def _zero_moment(bits: int, like: torch.Tensor) -> torch.Tensor:
+    dtype = torch.float32 if bits == 32 else torch.uint8
+    t = torch.zeros_like(like, dtype=dtype, memory_format=torch.contiguous_format)
+    return t if bits == 32 else t.view(FP8)
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW (decoupled weight decay) whose step is one launch for all parameters of one type in a group.
+
+    state_bits: 32, or 8 for block-quantised moments.  master_weights: keep a float32 copy of 16-bit parameters and
+    round the parameter from it at every step.  capturable: the step count lives on the device, so that `step()` can
+    be captured into a CUDA graph and replayed; `lr` may then be a 0-dim float32 CUDA tensor that the caller changes
+    between replays.  Parameters are dense float32, bfloat16 or float16 CUDA tensors, and contiguous."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
+                 state_bits: int = 32, master_weights: bool = False, capturable: bool = False):
+        if not isinstance(lr, torch.Tensor) and lr < 0.0:
+            raise ValueError(f"AdamW: negative learning rate {lr}")
+        if isinstance(lr, torch.Tensor) and not (capturable and lr.is_cuda and lr.dim() == 0 and lr.dtype == torch.float32):
+            raise ValueError("AdamW: a tensor lr must be a 0-dim float32 CUDA tensor and needs capturable=True")
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+            raise ValueError(f"AdamW: betas must be in [0, 1), not {betas}")
+        if eps < 0.0 or weight_decay < 0.0:
+            raise ValueError("AdamW: eps and weight_decay must not be negative")
+        if state_bits not in (8, 32):
+            raise ValueError(f"AdamW: state_bits must be 8 or 32, not {state_bits}")
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
+                                      master_weights=master_weights, capturable=capturable))
+
+    def load_state_dict(self, state_dict) -> None:
+        """As torch's, but the moments keep the types they were saved in (torch would cast them to the parameter's)."""
+        super().load_state_dict(state_dict)
+        saved = state_dict["state"]
+        for mine, theirs in zip(self.param_groups, state_dict["param_groups"]):
+            shared = {}  # one count on the device for all parameters that agree on it
+            for p, key in zip(mine["params"], theirs["params"]):
+                if key not in saved:
+                    continue
+                state = {k: v.detach().to(p.device, copy=True) if isinstance(v, torch.Tensor) else v
+                         for k, v in saved[key].items()}
+                step = int(state["step"])
+                if mine["capturable"]:
+                    step = shared.setdefault((p.device, step), torch.tensor(step, dtype=torch.int64, device=p.device))
+                state["step"] = step
+                self.state[p] = state
+
+    def _new_state(self, p, group, fresh) -> dict:
+        n, bits = p.numel(), group["state_bits"]
+        state = {"step": 0, "exp_avg": _zero_moment(bits, p), "exp_avg_sq": _zero_moment(bits, p)}
+        if group["capturable"]:  # parameters that begin together share a count
+            if p.device not in fresh:
+                fresh[p.device] = torch.zeros((), dtype=torch.int64, device=p.device)
+            state["step"] = fresh[p.device]
+        if bits == 8:
+            state["scales"] = torch.zeros(((n + STATE_BLOCK - 1) // STATE_BLOCK, 2), dtype=torch.float32, device=p.device)
+        if group["master_weights"] and p.dtype != torch.float32:
+            state["master"] = p.detach().to(torch.float32, memory_format=torch.contiguous_format)
+        self.state[p] = state
+        return state
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
+        for group in self.param_groups:
+            if capturing and not group["capturable"]:
+                raise RuntimeError("AdamW: a step that is captured into a graph needs capturable=True")
+            fresh, calls = {}, {}  # calls: (device, count) -> type -> members
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                _lib.require_cuda(p, p.grad)
+                if p.grad.is_sparse or not p.is_contiguous():
+                    raise RuntimeError("AdamW: parameters must be contiguous, gradients dense")
+                state = self.state[p]
+                if not state:
+                    if capturing:
+                        raise RuntimeError("AdamW: take one step before capturing (it creates the moments)")
+                    state = self._new_state(p, group, fresh)
+                if group["capturable"]:
+                    key = (p.device, id(state["step"]))
+                else:
+                    state["step"] += 1
+                    key = (p.device, state["step"])
+                calls.setdefault(key, {}).setdefault(p.dtype, []).append((p, state))
+            for (device, count), by_type in calls.items():
+                scalars = None
+                if group["capturable"]:
+                    scalars = self._tick(group, device, next(iter(by_type.values()))[0][1]["step"])
+                for members in by_type.values():
+                    self._update(group, members, 0 if group["capturable"] else count, scalars)
+        return loss
+
+    @staticmethod
+    def _tick(group, device, step):
+        """Counts a step on the device and returns its scalars."""
+        lib, lr, (b1, b2) = _lib.lib(), group["lr"], group["betas"]
+        lr_ptr, host_lr = (lr.data_ptr(), 0.0) if isinstance(lr, torch.Tensor) else (0, float(lr))
+        scalars = torch.empty(lib.gnnagg_adamw_scalars_bytes(), dtype=torch.uint8, device=device)
+        with _lib.device_of(scalars):
+            rc = lib.gnnagg_adamw_tick(step.data_ptr(), lr_ptr, host_lr, b1, b2, group["eps"], group["weight_decay"],
+                                       scalars.data_ptr(), _lib.stream_ptr(device))
+        _lib.check(rc, "adamw_tick")
+        return scalars
+
+    @staticmethod
+    def _update(group, members, step, scalars):
+        states = [s for _, s in members]
+        adamw_step([p for p, _ in members],
+                   [p.grad if p.grad.is_contiguous() else p.grad.contiguous() for p, _ in members],
+                   [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states], step=step,
+                   lr=0.0 if scalars is not None else group["lr"], betas=group["betas"], eps=group["eps"],
+                   weight_decay=group["weight_decay"],
+                   scales=[s["scales"] for s in states] if group["state_bits"] == 8 else None,
+                   masters=[s.get("master") for s in states] if group["master_weights"] else None,
+                   device_scalars=scalars)

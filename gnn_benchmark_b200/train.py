@@ -93,6 +93,7 @@ def main():
     Quantizer_for_all_procs(world_size, config["num_bits"])
     config["input_dir"] += "{}_{}_part/".format(config["graph_name"], world_size)
     device = torch.device("cuda", torch.cuda.current_device())
+    dense.MODE = config.get("dense_mode", dense.MODE)  # "fp8": the layers' transforms with 8-bit operands
     set_random_seed(config["random_seed"])
     model, optimizer = create_model_and_optimizer(config, device)
     data = load_data(config)

@@ -12,8 +12,9 @@
  *   - return value: 0 = ok, < 0 = argument / launch error found on the host
  *     (see gnnagg_error_string), never a device trap;
  *   - safe to call from one host thread per GPU; the library keeps no global state
- *     apart from a thread-local message for the last error and the built-in scratch
- *     buffer of gnnagg_spmm_csr_f32_static_scratch.
+ *     apart from a thread-local message for the last error, the built-in scratch
+ *     buffer of gnnagg_spmm_csr_f32_static_scratch and the status word of
+ *     gnnagg_fp8_matmul_status.
  */
 #ifndef GNNAGG_H
 #define GNNAGG_H
@@ -30,6 +31,11 @@ extern "C" {
 #define GNNAGG_ERR_UNSUPPORTED (-2) /* shape outside what the kernels are built for   */
 #define GNNAGG_ERR_CUDA (-3)        /* cudaGetLastError() after the launch was not ok */
 #define GNNAGG_ERR_SCRATCH (-4)     /* plan / scratch buffer too small or malformed   */
+
+/* Element types of the low-precision entry points. */
+#define GNNAGG_F32 0
+#define GNNAGG_BF16 1
+#define GNNAGG_F16 2
 
 /* Library version (major*10000 + minor*100 + patch). */
 int gnnagg_version(void);
@@ -333,6 +339,106 @@ int gnnagg_relu_dropout_fwd(const float *X, int64_t ldx, int64_t rows, int32_t F
                             float *Y, int64_t ldy, uint8_t *mask, void *stream);
 int gnnagg_relu_dropout_bwd(const float *GY, int64_t ldg, const uint8_t *mask, int64_t rows, int32_t F, float p_drop,
                             float *GX, int64_t ldgx, void *stream);
+
+/* ------------------------------------------------------------------------------------
+ * L1  root-mean-square norm with the residual's addition (no reference counterpart)
+ *
+ *     h = x + residual (rounded to the rows' type; h is what the norm is taken of)
+ *     y = h * r * w,  r = rsqrt(mean(h^2) + eps)
+ *
+ *   type      GNNAGG_F32 / BF16 / F16 of x, residual, h, y (and their gradients); w_type: the same or F32
+ *   residual  NULL: h = x, and h must be NULL too;  h may alias x or residual, y may alias x
+ *   rstd      rows floats r, for the backward; NULL in inference
+ *   F <= 16384; any alignment and strides of at least F elements (16-byte accesses where all rows allow them)
+ * gnnagg_rms_norm_fp8 writes e4m3 codes and a scale per row and 128 columns instead of y: with t = h * w and
+ * a = max(max |t| of the group, 2^-96), code = e4m3(t * (448 * (1 / a))), scale = a * (1 / 448) * r.  Code rows
+ * start on 16 bytes (ldc % 16 == 0; the padding behind column F is overwritten with zeros up to the next 8);
+ * the scale of (row, group j) is scales[row + j * lds].
+ * gnnagg_rms_norm_bwd: gx = gh + r * (w gy - hat * mean(w gy hat)) with hat = h r (gh may be NULL, gx may alias gy
+ * or gh) is the gradient of x and of the residual; dw = sum over the rows of gy * hat, of w's type, added up in a
+ * fixed order through `partial` (gnnagg_rms_norm_partial_bytes bytes).
+ * ---------------------------------------------------------------------------------- */
+int gnnagg_rms_norm_fwd(const void *x, int64_t ldx, const void *residual, int64_t ldr, const void *w, int32_t w_type,
+                        int64_t rows, int32_t F, int32_t type, float eps, void *h, int64_t ldh, void *y, int64_t ldy,
+                        float *rstd, void *stream);
+int gnnagg_rms_norm_fp8(const void *x, int64_t ldx, const void *residual, int64_t ldr, const void *w, int32_t w_type,
+                        int64_t rows, int32_t F, int32_t type, float eps, void *h, int64_t ldh, uint8_t *codes,
+                        int64_t ldc, float *scales, int64_t lds, void *stream);
+size_t gnnagg_rms_norm_partial_bytes(int64_t rows, int32_t F, int32_t type);
+int gnnagg_rms_norm_bwd(const void *gy, int64_t ldgy, const void *gh, int64_t ldgh, const void *h, int64_t ldh,
+                        const float *rstd, const void *w, int32_t w_type, int64_t rows, int32_t F, int32_t type,
+                        void *gx, int64_t ldgx, void *dw, float *partial, size_t partial_bytes, void *stream);
+
+/* ------------------------------------------------------------------------------------
+ * L2  e4m3 codes with block scales, and their matrix product (no reference counterpart)
+ *
+ * gnnagg_fp8_quantize: x[rows, cols] of `type` -> codes with one scale per block of block_rows x 128 elements
+ * (block_rows 1 or 128).  a = max(max |x| of the block, 2^-96), scale = a * (1 / 448), code = e4m3(x * (448 * (1 / a))),
+ * each step rounded to nearest in fp32.  A block that holds a NaN or an infinity reads back as NaN.
+ *   codes    [rows][ldc] with scales[i + j * lds] (i: row or row block, j: column group), and / or
+ *   codes_t  [cols][ldt], the same for the transpose: blocks of 1 x 128 lie along x's columns.
+ *   Code rows start on 16 bytes (ldc, ldt % 16 == 0); the padding behind a row is partly overwritten with zeros.
+ *
+ * gnnagg_fp8_matmul: C[M,N] = sum_k A[m,k] sa[m,k/128] B[n,k] sb[n,k/128] (+ bias[N]) (+ C).
+ *   a_block, b_block  rows that a scale covers: 1 or 128; the scale of (row or row block i, k-block j) is
+ *             sa[i * sa_stride + j * sa_stride_k]
+ *   out_type  GNNAGG_F32 / BF16 / F16; accumulate needs F32
+ *   workspace gnnagg_fp8_matmul_workspace_bytes(M, N, K) bytes, 16-byte aligned; NULL when that is 0.  Its contents
+ *             mean nothing between calls.
+ * Sums are fp32: chains of 128 elements in tensor memory, their scaled sum in registers; a sum that is split over
+ * CTAs is joined in a fixed order.
+ * gnnagg_fp8_matmul_status synchronises the stream and returns 0, or the positive code of the first wait that ran
+ * out inside a kernel on the current device (codes as for gnnagg_dense_status; the output is then undefined);
+ * gnnagg_fp8_matmul_status_clear resets it.  gnnagg_dense_stall_test covers these launches too.
+ * ---------------------------------------------------------------------------------- */
+int gnnagg_fp8_quantize(const void *x, int64_t ldx, int64_t rows, int64_t cols, int32_t type, int32_t block_rows,
+                        uint8_t *codes, int64_t ldc, float *scales, int64_t lds, uint8_t *codes_t, int64_t ldt,
+                        float *scales_t, int64_t lds_t, void *stream);
+size_t gnnagg_fp8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int gnnagg_fp8_matmul(const uint8_t *A, int64_t lda, const float *sa, int64_t sa_stride, int64_t sa_stride_k,
+                      int32_t a_block, const uint8_t *B, int64_t ldb, const float *sb, int64_t sb_stride,
+                      int64_t sb_stride_k, int32_t b_block, int64_t M, int64_t N, int64_t K, const float *bias,
+                      int32_t accumulate, void *C, int64_t ldc, int32_t out_type, void *workspace,
+                      size_t workspace_bytes, void *stream);
+int gnnagg_fp8_matmul_status(void *stream);
+int gnnagg_fp8_matmul_status_clear(void *stream);
+
+/* ------------------------------------------------------------------------------------
+ * L3  AdamW over many tensors in one launch (no reference counterpart; the reference's optimiser is
+ *     torch.optim.Adam, model/utils.py:24)
+ *
+ *     m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2
+ *     p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+ *
+ *   tensors     HOST array of `count` entries; pointers inside are device pointers.  It is read before the call
+ *               returns and travels in the launch's parameters.
+ *   type        GNNAGG_F32 / BF16 / F16 of parameters and gradients
+ *   state_bits  32: exp_avg, exp_avg_sq are fp32.  8: they are e4m3 codes of m and of sqrt(v) in blocks of 256
+ *               elements, scales[2 b], scales[2 b + 1] the scales of block b (8-byte aligned); code =
+ *               e4m3(u * (448 * (1 / a))), a = max(max |u|, 2^-96), scale = a * (1 / 448), the code of sqrt(v) at least
+ *               2^-9 where v > 0.  A non-finite gradient makes its block read back as NaN.
+ *   master      fp32 copy that is updated and that `param` is rounded from; NULL: param itself is updated
+ *   step        t, from 1; ignored when device_scalars is given
+ *   device_scalars  what gnnagg_adamw_tick left: that call adds 1 to *step and writes the step's scalars
+ *               (gnnagg_adamw_scalars_bytes bytes, 16-byte aligned) on the device, so that a replayed graph counts
+ *               its steps; lr (a device fp32) overrides host_lr when not NULL.
+ * No two tensors of a call may overlap.
+ * ---------------------------------------------------------------------------------- */
+typedef struct {
+    void *param;
+    const void *grad;
+    void *exp_avg;
+    void *exp_avg_sq;
+    float *scales;
+    float *master;
+    int64_t n;
+} gnnagg_adamw_tensor;
+size_t gnnagg_adamw_scalars_bytes(void);
+int gnnagg_adamw_tick(int64_t *step, const float *lr, double host_lr, double beta1, double beta2, double eps,
+                      double weight_decay, void *scalars, void *stream);
+int gnnagg_adamw_step(const gnnagg_adamw_tensor *tensors, int64_t count, int32_t type, int32_t state_bits, double lr,
+                      double beta1, double beta2, double eps, double weight_decay, int64_t step,
+                      const void *device_scalars, void *stream);
 
 #ifdef __cplusplus
 }

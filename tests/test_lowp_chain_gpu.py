@@ -1,0 +1,152 @@
+"""The low-precision operators together, as a model uses them: norm -> 8-bit operand -> product in inference, a
+residual block trained with the 8-bit linear layer, the norm and AdamW, and the framework's own layers and training
+entry with `dense.MODE = "fp8"` and the "adamw" optimiser.  Every stage is held to its definition in 64 bits, on the
+values that the stage before it produced."""
+import pytest
+import torch
+
+from lowp_ref import floor, quantise, unit, values
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def _room(a64, b64):  # as derived in test_fp8_gpu.py
+    return (4 * 33 * 2.0 ** -23 + ((a64.size(1) + 127) // 128 + 80) * U) * (a64.abs() @ b64.abs().t())
+
+
+def _close(got, a, b, extra=0):
+    ref = a @ b.t() + extra
+    assert ((got.double() - ref).abs() <= _room(a, b) + (unit(got.dtype) + 2 * U) * ref.abs() + floor(got.dtype)).all()
+
+
+@pytest.mark.parametrize("rows", [1, 5, 300])
+def test_inference_block(rows):
+    """A token's (or a batch's) way through a residual block: two normed 8-bit products, nothing else in between."""
+    from gnn_benchmark_b200 import dense, norm
+
+    torch.manual_seed(rows)
+    f, wide = 384, 1000
+    x = torch.randn(rows, f, device="cuda", dtype=torch.bfloat16)
+    stream = torch.randn(rows, f, device="cuda", dtype=torch.bfloat16)
+    w = torch.rand(f, device="cuda").bfloat16() + 0.5
+    w2 = torch.rand(wide, device="cuda").bfloat16() + 0.5
+    up = dense.quantize_fp8(torch.randn(wide, f, device="cuda") / f ** 0.5, (128, 128))
+    down = dense.quantize_fp8(torch.randn(f, wide, device="cuda") / wide ** 0.5, (128, 128))
+    codes, scales, h = norm.rms_norm_fp8(x, w, residual=stream)
+    a = dense.matmul_fp8(codes, scales, *up)
+    _close(a, values(codes, scales), values(*up))
+    codes2, scales2 = norm.rms_norm_fp8(a, w2)
+    b = dense.matmul_fp8(codes2, scales2, *down)
+    _close(b, values(codes2, scales2), values(*down))
+    y, h2 = norm.rms_norm(b, w, residual=h)
+    assert torch.equal(h2, (b.double() + h.double()).bfloat16())
+    dense.check_status()
+
+
+def test_train_block():
+    """Gradients of norm and 8-bit layer chained through a residual block, then one AdamW step with 8-bit moments."""
+    from gnn_benchmark_b200 import dense, norm, optim
+
+    torch.manual_seed(3)
+    rows, f, n = 700, 200, 130
+    x = torch.randn(rows, f, device="cuda", requires_grad=True)
+    res = torch.randn(rows, f, device="cuda", requires_grad=True)
+    w = (torch.rand(f, device="cuda") + 0.5).requires_grad_(True)
+    up = (torch.randn(n, f, device="cuda") / f ** 0.5).requires_grad_(True)
+    bias = torch.randn(n, device="cuda", requires_grad=True)
+    y, h = norm.rms_norm(x, w, residual=res)
+    z = dense.linear_fp8(y, up, bias)
+    for t in (y, h, z):
+        t.retain_grad()
+    (z.square().sum() + h.square().sum()).backward()
+    dense.check_status()
+    _close(z, values(*quantise(y)), values(*quantise(up, 128)), bias.double())
+    assert torch.equal(z.grad, 2 * z) and torch.equal(h.grad, 2 * h)
+    _close(y.grad, values(*quantise(z.grad)), values(*quantise(up.t(), 128)))
+    _close(up.grad, values(*quantise(z.grad.t())), values(*quantise(y.t())))
+    hd = h.double()
+    rms = (hd.square().mean(1, keepdim=True) + 1e-6).sqrt()
+    hat = hd / rms
+    a = y.grad.double() * w.double()
+    want = (a - hat * (a * hat).mean(1, keepdim=True)) / rms + h.grad.double()
+    room = (a.abs() + hat.abs() * (a * hat).abs().mean(1, keepdim=True)) / rms + h.grad.double().abs()
+    assert ((x.grad.double() - want).abs() <= 101 * U * room).all() and torch.equal(x.grad, res.grad)
+    before = [t.detach().clone() for t in (w, up, bias)]
+    opt = optim.AdamW([w, up, bias], lr=1e-2, weight_decay=0.1, state_bits=8)
+    opt.step()
+    for t, old in zip((w, up, bias), before):
+        g = t.grad.double()
+        # the first step: m / (1 - b1) = g and v / (1 - b2) = g^2, so the update is lr * g / (|g| + eps)
+        want = old.double() * (1 - 1e-2 * 0.1) - 1e-2 * g / (g.abs() + 1e-8)
+        assert ((t.double() - want).abs() <= 16 * U * 1e-2 + 3 * U * old.double().abs()).all()
+
+
+def _graph(n=500, width=64):
+    from gnn_benchmark_b200 import Communicator, Quantizer_for_all_procs, TimeRecorder, graphgen
+    from gnn_benchmark_b200.data_manager.DataLoader import build_graph
+
+    src, dst = graphgen.erdos_renyi_edges(n, 3000, seed=5, device="cuda")
+    src, dst = graphgen.symmetrize(src, dst, n, self_loops=True)
+    begin = graphgen.contiguous_partitions(n, 1)
+    Communicator(32)
+    Quantizer_for_all_procs(1, 32)
+    TimeRecorder(3, 3)
+    local, remote = graphgen.partition_edges(src, dst, begin, 0)
+    return build_graph(local, remote, begin, 0, 1, width, 32, False, device="cuda"), src, dst
+
+
+def test_gcn_layer_with_8_bit_transform(cuda_lib, monkeypatch):
+    """DistGCNConv under MODE "fp8": transform first (24 > 8), so the layer is A (values(x) values(W)^T) + b."""
+    from gnn_benchmark_b200 import dense
+    from gnn_benchmark_b200.model import DistGCNConv
+
+    monkeypatch.setattr(dense, "MODE", "fp8")
+    n = 500
+    graph, src, dst = _graph(n)
+    torch.manual_seed(0)
+    conv = DistGCNConv(24, 8, 32, False).cuda()
+    conv.reset_parameters()
+    x = torch.randn(n, 24, device="cuda", requires_grad=True)
+    out = conv(graph, x, 0)
+    g = torch.randn_like(out)
+    out.backward(g)
+    dense.check_status()
+    A = torch.zeros(n, n, device="cuda", dtype=torch.float64)
+    A[dst, src] = 1.0
+    d = A.sum(1)
+    A = A / torch.sqrt(d)[:, None] / torch.sqrt(d)[None, :]
+    xq, wq = values(*quantise(x)), values(*quantise(conv.lin.weight, 128))
+    ref = A @ (xq @ wq.t()) + conv.bias.detach().double()
+    # the aggregation's own tolerance (fp32 sums of some tens of edges) on top of the product's
+    assert torch.allclose(out.double(), ref, rtol=1e-5, atol=1e-5)
+    gh = (A.t() @ g.double()).float()  # the gradient that reaches the transform, up to fp32 rounding of its codes' input
+    coarse = values(*quantise(gh)) @ values(*quantise(conv.lin.weight.t(), 128)).t()
+    # a code may flip where gh sits on a border: one step (2^-3 of an element at most) of one factor
+    room = 2.0 ** -3 * (gh.double().abs().amax(1, keepdim=True) * conv.lin.weight.detach().double().abs().amax(0))
+    assert ((x.grad.double() - coarse).abs() <= room + 1e-5).all()
+    assert (x.grad.double() - coarse).abs().mean() <= 1e-3 * coarse.abs().mean()
+
+
+@pytest.mark.parametrize("name", ["sage", "gcn"])
+def test_training_entry(cuda_lib, monkeypatch, name):
+    """The config keys end to end: three epochs run, the parameters move, the moments are 8-bit."""
+    from gnn_benchmark_b200 import dense
+    from gnn_benchmark_b200.model import create_model_and_optimizer, set_random_seed
+    from gnn_benchmark_b200.train import train
+
+    monkeypatch.setattr(dense, "MODE", "fp8")
+    graph, _, _ = _graph()
+    set_random_seed(1)
+    config = dict(model_name=name, in_channels=47, hidden_channels=64, out_channels=7, num_layers=3, dropout=0.5, num_bits=32,
+                  is_pre_delay=False, lr=0.01, weight_decay=5e-4, optimizer="adamw", optimizer_state_bits=8)
+    model, opt = create_model_and_optimizer(config, torch.device("cuda"))
+    old = [p.detach().clone() for p in model.parameters()]
+    data = {"graph": graph, "nodes_features": torch.randn(500, 47, device="cuda"),
+            "nodes_labels": torch.randint(0, 7, (500,), device="cuda"),
+            "nodes_train_masks": torch.arange(300, device="cuda"), "nodes_valid_masks": torch.arange(300, 400, device="cuda"),
+            "nodes_test_masks": torch.arange(400, 500, device="cuda")}
+    losses, _ = train(model, data, opt, 3, 32, log=None)
+    assert all(l == l and abs(l) < 100 for l in losses)
+    assert all(not torch.equal(a, p) and torch.isfinite(p).all() for a, p in zip(old, model.parameters()))
+    assert all(s["exp_avg"].dtype == torch.float8_e4m3fn for s in opt.state.values())
