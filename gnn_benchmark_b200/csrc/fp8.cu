@@ -11,12 +11,18 @@
 // One operand lies along the 128 lanes of tensor memory (P), the other along its columns (Q).  P is A and Q is B,
 // except for few rows of A (SWAP): then the weight's rows fill the lanes and the few rows are the columns.
 //
-// One persistent CTA per SM, three warpgroups:
-//   warp 0      lane 0 issues the TMA loads (a 128-byte wide k-block of both operands per stage);
-//   warp 1      allocates tensor memory; lane 0 issues tcgen05.mma (kind::f8f6f4, 128 x BN x 32) and the commits;
-//   warps 2-3   idle; their registers go to
-//   warps 4-11  which read a block's product, scale and add it; after the last block, convert and store.  Warp w
-//               reads lane quarter w % 4 and one half of the columns.
+// One persistent CTA per SM:
+//   warp 0      issues the TMA loads (a 128-byte wide k-block of both operands per stage);
+//   warp 1      allocates tensor memory, issues tcgen05.mma (kind::f8f6f4) and the commits;
+//   warps 2-3   take turns with a block's scales: bring them (cp.async, two turns ahead), multiply the two operands'
+//               where one of Q's covers 128 columns, and lay them out beside the partial product, whose barrier
+//               hands over both;
+//   warps 4-11  read a block's product, scale and add it; after the last block, convert and store.  Warp w reads
+//               lane quarter w % 4 and one half of the columns.
+// What bounds a block is the hand-over and scaling: per scheduler 256 FMAs, 180 cycles of tensor-memory reads and a
+// round trip between the warps, against 512 cycles of MMA.  So the scaling loop holds nothing that another warp can do.
+// Output tiles leave through shared memory by TMA stores, which run under the next tile's MMAs; rows that TMA cannot
+// address, and outputs that are added to, by plain stores.
 // A tile's sum may be split along k over several CTAs (few tiles, long sums): each writes an fp32 partial product
 // to the workspace and a second kernel adds them in a fixed order.
 // Every wait is bounded (about a second); on a time-out the kernel records a code in the library's status word,
@@ -27,30 +33,41 @@
 namespace gnnagg {
 namespace {
 
-constexpr int BP = 128;                        // rows of P per tile = TMEM lanes
+constexpr int BP = 128;                        // rows of P per CTA and tile = TMEM lanes
 constexpr int BK = 128;                        // bytes = elements per k-block = one scale block = one swizzle row
 constexpr int UMMA_K = 32;                     // elements per tcgen05.mma
-constexpr int kThreads = 384;
-// Registers per thread: 168 at launch (64,512 in all), then 56 for the first warpgroup and 216 for the other two
-// (7,168 + 55,296).
-constexpr int kRegsControl = 56, kRegsScaling = 216;
-static_assert(128 * kRegsControl + 256 * kRegsScaling <= 168 * kThreads, "register split");
-constexpr int kWarpsOut = 8;
 constexpr int kTmemCols = 512;
 constexpr int P_BYTES = BP * BK;
-constexpr int kRowSpan = 128;                  // bytes of an output row that a warp stages at once
-constexpr int kStaging = 32 * kRowSpan;        // per warp: the output of 32 rows, or two blocks' column scales
+constexpr int kPanel = 32 * 128;               // 32 rows of 128 bytes of the output, as a warp stages them
+constexpr int kRing = 3;                       // a scale warp's blocks: in use and on their way
+constexpr int kBarBytes = 256;
 constexpr int kSmemLimit = 227 * 1024;
+// Registers per thread of the widest tiles after the launch: the control warpgroup gives up what the scaling ones
+// take (sums up to what the block was launched with; launch() checks that before the first run).
+constexpr int kRegsControl = 72, kRegsScaling = 216;
 
-template <int BN>
+// BN columns per tile; QROW: Q's scales are per row.
+template <int BN, bool QROW>
 struct Tile {
+    static constexpr int kParts = BN >= 32 ? 2 : 1;                        // shares of the columns
+    static constexpr int kCols = BN / kParts;                              // columns of a warp: 16 to 128
+    static constexpr int kWarps = 4 * kParts;                              // scaling warps
+    static constexpr int kThreads = 128 + 32 * kWarps;
     static constexpr int kStageBytes = P_BYTES + BN * BK;
-    static constexpr int kFit = (kSmemLimit - 1024 - 256 - kWarpsOut * kStaging) / kStageBytes;
-    static constexpr int kStages = kFit > 10 ? 10 : kFit;
     static constexpr int kBufs = kTmemCols / BN > 4 ? 4 : kTmemCols / BN;  // partial products in tensor memory
-    static constexpr int kCols = BN / 2;                                   // columns of a warp
-    static constexpr int kSmem = 1024 + kStages * kStageBytes + kWarpsOut * kStaging + 256;
-    static_assert(kSmem <= kSmemLimit && (2 * kStages + 2 * kBufs + 1) * 8 + 8 <= 256, "shared memory budget");
+    static constexpr int kSets = (BN + 127) / 128;                         // scales of Q, when one covers 128 columns
+    static constexpr int kRaw = BP + (QROW ? BN : 4);                      // floats: scales as loaded, of a block
+    static constexpr int kSlot = QROW ? BP + BN : BP * kSets;              // floats: scales as used, of a block
+    static constexpr int kPanels = kCols == 128 ? 2 : 1;                   // staged panels per warp
+    static constexpr int kWarpBytes = kPanels * kPanel + kCols * 4;
+    static constexpr int kFixed = 1024 + kBarBytes + kWarps * kWarpBytes + (2 * kRing * kRaw + kBufs * kSlot) * 4;
+    static constexpr int kFit = (kSmemLimit - kFixed) / kStageBytes;
+    static constexpr int kStages = kFit > 10 ? 10 : kFit;
+    static constexpr int kSmem = kFixed + kStages * kStageBytes;
+    static constexpr int kBarriers = 2 * kStages + 2 * kBufs + 1;
+    static_assert(kSmem <= kSmemLimit && kStages >= 3 && kBarriers * 8 + 8 <= kBarBytes, "shared memory budget");
+    static constexpr bool kSplitRegs = BN == 256;
+    static constexpr int kRegsNeeded = 128 * kRegsControl + 32 * kWarps * kRegsScaling;
 };
 
 enum : int {
@@ -80,6 +97,7 @@ struct Params {
     int tiles_p, tiles_q, items;
     int accumulate;
     int vec_out;         // 16-byte stores of the output's rows
+    int tma_out;         // the output leaves by TMA
     unsigned long long wait_ns;
     uint32_t tx_excess;
 };
@@ -96,31 +114,40 @@ __device__ __forceinline__ void tc_mma_f8(uint32_t tmem_d, uint64_t adesc, uint6
         : "memory");
 }
 
+// 4 bytes global -> shared, or zero when !ok.
+__device__ __forceinline__ void cp_async_4_or_zero(uint32_t dst, const float *src, bool ok) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(ok ? 4 : 0) : "memory");
+}
+
+// 16 bytes, of which the first `bytes` (0 to 16) are read and the others zero.
+__device__ __forceinline__ void cp_async_16_or_less(uint32_t dst, const float *src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+// The warp's copies of N scales of block kb, of the rows from row0 on (zero behind `rows`): 16 bytes a lane where the
+// rows' scales lie side by side, a quarter of the instructions (4-byte copies kept the scale warps at 900 cycles a block).
+template <int N>
+__device__ __forceinline__ void fetch_scales(uint32_t dst, const Scales &s, int64_t row0, int64_t rows, int rows_each, int kb,
+                                             int lane) {
+    const float *base = s.p + kb * s.stride_k;
+    if (s.stride == 1 && rows_each == 1 && (reinterpret_cast<uintptr_t>(base) & 15u) == 0) {
+#pragma unroll
+        for (int j = 0; j < N; j += 128) {
+            const int64_t r = row0 + j + 4 * lane;
+            const int left = (int)(rows - r < 4 ? (rows - r < 0 ? 0 : rows - r) : 4);
+            if (j + 4 * lane < N) cp_async_16_or_less(dst + (j + 4 * lane) * 4, left > 0 ? base + r : s.p, 4 * left);
+        }
+    } else {
+#pragma unroll 1
+        for (int j = lane; j < N; j += 32) {
+            const int64_t r = row0 + j;
+            cp_async_4_or_zero(dst + j * 4, r < rows ? base + (rows_each == 1 ? r : r / 128) * s.stride : s.p, r < rows);
+        }
+    }
+}
+
 // Instruction descriptor of kind::f8f6f4: fp32 accumulator, e4m3 A and B (format 0), both K-major, M = 128.
 __host__ __device__ constexpr uint32_t f8_instr_desc(int n) {
     return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(BP >> 4) << 24);
-}
-
-// Two fp32 values in one 64-bit register pair.
-__device__ __forceinline__ uint64_t pair(float lo, float hi) {
-    uint64_t d;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
-    return d;
-}
-__device__ __forceinline__ float2 unpair(uint64_t d) {
-    float2 v;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(d));
-    return v;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
 }
 
 // A work item: one tile of the output and a range of its k-blocks.
@@ -130,31 +157,51 @@ struct Item {
 // Tiles of one column strip of 16 P-tiles are neighbours, so that concurrent CTAs share operand panels in L2.
 __device__ __forceinline__ Item item_of(const Params &p, int i) {
     Item w;
-    w.split = i % p.splits;
-    const int t = i / p.splits;
-    constexpr int kGroup = 16;
-    const int per = kGroup * p.tiles_q, g = t / per, r = t - g * per;
-    const int high = min(kGroup, p.tiles_p - g * kGroup);
-    w.tq = r / high;
-    w.tp = g * kGroup + (r - w.tq * high);
+    int t = i;
+    w.split = 0, w.tq = 0;
+    if (p.splits > 1) {
+        t = i / p.splits;
+        w.split = i - t * p.splits;
+    }
+    w.tp = t;
+    if (p.tiles_q > 1) {
+        constexpr int kGroup = 16;
+        const int per = kGroup * p.tiles_q, g = t / per, r = t - g * per;
+        const int high = min(kGroup, p.tiles_p - g * kGroup);
+        w.tq = r / high;
+        w.tp = g * kGroup + (r - w.tq * high);
+    }
     w.kb0 = w.split * p.kb_per_split;
     w.kb1 = min(p.kblocks, w.kb0 + p.kb_per_split);
     return w;
 }
 
-// BN columns per tile; QROW: Q's scales are per row (per column of the tile); SWAP: the output is stored
-// transposed, C[column][lane].
+// Place and phase parity in a ring of N barriers.
+template <int N>
+struct Ring {
+    int i = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void next() {
+        if (++i == N) i = 0, phase ^= 1u;
+    }
+};
+
+// SWAP: the output is stored transposed, C[column][lane].
 template <int BN, bool QROW, bool SWAP, typename TOut>
-__global__ void __launch_bounds__(kThreads, 1)
-fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q, const Params p) {
-    using S = Tile<BN>;
-    constexpr int kStages = S::kStages, kBufs = S::kBufs, kCols = S::kCols;
+__global__ void __launch_bounds__((Tile<BN, QROW>::kThreads), 1)
+fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
+                  const __grid_constant__ CUtensorMap map_c, const Params p) {
+    using S = Tile<BN, QROW>;
+    constexpr int kStages = S::kStages, kBufs = S::kBufs, kCols = S::kCols, kWarps = S::kWarps;
     extern __shared__ uint8_t smem_raw[];
     // 1024-byte alignment: the swizzle pattern and the descriptors assume it
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t *staging = smem + kStages * S::kStageBytes;
-    uint64_t *bars = reinterpret_cast<uint64_t *>(staging + kWarpsOut * kStaging);
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * kStages + 2 * kBufs + 1);
+    float *bias_s = reinterpret_cast<float *>(staging + kWarps * S::kPanels * kPanel);  // kCols per warp
+    float *raw = bias_s + kWarps * kCols;                                                // kRing * kRaw per scale warp
+    float *slots = raw + 2 * kRing * S::kRaw;                                                // one per partial product
+    uint64_t *bars = reinterpret_cast<uint64_t *>(slots + kBufs * S::kSlot);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + S::kBarriers);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const uint32_t bar0 = smem_u32(bars);
     auto bar_full = [&](int s) { return bar0 + 8u * (uint32_t)s; };
@@ -170,8 +217,8 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_consta
             mbar_init(bar_empty(s), 1);
         }
         for (int b = 0; b < kBufs; ++b) {
-            mbar_init(bar_acc_full(b), 1);
-            mbar_init(bar_acc_empty(b), 32 * kWarpsOut);
+            mbar_init(bar_acc_full(b), 2);  // the product, the scales
+            mbar_init(bar_acc_empty(b), kWarps);
         }
         mbar_init(bar_drain, 1);
         *abort_flag = 0;
@@ -189,25 +236,26 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_consta
     const uint32_t tmem_base = *tmem_slot;
 
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
-    if (warp == 0) {
-        // ---------------- TMA issuer ----------------
-        if (lane == 0) {
+        if (S::kSplitRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
+        if (warp == 0) {
+            // ---------------- TMA issuer ----------------
+            Ring<kStages> st;
             uint32_t it = 0;
             bool ok = true;
             for (int i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
                 const Item w = item_of(p, i);
-                for (int kb = w.kb0; kb < w.kb1; ++kb, ++it) {
-                    const int s = it % kStages;
-                    if (!mbar_wait(bar_empty(s), ((it / kStages) & 1u) ^ 1u, abort_flag, &g_status, kErrWaitEmpty,
-                                   p.wait_ns)) {
+                for (int kb = w.kb0; kb < w.kb1; ++kb, ++it, st.next()) {
+                    if (!mbar_wait(bar_empty(st.i), st.phase ^ 1u, abort_flag, &g_status, kErrWaitEmpty, p.wait_ns)) {
                         ok = false;
                         break;
                     }
-                    const uint32_t sp = smem_u32(smem + s * S::kStageBytes);
-                    mbar_arrive_expect_tx(bar_full(s), (uint32_t)S::kStageBytes + p.tx_excess);
-                    tma_load_2d(sp, &map_p, bar_full(s), kb * BK, w.tp * BP);
-                    tma_load_2d(sp + P_BYTES, &map_q, bar_full(s), kb * BK, w.tq * BN);
+                    if (elect_one()) {
+                        const uint32_t sp = smem_u32(smem) + (uint32_t)(st.i * S::kStageBytes);
+                        mbar_arrive_expect_tx(bar_full(st.i), (uint32_t)S::kStageBytes + p.tx_excess);
+                        tma_load_2d(sp, &map_p, bar_full(st.i), kb * BK, w.tp * BP);
+                        tma_load_2d(sp + P_BYTES, &map_q, bar_full(st.i), kb * BK, w.tq * BN);
+                    }
+                    __syncwarp();
                 }
             }
             if (!ok) {
@@ -223,36 +271,38 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_consta
                     }
                 }
             }
-        }
-    } else if (warp == 1) {
-        // ---------------- MMA issuer ----------------
-        if (lane == 0) {
-            uint32_t it = 0;
+        } else if (warp == 1) {
+            // ---------------- MMA issuer ----------------
+            Ring<kStages> st;
+            Ring<kBufs> ac;
             bool ok = true;
             for (int i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
                 const Item w = item_of(p, i);
-                for (int kb = w.kb0; kb < w.kb1; ++kb, ++it) {
-                    const int s = it % kStages, b = it % kBufs;
-                    if (!mbar_wait(bar_acc_empty(b), ((it / kBufs) & 1u) ^ 1u, abort_flag, &g_status, kErrWaitAccFree,
-                                   p.wait_ns) ||
-                        !mbar_wait(bar_full(s), (it / kStages) & 1u, abort_flag, &g_status, kErrWaitFull, p.wait_ns)) {
+                for (int kb = w.kb0; kb < w.kb1; ++kb, st.next(), ac.next()) {
+                    if (!mbar_wait(bar_full(st.i), st.phase, abort_flag, &g_status, kErrWaitFull, p.wait_ns) ||
+                        !mbar_wait(bar_acc_empty(ac.i), ac.phase ^ 1u, abort_flag, &g_status, kErrWaitAccFree, p.wait_ns)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t sp = smem_u32(smem + s * S::kStageBytes);
-                    const uint64_t dp = make_smem_desc(sp), dq = make_smem_desc(sp + P_BYTES);
+                    if (elect_one()) {
+                        const uint32_t sp = smem_u32(smem) + (uint32_t)(st.i * S::kStageBytes);
+                        const uint64_t dp = make_smem_desc(sp), dq = make_smem_desc(sp + P_BYTES);
+                        const uint32_t d = tmem_base + (uint32_t)(ac.i * BN);
 #pragma unroll
-                    for (int k = 0; k < BK / UMMA_K; ++k)  // 32 bytes further inside the swizzled row
-                        tc_mma_f8(tmem_base + (uint32_t)(b * BN), dp + (uint64_t)(2 * k), dq + (uint64_t)(2 * k),
-                                  f8_instr_desc(BN), k > 0 ? 1u : 0u);
-                    tc_commit(bar_empty(s));
-                    tc_commit(bar_acc_full(b));
+                        for (int k = 0; k < BK / UMMA_K; ++k)  // 32 bytes further inside the swizzled row
+                            tc_mma_f8(d, dp + (uint64_t)(2 * k), dq + (uint64_t)(2 * k), f8_instr_desc(BN), k > 0 ? 1u : 0u);
+                        tc_commit(bar_acc_full(ac.i));
+                        tc_commit(bar_empty(st.i));
+                    }
+                    __syncwarp();
                 }
             }
             if (!ok) {
                 // MMAs already issued still read shared memory and write tensor memory: drain, bounded
-                tc_commit(bar_drain);
+                __syncwarp();
+                if (elect_one()) tc_commit(bar_drain);
+                __syncwarp();
                 const unsigned long long t0 = globaltimer_ns();
                 while (!mbar_try_wait(bar_drain, 0)) {
                     if (globaltimer_ns() - t0 > p.wait_ns) {
@@ -261,142 +311,218 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_consta
                     }
                 }
             }
+        } else {
+            // ---------------- scales ----------------
+            float *mine = raw + (warp - 2) * kRing * S::kRaw;
+            Ring<kBufs> ac;
+            uint32_t it = 0;  // of all blocks; this warp has every second
+            bool ok = true;
+            for (int i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
+                const Item w = item_of(p, i);
+                const int64_t row0 = (int64_t)w.tp * BP, col0 = (int64_t)w.tq * BN;
+                const int first = w.kb0 + (int)((it ^ (uint32_t)(warp - 2)) & 1u);
+                auto fetch = [&](int kb) {
+                    if (kb < w.kb1) {
+                        const uint32_t dst = smem_u32(mine) + (uint32_t)((kb - first) / 2 % kRing * S::kRaw) * 4;
+                        fetch_scales<BP>(dst, p.sp, row0, p.rows_p, p.p_block ? 128 : 1, kb, lane);
+                        if (QROW)
+                            fetch_scales<BN>(dst + BP * 4, p.sq, col0, p.rows_q, 1, kb, lane);
+                        else if (lane < S::kSets)
+                            cp_async_4_or_zero(dst + (BP + lane) * 4,
+                                               p.sq.p + min(col0 / 128 + lane, (p.rows_q - 1) / 128) * p.sq.stride +
+                                                   kb * p.sq.stride_k,
+                                               true);
+                    }
+                    cp_async_commit();
+                };
+                for (int a = 0; a + 1 < kRing; ++a) fetch(first + 2 * a);
+                for (int kb = w.kb0; kb < w.kb1; ++kb, ++it, ac.next()) {
+                    if (((kb - first) & 1) != 0) continue;
+                    cp_async_wait<kRing - 2>();
+                    // the scaling warps have read what this slot held
+                    if (!__all_sync(kFullMask, mbar_wait(bar_acc_empty(ac.i), ac.phase ^ 1u, abort_flag, &g_status,
+                                                         kErrWaitAccFree, p.wait_ns))) {
+                        ok = false;
+                        break;
+                    }
+                    const float *src = mine + (kb - first) / 2 % kRing * S::kRaw;
+                    float *dst = slots + ac.i * S::kSlot;
+                    const float4 a = *reinterpret_cast<const float4 *>(src + 4 * lane);
+                    if (QROW) {
+                        *reinterpret_cast<float4 *>(dst + 4 * lane) = a;
+#pragma unroll
+                        for (int j = 0; j < BN; j += 128)
+                            if (j + 4 * lane < BN)
+                                *reinterpret_cast<float4 *>(dst + BP + j + 4 * lane) =
+                                    *reinterpret_cast<const float4 *>(src + BP + j + 4 * lane);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < S::kSets; ++j) {
+                            const float b = src[BP + j];
+                            *reinterpret_cast<float4 *>(dst + j * BP + 4 * lane) = make_float4(a.x * b, a.y * b, a.z * b, a.w * b);
+                        }
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar_acc_full(ac.i));
+                    fetch(kb + 2 * (kRing - 1));
+                }
+                cp_async_wait<0>();
+                __syncwarp();
+            }
         }
-    }
     } else {
         // ---------------- scaling warps ----------------
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsScaling));
-        const int q = warp & 3, half = (warp - 4) >> 2;
-        uint8_t *mine = staging + (warp - 4) * kStaging;
-        constexpr int kChunk = kCols < 32 ? kCols : 32;
-        constexpr int kQLoads = (kCols + 31) / 32;
-        uint32_t it = 0;
-        bool ok = true;
-        for (int i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
+        if (S::kSplitRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsScaling));
+        const int q = warp & 3, part = (warp - 4) >> 2;
+        uint8_t *mine = staging + (warp - 4) * S::kPanels * kPanel;
+        auto release = [&](uint32_t bar) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+        };
+        constexpr int kChunk = kCols > 32 ? (QROW ? 8 : 16) : kCols;
+        Ring<kBufs> ac;
+        uint32_t stores = 0;  // TMA stores of this warp so far
+        float *bias = bias_s + (warp - 4) * kCols;
+        int64_t bias_at = -1;  // first column of the bias that is there
+        uint32_t limit = 1u << 22;
+        for (int i = blockIdx.x; i < p.items; i += gridDim.x) {
             const Item w = item_of(p, i);
-            const int64_t row = (int64_t)w.tp * BP + q * 32 + lane;              // of P
-            const int64_t col0 = (int64_t)w.tq * BN + half * kCols;              // of Q
-            const bool row_ok = row < p.rows_p;
-            const float *sp = p.sp.p + (p.p_block ? row / 128 : row) * p.sp.stride;
-            const float *sq = p.sq.p + (QROW ? col0 + lane : col0 / 128) * p.sq.stride;
-            float next_p = 0.0f, next_q[kQLoads] = {};
-            auto fetch = [&](int kb) {
-                next_p = row_ok ? __ldg(sp + kb * p.sp.stride_k) : 0.0f;
+            const int64_t row0 = (int64_t)w.tp * BP + q * 32;                    // of P
+            const int64_t col0 = (int64_t)w.tq * BN + part * kCols;              // of Q
+            float acc[kCols];
 #pragma unroll
-                for (int j = 0; j < kQLoads; ++j) {
-                    const int64_t c = col0 + (QROW ? 32 * j + lane : 0);
-                    next_q[j] = 0.0f;
-                    if (c < p.rows_q && (!QROW || 32 * j + lane < kCols) && (QROW || j == 0))
-                        next_q[j] = __ldg(sq + (QROW ? 32 * j * p.sq.stride : 0) + kb * p.sq.stride_k);
-                }
-            };
-            uint64_t acc[kCols / 2];
-#pragma unroll
-            for (int j = 0; j < kCols / 2; ++j) acc[j] = 0;
-            if (QROW) __syncwarp();  // the last item's column scales have been read
-            if (w.kb0 < w.kb1) fetch(w.kb0);
-            for (int kb = w.kb0; kb < w.kb1; ++kb, ++it) {
-                const int b = it % kBufs;
-                const float scale_p = next_p;
-                uint64_t scale = pair(scale_p * next_q[0], scale_p * next_q[0]);
-                const float *cols = reinterpret_cast<const float *>(mine) + (kb & 1) * kCols;
-                if (QROW) {
-                    scale = pair(scale_p, scale_p);
-#pragma unroll
-                    for (int j = 0; j < kQLoads; ++j)
-                        if (32 * j + lane < kCols) const_cast<float *>(cols)[32 * j + lane] = next_q[j];
-                    __syncwarp();
-                }
-                if (kb + 1 < w.kb1) fetch(kb + 1);
-                // warp-uniform outcome: the tensor-memory loads below are warp-collective
-                if (!__all_sync(kFullMask, mbar_wait(bar_acc_full(b), (it / kBufs) & 1u, abort_flag, &g_status,
-                                                     kErrWaitAccFull, p.wait_ns))) {
-                    ok = false;
-                    break;
-                }
+            for (int j = 0; j < kCols; ++j) acc[j] = 0.0f;
+            for (int kb = w.kb0; kb < w.kb1; ++kb, ac.next()) {
+                // a wait that is counted in polls (up to about a second) and leaves the loop alone: after a time-out the
+                // sums are not used, and no later wait polls more than once
+                uint32_t polls = 0;
+                while (!mbar_try_wait(bar_acc_full(ac.i), ac.phase))
+                    if ((++polls & 1023u) == 0 && (polls > limit || *abort_flag != 0)) {
+                        limit = 0;
+                        break;
+                    }
+                __syncwarp();  // the tensor-memory loads are warp-collective
+                const float *slot = slots + ac.i * S::kSlot;
+                const float scale = slot[(QROW ? 0 : part * kCols / 128 * BP) + q * 32 + lane];
+                const float *col = slot + BP + part * kCols;
                 tc_fence_after();
-                const uint32_t taddr = tmem_base + (uint32_t)(b * BN + half * kCols) + ((uint32_t)(q * 32) << 16);
+                const uint32_t taddr = tmem_base + (uint32_t)(ac.i * BN + part * kCols) + ((uint32_t)(q * 32) << 16);
+                // the next columns are on their way while the FMAs of the last ones run
+                uint32_t r[2][kChunk];
+                TmemLoad<kChunk>::run(taddr, r[0]);
 #pragma unroll
-                for (int c = 0; c < kCols; c += kChunk) {
-                    uint32_t r[kChunk];
-                    TmemLoad<kChunk>::run(taddr + (uint32_t)c, r);
-                    TmemLoad<kChunk>::wait(r);
+                for (int c0 = 0; c0 < kCols; c0 += kChunk) {
+                    uint32_t(&now)[kChunk] = r[c0 / kChunk & 1];
+                    TmemLoad<kChunk>::wait(now);
+                    if (c0 + kChunk < kCols) {
+                        TmemLoad<kChunk>::run(taddr + (uint32_t)(c0 + kChunk), r[(c0 / kChunk + 1) & 1]);
+                    } else if (!QROW) {  // all of the partial product is in registers
+                        release(bar_acc_empty(ac.i));
+                    }
 #pragma unroll
-                    for (int j = 0; j < kChunk; j += 2) {
-                        const uint64_t v = pair(__uint_as_float(r[j]), __uint_as_float(r[j + 1]));
-                        uint64_t f = scale;
+                    for (int j = 0; j < kChunk; j += 4) {
                         if (QROW) {
-                            const float2 cs = *reinterpret_cast<const float2 *>(cols + c + j);
-                            f = mul2(scale, pair(cs.x, cs.y));
+                            const float4 cs = *reinterpret_cast<const float4 *>(col + c0 + j);
+                            acc[c0 + j] = fmaf(__uint_as_float(now[j]), scale * cs.x, acc[c0 + j]);
+                            acc[c0 + j + 1] = fmaf(__uint_as_float(now[j + 1]), scale * cs.y, acc[c0 + j + 1]);
+                            acc[c0 + j + 2] = fmaf(__uint_as_float(now[j + 2]), scale * cs.z, acc[c0 + j + 2]);
+                            acc[c0 + j + 3] = fmaf(__uint_as_float(now[j + 3]), scale * cs.w, acc[c0 + j + 3]);
+                        } else {
+#pragma unroll
+                            for (int e = j; e < j + 4; ++e) acc[c0 + e] = fmaf(__uint_as_float(now[e]), scale, acc[c0 + e]);
                         }
-                        acc[(c + j) / 2] = fma2(v, f, acc[(c + j) / 2]);
                     }
                 }
-                tc_fence_before();
-                mbar_arrive(bar_acc_empty(b));
+                if (QROW) release(bar_acc_empty(ac.i));  // the column scales have been read too
             }
-            if (!ok) break;
-            TOut *out = static_cast<TOut *>(p.C) + w.split * p.split_stride;
+            if (__any_sync(kFullMask, limit == 0)) {
+                *abort_flag = 1;
+                atomicCAS(&g_status, 0, (int)kErrWaitAccFull);
+                break;
+            }
             if (SWAP) {
                 // lane = column of the output: 32 neighbouring columns of one output row per store
-                const float bias = p.bias != nullptr && row_ok ? __ldg(p.bias + row) : 0.0f;
+                const int64_t row = row0 + lane;
+                const float bias = p.bias != nullptr && row < p.rows_p ? __ldg(p.bias + row) : 0.0f;
+                TOut *dst = static_cast<TOut *>(p.C) + w.split * p.split_stride + col0 * p.ldc + row;
 #pragma unroll
-                for (int j = 0; j < kCols / 2; ++j) {
-                    const float2 v = unpair(acc[j]);
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int64_t m = col0 + 2 * j + e;
-                        if (row_ok && m < p.rows_q) {
-                            TOut *dst = out + m * p.ldc + row;
-                            float o = (e ? v.y : v.x) + bias;
-                            if (p.accumulate) o += to_f32(*dst);
-                            *dst = from_f32<TOut>(o);
-                        }
+                for (int j = 0; j < kCols; ++j, dst += p.ldc) {
+                    if (row < p.rows_p && col0 + j < p.rows_q) {
+                        float o = acc[j] + bias;
+                        if (p.accumulate) o += to_f32(*dst);
+                        *dst = from_f32<TOut>(o);
                     }
                 }
             } else {
-                // 128 bytes of each of the warp's 32 rows at a time through shared memory (16-byte piece j of row r
-                // sits at piece j ^ (r & 7)), then 8 lanes per row store them
+                // panels of 128 bytes of each of the warp's 32 rows in shared memory; 16-byte piece j of row r sits at
+                // piece j ^ (r & 7), the 128-byte swizzle of the output's tensor map
                 constexpr int kPiece = 16 / (int)sizeof(TOut);                       // columns per 16 bytes
-                constexpr int kSpan = kCols < 8 * kPiece ? kCols : 8 * kPiece;       // columns per turn
+                constexpr int kSpan = kCols < 8 * kPiece ? kCols : 8 * kPiece;       // columns per panel
                 constexpr int kPieces = kSpan / kPiece;
-                __syncwarp();
+                const int valid = (int)(p.rows_q - col0 < kCols ? p.rows_q - col0 : kCols);
+                if (col0 != bias_at) {  // zeros where there is no bias
+                    __syncwarp();
+                    for (int j = lane; j < kCols; j += 32)
+                        bias[j] = p.bias != nullptr && j < valid ? __ldg(p.bias + col0 + j) : 0.0f;
+                    __syncwarp();
+                    bias_at = col0;
+                }
 #pragma unroll
-                for (int c = 0; c < kCols; c += kSpan) {
+                for (int c0 = 0; c0 < kCols; c0 += kSpan * S::kPanels) {
+                    if (p.tma_out) {
+                        if (lane == 0) tma_store_wait_read<0>();  // the stores that last read the panels are done
+                        __syncwarp();
+                    }
 #pragma unroll
-                    for (int j = 0; j < kPieces; ++j) {
-                        float v[kPiece];
+                    for (int c = c0; c < c0 + kSpan * S::kPanels && c < kCols; c += kSpan) {
+                        uint8_t *panel = mine + (c - c0) / kSpan * kPanel;
 #pragma unroll
-                        for (int e = 0; e < kPiece; e += 2) {
-                            const float2 u = unpair(acc[(c + j * kPiece + e) / 2]);
-                            v[e] = u.x, v[e + 1] = u.y;
-                        }
-                        if (p.bias != nullptr) {
+                        for (int j = 0; j < kPieces; ++j) {
+                            float v[kPiece];
 #pragma unroll
-                            for (int e = 0; e < kPiece; ++e) {
-                                const int64_t n = col0 + c + j * kPiece + e;
-                                if (n < p.rows_q) v[e] += __ldg(p.bias + n);
+                            for (int e = 0; e < kPiece; e += 4) {
+                                const float4 u = *reinterpret_cast<const float4 *>(bias + c + j * kPiece + e);
+                                const float *a = acc + c + j * kPiece + e;
+                                v[e] = a[0] + u.x, v[e + 1] = a[1] + u.y, v[e + 2] = a[2] + u.z, v[e + 3] = a[3] + u.w;
                             }
+                            *reinterpret_cast<uint4 *>(panel + lane * 128 + ((j ^ (lane & 7)) << 4)) = pack16<TOut>(v);
                         }
-                        *reinterpret_cast<uint4 *>(mine + lane * kRowSpan + ((j ^ (lane & 7)) << 4)) = pack16<TOut>(v);
+                    }
+                    if (p.tma_out) {
+                        fence_generic_to_async_smem();
+                        __syncwarp();
+                        if (lane == 0) {
+#pragma unroll
+                            for (int c = c0; c < c0 + kSpan * S::kPanels && c < kCols; c += kSpan)
+                                if (c < valid)
+                                    tma_store_3d(&map_c, smem_u32(mine) + (uint32_t)((c - c0) / kSpan * kPanel), (int)col0 + c,
+                                                 (int)row0, w.split);
+                            tma_store_commit();
+                        }
+                        continue;
                     }
                     __syncwarp();
 #pragma unroll
-                    for (int t = 0; t < 8; ++t) {
-                        const int r = 4 * t + (lane >> 3), j = lane & 7;
-                        const int64_t m = (int64_t)w.tp * BP + q * 32 + r;
-                        const int64_t n = col0 + c + j * kPiece;
-                        if (j < kPieces && m < p.rows_p && n < p.rows_q) {
-                            uint4 u = *reinterpret_cast<const uint4 *>(mine + r * kRowSpan + ((j ^ (r & 7)) << 4));
-                            TOut *dst = out + m * p.ldc + n;
-                            if (p.vec_out && n + kPiece <= p.rows_q && !p.accumulate) {
-                                *reinterpret_cast<uint4 *>(dst) = u;
-                            } else {
-                                const TOut *e = reinterpret_cast<const TOut *>(&u);
+                    for (int c = c0; c < c0 + kSpan * S::kPanels && c < kCols; c += kSpan) {
+                        const uint8_t *panel = mine + (c - c0) / kSpan * kPanel;
+                        const int j0 = lane & 7, left = valid - (c + j0 * kPiece);  // columns of this lane's piece that exist
+                        TOut *dst = static_cast<TOut *>(p.C) + w.split * p.split_stride + (row0 + (lane >> 3)) * p.ldc + col0 + c +
+                                    j0 * kPiece;
 #pragma unroll
-                                for (int x = 0; x < kPiece; ++x)
-                                    if (n + x < p.rows_q)
-                                        dst[x] = p.accumulate ? from_f32<TOut>(to_f32(dst[x]) + to_f32(e[x])) : e[x];
+                        for (int t = 0; t < 8; ++t, dst += 4 * p.ldc) {
+                            const int r = 4 * t + (lane >> 3);
+                            if (j0 < kPieces && left > 0 && row0 + r < p.rows_p) {
+                                const uint4 u = *reinterpret_cast<const uint4 *>(panel + r * 128 + ((j0 ^ (r & 7)) << 4));
+                                if (p.vec_out && left >= kPiece) {
+                                    *reinterpret_cast<uint4 *>(dst) = u;
+                                } else {
+                                    const TOut *e = reinterpret_cast<const TOut *>(&u);
+#pragma unroll
+                                    for (int x = 0; x < kPiece; ++x)
+                                        if (x < left)
+                                            dst[x] = p.accumulate ? from_f32<TOut>(to_f32(dst[x]) + to_f32(e[x])) : e[x];
+                                }
                             }
                         }
                     }
@@ -404,6 +530,7 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_consta
                 }
             }
         }
+        if (!SWAP && p.tma_out && lane == 0) tma_store_wait_all();  // shared memory stays valid until TMA has read it
     }
 
     tc_fence_before();
@@ -455,9 +582,9 @@ Plan plan_of(int64_t M, int64_t N, int64_t K) {
     Plan p;
     p.swap = M <= 64;
     const int64_t rp = p.swap ? N : M, rq = p.swap ? M : N;
-    p.tiles_p = (int)div_up(rp, BP);
     p.bn = rq <= 16 ? 16 : rq <= 32 ? 32 : rq <= 64 ? 64 : 128;
-    if (p.bn == 128 && (int64_t)p.tiles_p * div_up(rq, 256) >= kNumSMs / 2) p.bn = 256;
+    if (rp > BP && rq > 128) p.bn = 256;
+    p.tiles_p = (int)div_up(rp, BP);
     p.tiles_q = (int)div_up(rq, p.bn);
     p.kblocks = (int)div_up(K, BK);
     const int64_t tiles = (int64_t)p.tiles_p * p.tiles_q;
@@ -486,37 +613,64 @@ int make_map_f8(CUtensorMap *map, const void *base, int64_t rows, int64_t cols, 
     return GNNAGG_OK;
 }
 
+// The output as `splits` matrices of M x N one behind the other, in boxes of 128 bytes x 32 rows; a tile's part
+// outside its matrix is not written.
+int make_map_out(CUtensorMap *map, void *base, int type, int splits, int64_t M, int64_t N, int64_t ld) {
+    EncodeTiledFn fn = encode_fn();
+    const int size = type_size(type);
+    const cuuint64_t dims[3] = {(cuuint64_t)N, (cuuint64_t)M, (cuuint64_t)splits};
+    const cuuint64_t strides[2] = {(cuuint64_t)(ld * size), (cuuint64_t)(M * ld * size)};
+    const cuuint32_t box[3] = {(cuuint32_t)(128 / size), 32, 1};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUtensorMapDataType dt = type == kTypeF32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : type == kTypeBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                       : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const CUresult r = fn(map, dt, 3, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(GNNAGG_ERR_CUDA, "fp8_matmul: cuTensorMapEncodeTiled failed with code %d", (int)r);
+    return GNNAGG_OK;
+}
+
 template <int BN, bool QROW, bool SWAP, typename TOut>
-int launch(const CUtensorMap &mp, const CUtensorMap &mq, const Params &p, cudaStream_t st) {
+int launch(const CUtensorMap &mp, const CUtensorMap &mq, const CUtensorMap &mc, const Params &p, cudaStream_t st) {
+    using S = Tile<BN, QROW>;
     static PerDeviceOnce attr_done;
     const cudaError_t e = attr_done.run([] {
+        cudaFuncAttributes a;
+        const cudaError_t r = cudaFuncGetAttributes(&a, fp8_matmul_kernel<BN, QROW, SWAP, TOut>);
+        if (r != cudaSuccess) return r;
+        // a register split above what the launch allocates would wait forever
+        if (S::kSplitRegs && (a.numRegs > kRegsScaling || a.numRegs * S::kThreads < S::kRegsNeeded))
+            return cudaErrorInvalidConfiguration;
         return cudaFuncSetAttribute(fp8_matmul_kernel<BN, QROW, SWAP, TOut>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    Tile<BN>::kSmem);
+                                    S::kSmem);
     });
     if (e != cudaSuccess)
-        return fail(GNNAGG_ERR_CUDA, "fp8_matmul: cannot reserve %d bytes of shared memory: %s", Tile<BN>::kSmem,
+        return fail(GNNAGG_ERR_CUDA, "fp8_matmul: cannot reserve %d bytes of shared memory and the registers: %s", S::kSmem,
                     cudaGetErrorString(e));
     const int grid = p.items < kNumSMs ? p.items : kNumSMs;
-    fp8_matmul_kernel<BN, QROW, SWAP, TOut><<<grid, kThreads, Tile<BN>::kSmem, st>>>(mp, mq, p);
+    fp8_matmul_kernel<BN, QROW, SWAP, TOut><<<grid, S::kThreads, S::kSmem, st>>>(mp, mq, mc, p);
     return check_launch("fp8_matmul_kernel");
 }
 
 template <bool QROW, typename TOut>
-int launch_tile(const Plan &plan, const CUtensorMap &mp, const CUtensorMap &mq, const Params &p, cudaStream_t st) {
+int launch_tile(const Plan &plan, const CUtensorMap &mp, const CUtensorMap &mq, const CUtensorMap &mc, const Params &p,
+                cudaStream_t st) {
     if (plan.swap)
-        return plan.bn == 16   ? launch<16, QROW, true, TOut>(mp, mq, p, st)
-               : plan.bn == 32 ? launch<32, QROW, true, TOut>(mp, mq, p, st)
-                               : launch<64, QROW, true, TOut>(mp, mq, p, st);
-    return plan.bn == 16    ? launch<16, QROW, false, TOut>(mp, mq, p, st)
-           : plan.bn == 32  ? launch<32, QROW, false, TOut>(mp, mq, p, st)
-           : plan.bn == 64  ? launch<64, QROW, false, TOut>(mp, mq, p, st)
-           : plan.bn == 128 ? launch<128, QROW, false, TOut>(mp, mq, p, st)
-                            : launch<256, QROW, false, TOut>(mp, mq, p, st);
+        return plan.bn == 16   ? launch<16, QROW, true, TOut>(mp, mq, mc, p, st)
+               : plan.bn == 32 ? launch<32, QROW, true, TOut>(mp, mq, mc, p, st)
+                               : launch<64, QROW, true, TOut>(mp, mq, mc, p, st);
+    return plan.bn == 16    ? launch<16, QROW, false, TOut>(mp, mq, mc, p, st)
+           : plan.bn == 32  ? launch<32, QROW, false, TOut>(mp, mq, mc, p, st)
+           : plan.bn == 64  ? launch<64, QROW, false, TOut>(mp, mq, mc, p, st)
+           : plan.bn == 128 ? launch<128, QROW, false, TOut>(mp, mq, mc, p, st)
+                            : launch<256, QROW, false, TOut>(mp, mq, mc, p, st);
 }
 
 template <typename TOut>
-int launch_out(bool qrow, const Plan &plan, const CUtensorMap &mp, const CUtensorMap &mq, const Params &p, cudaStream_t st) {
-    return qrow ? launch_tile<true, TOut>(plan, mp, mq, p, st) : launch_tile<false, TOut>(plan, mp, mq, p, st);
+int launch_out(bool qrow, const Plan &plan, const CUtensorMap &mp, const CUtensorMap &mq, const CUtensorMap &mc,
+               const Params &p, cudaStream_t st) {
+    return qrow ? launch_tile<true, TOut>(plan, mp, mq, mc, p, st) : launch_tile<false, TOut>(plan, mp, mq, mc, p, st);
 }
 
 template <typename TOut>
@@ -583,15 +737,24 @@ extern "C" int gnnagg_fp8_matmul(const uint8_t *A, int64_t lda, const float *sa,
     if (rc == GNNAGG_OK)
         rc = plan.swap ? make_map_f8(&map_q, A, M, K, lda, plan.bn) : make_map_f8(&map_q, B, N, K, ldb, plan.bn);
     if (rc != GNNAGG_OK) return rc;
+    const int type = split ? (int)kTypeF32 : out_type;
+    const int64_t ldo = split ? plan.ldp : ldc;
+    void *out = split ? workspace : C;
+    const bool vec_out = aligned16(out) && (ldo * type_size(type)) % 16 == 0 && !(accumulate && !split);
+    // wide tiles leave by TMA where it can address the rows
+    const bool tma_out = vec_out && !plan.swap && plan.bn >= 128;
+    CUtensorMap map_c = map_p;  // not used without tma_out
+    if (tma_out) rc = make_map_out(&map_c, out, type, plan.splits, M, N, ldo);
+    if (rc != GNNAGG_OK) return rc;
 
     Params p;
-    p.C = split ? workspace : C;
+    p.C = out;
     p.bias = split ? nullptr : bias;
     p.sp = plan.swap ? zb : za;
     p.sq = plan.swap ? za : zb;
     p.rows_p = plan.swap ? N : M;
     p.rows_q = plan.swap ? M : N;
-    p.ldc = split ? plan.ldp : ldc;
+    p.ldc = ldo;
     p.split_stride = split ? M * plan.ldp : 0;
     p.p_block = (plan.swap ? b_block : a_block) == 128;
     p.kblocks = plan.kblocks;
@@ -601,14 +764,14 @@ extern "C" int gnnagg_fp8_matmul(const uint8_t *A, int64_t lda, const float *sa,
     p.tiles_q = plan.tiles_q;
     p.items = plan.tiles_p * plan.tiles_q * plan.splits;
     p.accumulate = split ? 0 : accumulate;
-    p.vec_out = split || (aligned16(C) && (ldc * type_size(out_type)) % 16 == 0);
+    p.vec_out = vec_out;
+    p.tma_out = tma_out;
     p.wait_ns = g_stall.wait_ns;
     p.tx_excess = g_stall.tx_excess;
     const bool qrow = (plan.swap ? a_block : b_block) == 1;
-    const int type = split ? (int)kTypeF32 : out_type;
-    rc = type == kTypeF32    ? launch_out<float>(qrow, plan, map_p, map_q, p, st)
-         : type == kTypeBf16 ? launch_out<__nv_bfloat16>(qrow, plan, map_p, map_q, p, st)
-                             : launch_out<__half>(qrow, plan, map_p, map_q, p, st);
+    rc = type == kTypeF32    ? launch_out<float>(qrow, plan, map_p, map_q, map_c, p, st)
+         : type == kTypeBf16 ? launch_out<__nv_bfloat16>(qrow, plan, map_p, map_q, map_c, p, st)
+                             : launch_out<__half>(qrow, plan, map_p, map_q, map_c, p, st);
     if (rc != GNNAGG_OK || !split) return rc;
     return join_out(out_type, plan, static_cast<const float *>(workspace), plan.splits, M, N, bias, accumulate, C, ldc, st);
 }

@@ -16,6 +16,20 @@ __device__ __forceinline__ unsigned long long globaltimer_ns() {
     return t;
 }
 
+// One lane of a converged warp: the same one at every call, so a single thread issues all copies or MMAs.  A warp
+// that runs its loop as a whole and elects a lane for the issue keeps addresses and descriptors in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t ok;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "elect.sync _|p, 0xffffffff;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(ok));
+    return ok != 0;
+}
+
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
@@ -40,10 +54,10 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
 }
 
 // Bounded wait.  Returns false when another role has raised `abort_flag` or when this wait ran out
-// of time (it then raises the flag and leaves `code` in the status word, first writer wins).
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *status,
-                                          int code, unsigned long long limit_ns) {
-    if (mbar_try_wait(bar, parity)) return true;
+// of time (it then raises the flag and leaves `code` in the status word, first writer wins).  The clock and the
+// flag are looked at only after some polls: a read of the clock costs about as much as a short wait.
+__device__ __forceinline__ bool mbar_wait_long(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *status,
+                                            int code, unsigned long long limit_ns) {
     const unsigned long long t0 = globaltimer_ns();
     uint32_t n = 0;
     while (!mbar_try_wait(bar, parity)) {
@@ -56,6 +70,13 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
             }
         }
     }
+    return true;
+}
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *status,
+                                          int code, unsigned long long limit_ns) {
+    uint32_t n = 0;
+    while (!mbar_try_wait(bar, parity))
+        if (++n == 64) return mbar_wait_long(bar, parity, abort_flag, status, code, limit_ns);
     return true;
 }
 
@@ -73,6 +94,11 @@ __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap *map, int x, i
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, uint32_t src, int x, int y) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(src),
                  "r"(x), "r"(y)
+                 : "memory");
+}
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap *map, uint32_t src, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(src),
+                 "r"(x), "r"(y), "r"(z)
                  : "memory");
 }
 __device__ __forceinline__ void tma_reduce_add_2d(const CUtensorMap *map, uint32_t src, int x, int y) {
