@@ -70,10 +70,16 @@ SIGNATURES = {
     "gnnagg_rms_norm_bwd": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i32, _i64, _i32, _i32, _vp, _i64,
                                            _vp, _vp, _sz, _vp]),
     "gnnagg_fp8_quantize": (ctypes.c_int, [_vp, _i64, _i64, _i64, _i32, _i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64,
-                                           _vp]),
+                                           _vp, _vp]),
     "gnnagg_fp8_matmul_workspace_bytes": (_sz, [_i64, _i64, _i64]),
     "gnnagg_fp8_matmul": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i64, _i32, _vp, _i64, _vp, _i64, _i64, _i32, _i64, _i64,
-                                         _i64, _vp, _i32, _vp, _i64, _i32, _vp, _sz, _vp]),
+                                         _i64, _vp, _i32, _i32, _vp, _i64, _i32, _vp, _sz, _vp]),
+    "gnnagg_fp8_linear_kept_bytes": (_sz, [_i64, _i64, _i64, _i32, _i32]),
+    "gnnagg_fp8_linear_scratch_bytes": (_sz, [_i64, _i64, _i64, _i32]),
+    "gnnagg_fp8_linear_fwd": (ctypes.c_int, [_vp, _i64, _i32, _vp, _i64, _i32, _vp, _i32, _i64, _i64, _i64, _vp, _i32, _i32,
+                                             _i32, _vp, _sz, _vp, _sz, _vp]),
+    "gnnagg_fp8_linear_bwd": (ctypes.c_int, [_vp, _i64, _i32, _i64, _i64, _i64, _i32, _i32, _vp, _sz, _vp, _i32, _vp, _i32,
+                                             _vp, _i32, _vp, _sz, _vp]),
     "gnnagg_fp8_matmul_status": (ctypes.c_int, [_vp]),
     "gnnagg_fp8_matmul_status_clear": (ctypes.c_int, [_vp]),
     "gnnagg_adamw_scalars_bytes": (_sz, []),
@@ -112,8 +118,9 @@ def check(rc: int, what: str) -> None:
 
 
 def stream_ptr(device=None) -> int:
-    """cudaStream_t of torch's current stream on `device`."""
-    return torch.cuda.current_stream(device).cuda_stream
+    """cudaStream_t of torch's current stream on `device` (without building torch's Stream object: 2 us a call)."""
+    index = None if device is None else torch.device(device).index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 def ptr(t) -> int:
@@ -141,11 +148,15 @@ class device_of:
 
 
 def empty_codes(rows: int, cols: int, device):
-    """Uninitialised e4m3 codes (rows, cols) whose rows start on 16 bytes, and their scales, one per row and 128
-    columns, (rows, ceil(cols / 128)) lying column by column."""
-    codes = torch.empty((rows, (cols + 15) // 16 * 16), dtype=torch.float8_e4m3fn, device=device)
-    scales = torch.empty(((cols + 127) // 128, rows), dtype=torch.float32, device=device)
-    return codes[:, :cols], scales.t()
+    """Uninitialised e4m3 codes (rows, cols) whose rows start on 16 bytes, and their scales (`empty_scales`)."""
+    ld = (cols + 15) // 16 * 16
+    codes = torch.empty_strided((rows, cols) if ld == cols else (rows, ld), (ld, 1), dtype=torch.float8_e4m3fn, device=device)
+    return codes if ld == cols else codes[:, :cols], empty_scales(rows, cols, device)
+
+
+def empty_scales(rows: int, cols: int, device):
+    """Uninitialised scales, one per row and 128 columns, lying column by column, each column on 16 bytes."""
+    return torch.empty_strided((rows, (cols + 127) // 128), (1, (rows + 3) // 4 * 4), dtype=torch.float32, device=device)
 
 
 def require_cuda(*tensors) -> None:

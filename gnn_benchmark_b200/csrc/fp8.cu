@@ -89,7 +89,8 @@ struct Scales {
 
 struct Params {
     void *C;             // output, or the workspace's partial products
-    const float *bias;
+    const void *bias;
+    int bias_type;
     Scales sp, sq;
     int64_t rows_p, rows_q, ldc, split_stride;
     int p_block;         // P's scales are per 128 rows
@@ -382,7 +383,6 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_consta
         };
         constexpr int kChunk = kCols > 32 ? (QROW ? 8 : 16) : kCols;
         Ring<kBufs> ac;
-        uint32_t stores = 0;  // TMA stores of this warp so far
         float *bias = bias_s + (warp - 4) * kCols;
         int64_t bias_at = -1;  // first column of the bias that is there
         uint32_t limit = 1u << 22;
@@ -444,7 +444,7 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_consta
             if (SWAP) {
                 // lane = column of the output: 32 neighbouring columns of one output row per store
                 const int64_t row = row0 + lane;
-                const float bias = p.bias != nullptr && row < p.rows_p ? __ldg(p.bias + row) : 0.0f;
+                const float bias = p.bias != nullptr && row < p.rows_p ? load_as_f32(p.bias, p.bias_type, row) : 0.0f;
                 TOut *dst = static_cast<TOut *>(p.C) + w.split * p.split_stride + col0 * p.ldc + row;
 #pragma unroll
                 for (int j = 0; j < kCols; ++j, dst += p.ldc) {
@@ -464,7 +464,7 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_consta
                 if (col0 != bias_at) {  // zeros where there is no bias
                     __syncwarp();
                     for (int j = lane; j < kCols; j += 32)
-                        bias[j] = p.bias != nullptr && j < valid ? __ldg(p.bias + col0 + j) : 0.0f;
+                        bias[j] = p.bias != nullptr && j < valid ? load_as_f32(p.bias, p.bias_type, col0 + j) : 0.0f;
                     __syncwarp();
                     bias_at = col0;
                 }
@@ -546,7 +546,7 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_consta
 template <typename TOut>
 __global__ void __launch_bounds__(256)
 fp8_join_kernel(const float *__restrict__ partial, int splits, int64_t split_stride, int64_t ldp, int64_t M, int64_t N,
-                const float *__restrict__ bias, int accumulate, TOut *C, int64_t ldc) {
+                const void *bias, int bias_type, int accumulate, TOut *C, int64_t ldc) {
     const int64_t quads = ldp / 4, total = M * quads;
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
         const int64_t m = i / quads, n = (i - m * quads) * 4;
@@ -562,7 +562,7 @@ fp8_join_kernel(const float *__restrict__ partial, int splits, int64_t split_str
         for (int e = 0; e < 4; ++e)
             if (n + e < N) {
                 TOut *dst = C + m * ldc + n + e;
-                float o = v[e] + (bias != nullptr ? __ldg(bias + n + e) : 0.0f);
+                float o = v[e] + (bias != nullptr ? load_as_f32(bias, bias_type, n + e) : 0.0f);
                 if (accumulate) o += to_f32(*dst);
                 *dst = from_f32<TOut>(o);
             }
@@ -674,20 +674,20 @@ int launch_out(bool qrow, const Plan &plan, const CUtensorMap &mp, const CUtenso
 }
 
 template <typename TOut>
-int join(const Plan &plan, const float *partial, int splits, int64_t M, int64_t N, const float *bias, int accumulate,
-         void *C, int64_t ldc, cudaStream_t st) {
+int join(const Plan &plan, const float *partial, int splits, int64_t M, int64_t N, const void *bias,
+         int bias_type, int accumulate, void *C, int64_t ldc, cudaStream_t st) {
     const int64_t want = div_up(M * (plan.ldp / 4), 256);
     const int64_t cap = (int64_t)kNumSMs * 8;
     fp8_join_kernel<TOut><<<(unsigned)(want < cap ? want : cap), 256, 0, st>>>(
-        partial, splits, M * plan.ldp, plan.ldp, M, N, bias, accumulate, static_cast<TOut *>(C), ldc);
+        partial, splits, M * plan.ldp, plan.ldp, M, N, bias, bias_type, accumulate, static_cast<TOut *>(C), ldc);
     return check_launch("fp8_join_kernel");
 }
 
-int join_out(int type, const Plan &plan, const float *partial, int splits, int64_t M, int64_t N, const float *bias,
-             int accumulate, void *C, int64_t ldc, cudaStream_t st) {
-    return type == kTypeF32    ? join<float>(plan, partial, splits, M, N, bias, accumulate, C, ldc, st)
-           : type == kTypeBf16 ? join<__nv_bfloat16>(plan, partial, splits, M, N, bias, accumulate, C, ldc, st)
-                               : join<__half>(plan, partial, splits, M, N, bias, accumulate, C, ldc, st);
+int join_out(int type, const Plan &plan, const float *partial, int splits, int64_t M, int64_t N, const void *bias,
+             int bias_type, int accumulate, void *C, int64_t ldc, cudaStream_t st) {
+    return type == kTypeF32    ? join<float>(plan, partial, splits, M, N, bias, bias_type, accumulate, C, ldc, st)
+           : type == kTypeBf16 ? join<__nv_bfloat16>(plan, partial, splits, M, N, bias, bias_type, accumulate, C, ldc, st)
+                               : join<__half>(plan, partial, splits, M, N, bias, bias_type, accumulate, C, ldc, st);
 }
 
 }  // namespace
@@ -703,12 +703,14 @@ extern "C" size_t gnnagg_fp8_matmul_workspace_bytes(int64_t M, int64_t N, int64_
 extern "C" int gnnagg_fp8_matmul(const uint8_t *A, int64_t lda, const float *sa, int64_t sa_stride, int64_t sa_stride_k,
                                  int32_t a_block, const uint8_t *B, int64_t ldb, const float *sb, int64_t sb_stride,
                                  int64_t sb_stride_k, int32_t b_block, int64_t M, int64_t N, int64_t K,
-                                 const float *bias, int32_t accumulate, void *C, int64_t ldc, int32_t out_type,
+                                 const void *bias, int32_t bias_type, int32_t accumulate, void *C, int64_t ldc, int32_t out_type,
                                  void *workspace, size_t workspace_bytes, void *stream) {
     if (M < 0 || N < 0 || K < 0 || (accumulate != 0 && accumulate != 1))
         return fail(GNNAGG_ERR_ARG, "fp8_matmul: negative size or bad accumulate flag");
     if ((a_block != 1 && a_block != 128) || (b_block != 1 && b_block != 128))
         return fail(GNNAGG_ERR_ARG, "fp8_matmul: a scale covers 1 or 128 rows");
+    if (bias != nullptr && type_size(bias_type) == 0)
+        return fail(GNNAGG_ERR_ARG, "fp8_matmul: unknown bias type %d", bias_type);
     if (type_size(out_type) == 0) return fail(GNNAGG_ERR_ARG, "fp8_matmul: unknown output type %d", out_type);
     if (accumulate && out_type != kTypeF32)
         return fail(GNNAGG_ERR_UNSUPPORTED, "fp8_matmul: accumulation needs an fp32 output");
@@ -724,7 +726,7 @@ extern "C" int gnnagg_fp8_matmul(const uint8_t *A, int64_t lda, const float *sa,
         return fail(GNNAGG_ERR_ARG, "fp8_matmul: negative scale stride");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const Plan plan = plan_of(M, N, K);
-    if (K == 0) return join_out(out_type, plan, nullptr, 0, M, N, bias, accumulate, C, ldc, st);
+    if (K == 0) return join_out(out_type, plan, nullptr, 0, M, N, bias, bias_type, accumulate, C, ldc, st);
     const bool split = plan.splits > 1;
     if (split && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < plan.bytes()))
         return fail(GNNAGG_ERR_SCRATCH, "fp8_matmul: workspace too small or misaligned (need %zu bytes)", plan.bytes());
@@ -750,6 +752,7 @@ extern "C" int gnnagg_fp8_matmul(const uint8_t *A, int64_t lda, const float *sa,
     Params p;
     p.C = out;
     p.bias = split ? nullptr : bias;
+    p.bias_type = bias_type;
     p.sp = plan.swap ? zb : za;
     p.sq = plan.swap ? za : zb;
     p.rows_p = plan.swap ? N : M;
@@ -773,7 +776,7 @@ extern "C" int gnnagg_fp8_matmul(const uint8_t *A, int64_t lda, const float *sa,
          : type == kTypeBf16 ? launch_out<__nv_bfloat16>(qrow, plan, map_p, map_q, map_c, p, st)
                              : launch_out<__half>(qrow, plan, map_p, map_q, map_c, p, st);
     if (rc != GNNAGG_OK || !split) return rc;
-    return join_out(out_type, plan, static_cast<const float *>(workspace), plan.splits, M, N, bias, accumulate, C, ldc, st);
+    return join_out(out_type, plan, static_cast<const float *>(workspace), plan.splits, M, N, bias, bias_type, accumulate, C, ldc, st);
 }
 
 extern "C" int gnnagg_fp8_matmul_status(void *stream) {

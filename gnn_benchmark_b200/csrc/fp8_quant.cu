@@ -1,8 +1,8 @@
 // e4m3 codes and block scales of a matrix, along its rows, along its columns (transposed codes), or both from one
 // read: the operands of the 8-bit product.
 //
-// A block of the grid holds a 128 x 128 tile in registers: 256 threads, each V neighbouring columns (16 bytes of
-// input) of a run of neighbouring rows.  Largest magnitudes are maxima of bit patterns, by shuffles along a row and
+// A block of the grid holds a 128 x 128 tile in registers, as it lies in memory: 256 threads, each V neighbouring
+// columns (16 bytes of input) of a run of neighbouring rows.  Largest magnitudes are maxima of bit patterns, by shuffles along a row and
 // by shared-memory atomics along columns (a maximum does not depend on the order).  Transposed codes go through a
 // 16 KB shared tile: 8 rows of a column are one 8-byte piece, at piece index XOR (column / V) so that a warp's
 // stores meet different banks, and leave as 16-byte stores.
@@ -22,6 +22,7 @@ struct QuantParams {
     int64_t ldc, ldt;
     float *scales, *scales_t;      // scale of (row or row block i, column group j) at i + j * lds, likewise for the
     int64_t lds, lds_t;            // transpose
+    float *column_sums;            // [row blocks][cols] sums of x over a tile's rows, or null
 };
 
 // BLOCK: one scale for the whole tile; otherwise one per row (ROWS) and one per column (COLS) of the tile.
@@ -38,20 +39,38 @@ __global__ void __launch_bounds__(kThreads) fp8_quantize_kernel(const QuantParam
     const int valid = (int)(p.cols - col < V ? p.cols - col : V);
     if (threadIdx.x < kTile) top[threadIdx.x] = 0;
     __syncthreads();
-    float v[kRun][V];
+    uint4 raw[kRun];
+    auto at = [&](int i, int e) { return to_f32(reinterpret_cast<const T *>(&raw[i])[e]); };
 #pragma unroll
     for (int i = 0; i < kRun; ++i) {
         const int64_t row = row0 + rg * kRun + i;
+        raw[i] = make_uint4(0, 0, 0, 0);
+        if (row < p.rows && valid > 0) raw[i] = load_raw<T, VEC>(static_cast<const T *>(p.x) + row * p.ldx + col, valid);
+    }
+    if (p.column_sums != nullptr) {
+        constexpr int kRuns = kTile / kRun;
+        __shared__ float red[kRuns][kTile];
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[i][e] = 0.0f;
-        if (row < p.rows && valid > 0) load_chunk<T, VEC>(static_cast<const T *>(p.x) + row * p.ldx + col, valid, v[i]);
+        for (int e = 0; e < V; ++e) {
+            float s = at(0, e);
+#pragma unroll
+            for (int i = 1; i < kRun; ++i) s += at(i, e);
+            red[rg][ch * V + e] = s;
+        }
+        __syncthreads();
+        if (threadIdx.x < kTile && col0 + threadIdx.x < p.cols) {
+            float s = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kRuns; ++i) s += red[i][threadIdx.x];
+            p.column_sums[blockIdx.x * p.cols + col0 + threadIdx.x] = s;
+        }
     }
     uint32_t whole = 0;
     if (BLOCK) {
 #pragma unroll
         for (int i = 0; i < kRun; ++i)
 #pragma unroll
-            for (int e = 0; e < V; ++e) whole = max(whole, abs_bits(v[i][e]));
+            for (int e = 0; e < V; ++e) whole = max(whole, abs_bits(at(i, e)));
         whole = __reduce_max_sync(kFullMask, whole);
         if ((threadIdx.x & 31) == 0) atomicMax(&top[0], whole);
         __syncthreads();
@@ -69,7 +88,7 @@ __global__ void __launch_bounds__(kThreads) fp8_quantize_kernel(const QuantParam
             uint32_t m = whole;
             if (!BLOCK) {
 #pragma unroll
-                for (int e = 0; e < V; ++e) m = max(m, abs_bits(v[i][e]));
+                for (int e = 0; e < V; ++e) m = max(m, abs_bits(at(i, e)));
 #pragma unroll
                 for (int off = kLanes / 2; off > 0; off >>= 1) m = max(m, __shfl_xor_sync(kFullMask, m, off));
             }
@@ -78,8 +97,8 @@ __global__ void __launch_bounds__(kThreads) fp8_quantize_kernel(const QuantParam
                 uint32_t c[V / 4];
 #pragma unroll
                 for (int k = 0; k < V / 4; ++k)
-                    c[k] = e4m3x4(__fmul_rn(v[i][4 * k], f), __fmul_rn(v[i][4 * k + 1], f), __fmul_rn(v[i][4 * k + 2], f),
-                                  __fmul_rn(v[i][4 * k + 3], f));
+                    c[k] = e4m3x4(__fmul_rn(at(i, 4 * k), f), __fmul_rn(at(i, 4 * k + 1), f), __fmul_rn(at(i, 4 * k + 2), f),
+                                  __fmul_rn(at(i, 4 * k + 3), f));
                 // code rows are padded to 16 bytes, so a whole chunk always fits
                 uint32_t *dst = reinterpret_cast<uint32_t *>(p.codes + row * p.ldc + col);
                 if (V == 8)
@@ -96,7 +115,7 @@ __global__ void __launch_bounds__(kThreads) fp8_quantize_kernel(const QuantParam
             for (int e = 0; e < V; ++e) {
                 uint32_t m = 0;
 #pragma unroll
-                for (int i = 0; i < kRun; ++i) m = max(m, abs_bits(v[i][e]));
+                for (int i = 0; i < kRun; ++i) m = max(m, abs_bits(at(i, e)));
                 if (V == 8) m = max(m, __shfl_xor_sync(kFullMask, m, 16));  // the warp's other run of rows
                 if (V == 4 || (threadIdx.x & 16) == 0) atomicMax(&top[ch * V + e], m);
             }
@@ -108,10 +127,10 @@ __global__ void __launch_bounds__(kThreads) fp8_quantize_kernel(const QuantParam
 #pragma unroll
             for (int k = 0; k < kRun / 8; ++k) {
                 uint2 u;
-                u.x = e4m3x4(__fmul_rn(v[8 * k][e], f), __fmul_rn(v[8 * k + 1][e], f), __fmul_rn(v[8 * k + 2][e], f),
-                             __fmul_rn(v[8 * k + 3][e], f));
-                u.y = e4m3x4(__fmul_rn(v[8 * k + 4][e], f), __fmul_rn(v[8 * k + 5][e], f), __fmul_rn(v[8 * k + 6][e], f),
-                             __fmul_rn(v[8 * k + 7][e], f));
+                u.x = e4m3x4(__fmul_rn(at(8 * k, e), f), __fmul_rn(at(8 * k + 1, e), f), __fmul_rn(at(8 * k + 2, e), f),
+                             __fmul_rn(at(8 * k + 3, e), f));
+                u.y = e4m3x4(__fmul_rn(at(8 * k + 4, e), f), __fmul_rn(at(8 * k + 5, e), f), __fmul_rn(at(8 * k + 6, e), f),
+                             __fmul_rn(at(8 * k + 7, e), f));
                 const int piece = (rg * (kRun / 8) + k) ^ (ch & 15);
                 *reinterpret_cast<uint2 *>(tile + (ch * V + e) * kTile + piece * 8) = u;
             }
@@ -157,7 +176,7 @@ using namespace gnnagg;
 
 extern "C" int gnnagg_fp8_quantize(const void *x, int64_t ldx, int64_t rows, int64_t cols, int32_t type, int32_t block_rows,
                                    uint8_t *codes, int64_t ldc, float *scales, int64_t lds, uint8_t *codes_t, int64_t ldt,
-                                   float *scales_t, int64_t lds_t, void *stream) {
+                                   float *scales_t, int64_t lds_t, float *column_sums, void *stream) {
     if (rows < 0 || cols < 0) return fail(GNNAGG_ERR_ARG, "fp8_quantize: negative size");
     if (type_size(type) == 0) return fail(GNNAGG_ERR_ARG, "fp8_quantize: unknown element type %d", type);
     if (block_rows != 1 && block_rows != 128) return fail(GNNAGG_ERR_ARG, "fp8_quantize: blocks are 1 x 128 or 128 x 128");
@@ -175,7 +194,7 @@ extern "C" int gnnagg_fp8_quantize(const void *x, int64_t ldx, int64_t rows, int
     const int64_t r = block_rows == 1 ? rows : div_up(rows, kTile), c = block_rows == 1 ? cols : div_up(cols, kTile);
     if ((codes != nullptr && lds < r) || (codes_t != nullptr && lds_t < c))
         return fail(GNNAGG_ERR_ARG, "fp8_quantize: a stride of the scales is too small");
-    const QuantParams p{x, ldx, rows, cols, codes, codes_t, ldc, ldt, scales, scales_t, lds, lds_t};
+    const QuantParams p{x, ldx, rows, cols, codes, codes_t, ldc, ldt, scales, scales_t, lds, lds_t, column_sums};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool block = block_rows == 128;
     return type == kTypeF32    ? launch_type<float>(p, block, st)

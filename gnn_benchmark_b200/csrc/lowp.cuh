@@ -54,6 +54,12 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { retu
 template <>
 __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
 
+__device__ __forceinline__ float load_as_f32(const void *p, int type, int64_t i) {
+    return type == kTypeF32    ? static_cast<const float *>(p)[i]
+           : type == kTypeBf16 ? to_f32(static_cast<const __nv_bfloat16 *>(p)[i])
+                               : to_f32(static_cast<const __half *>(p)[i]);
+}
+
 template <typename T>
 struct Vec {
     static constexpr int N = 16 / (int)sizeof(T);  // elements of one 16-byte access
@@ -74,25 +80,55 @@ __device__ __forceinline__ uint4 pack16(const float (&f)[Vec<T>::N]) {
     return u;
 }
 
-// Vec<T>::N consecutive elements at p, of which `valid` exist (the others read as zero).  VEC: one 16-byte
-// access (p aligned, all valid); otherwise element by element.
+// Vec<T>::N consecutive elements at p, of which `valid` exist (the others read as zero), as they lie in memory: a
+// 16-bit row held this way takes half the registers of its fp32 values.  VEC: one 16-byte access (p aligned, all
+// valid); otherwise element by element.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load_chunk(const T *p, int valid, float (&f)[Vec<T>::N]) {
-    if (VEC) {
-        unpack16<T>(__ldcs(reinterpret_cast<const uint4 *>(p)), f);
-    } else {
+__device__ __forceinline__ uint4 load_raw(const T *p, int valid) {
+    if (VEC) return __ldcs(reinterpret_cast<const uint4 *>(p));
+    uint4 u = make_uint4(0, 0, 0, 0);
+    T *e = reinterpret_cast<T *>(&u);
 #pragma unroll
-        for (int i = 0; i < Vec<T>::N; ++i) f[i] = i < valid ? to_f32(p[i]) : 0.0f;
+    for (int i = 0; i < Vec<T>::N; ++i)
+        if (i < valid) e[i] = p[i];
+    return u;
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void store_raw(T *p, int valid, const uint4 &u) {
+    if (VEC) {
+        __stcs(reinterpret_cast<uint4 *>(p), u);
+    } else {
+        const T *e = reinterpret_cast<const T *>(&u);
+#pragma unroll
+        for (int i = 0; i < Vec<T>::N; ++i)
+            if (i < valid) p[i] = e[i];
     }
 }
 template <typename T, bool VEC>
+__device__ __forceinline__ void load_chunk(const T *p, int valid, float (&f)[Vec<T>::N]) {
+    unpack16<T>(load_raw<T, VEC>(p, valid), f);
+}
+template <typename T, bool VEC>
 __device__ __forceinline__ void store_chunk(T *p, int valid, const float (&f)[Vec<T>::N]) {
-    if (VEC) {
-        *reinterpret_cast<uint4 *>(p) = pack16<T>(f);
-    } else {
+    store_raw<T, VEC>(p, valid, pack16<T>(f));
+}
+
+// out[c] = sum of partial[b][c] over the blocks, in a fixed order: 16 threads take every 16th block of a column.
+template <typename T>
+__global__ void __launch_bounds__(512) column_sum_kernel(const float *__restrict__ partial, int64_t blocks, int64_t F, T *out) {
+    __shared__ float red[16][33];
+    const int64_t c = (int64_t)blockIdx.x * 32 + threadIdx.x;
+    float s = 0.0f;
+    if (c < F) {
+#pragma unroll 8
+        for (int64_t b = threadIdx.y; b < blocks; b += 16) s += partial[b * F + c];
+    }
+    red[threadIdx.y][threadIdx.x] = s;
+    __syncthreads();
+    if (threadIdx.y == 0 && c < F) {
 #pragma unroll
-        for (int i = 0; i < Vec<T>::N; ++i)
-            if (i < valid) p[i] = from_f32<T>(f[i]);
+        for (int i = 1; i < 16; ++i) s += red[i][threadIdx.x];
+        out[c] = from_f32<T>(s);
     }
 }
 

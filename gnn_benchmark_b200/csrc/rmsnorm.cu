@@ -4,10 +4,11 @@
 //     y = h * r * w,   r = rsqrt(mean(h^2) + eps)
 //     dh = gh + r * (w gy - hat * mean(w gy hat)),  hat = h r;   dw = sum over rows of gy hat
 //
-// Forward is one pass: a row stays in registers between the sum of squares and the scaling.  A row of up to
-// 128 16-byte chunks belongs to a warp (eight rows a block), a longer one to a block.  Backward reads h and the
-// two gradients once, writes dh once and keeps the column sums of dw in registers over all rows of a
-// persistent block; a second kernel adds the blocks' sums in a fixed order (no atomics).
+// Forward is one pass: a row stays in registers, as it lies in memory, between the sum of squares and the scaling.  A
+// row of up to 128 16-byte chunks belongs to a warp (short ones two at a time, so that a warp has 1 to 2 KB on their
+// way), a longer one to a block of as many threads as it fills.  Backward reads h and the two gradients once, writes dh
+// once and keeps the column sums of dw in registers over all rows of a persistent block; a second kernel adds the
+// blocks' sums in a fixed order (no atomics).
 //
 // As codes: with t = h w and a = max |t| over 128 columns, code = e4m3(t * (448 / a)) and scale = a / 448 * r.
 // The row's statistic enters the scale alone, so the codes are ready before the sum of squares is, and do not
@@ -17,27 +18,21 @@
 namespace gnnagg {
 namespace {
 
-constexpr int kRowThreads = 256;             // block of the warp-per-row and the block-per-row forms
-constexpr int kWideThreads = 1024;           // block of the widest rows
+constexpr int kRowThreads = 256;    // block of the warp-per-row forms: eight rows at a time
+constexpr int kBlockThreads = 512;  // largest block of the block-per-row forms
+constexpr int kWideThreads = 1024;  // block of rows too wide for these
 constexpr int kMaxWidth = 16384;
 
-template <int GT>
-struct Shape {
-    static constexpr int kThreads = GT == 32 ? kRowThreads : GT;
-    static constexpr int kRows = kThreads / GT;  // rows a block works on at once
-};
-
-// Sum over the GT threads of a row; every thread gets it.  `red` holds a value per warp.
-template <int GT>
+// Sum over the threads of a row (WARP: a warp, else the block); every thread gets it.  `red` holds a value per warp.
+template <bool WARP>
 __device__ __forceinline__ float row_sum(float v, float *red) {
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(kFullMask, v, off);
-    if (GT == 32) return v;
+    if (WARP) return v;
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
     float s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < GT / 32; ++i) s += red[i];
+    for (int i = 0; i < (int)blockDim.x / 32; ++i) s += red[i];
     return s;
 }
 
@@ -71,76 +66,88 @@ struct FwdParams {
     float eps;
 };
 
-template <typename T, int GT, int NV, bool VEC, bool FP8>
-__global__ void __launch_bounds__(Shape<GT>::kThreads) rms_norm_fwd_kernel(const FwdParams p) {
+// NV chunks a thread and row, R rows a warp at once.
+template <typename T, bool WARP, int NV, int R, bool VEC, bool FP8>
+__global__ void __launch_bounds__(WARP ? kRowThreads : kBlockThreads) rms_norm_fwd_kernel(const FwdParams p) {
     constexpr int V = Vec<T>::N;
     __shared__ float red[32];
-    const int lane = threadIdx.x % GT;
-    const int64_t row = (int64_t)blockIdx.x * Shape<GT>::kRows + threadIdx.x / GT;
-    if (GT == 32 && row >= p.rows) return;  // whole warps; a wider row's block has a row of its own
-    const T *x = static_cast<const T *>(p.x) + row * p.ldx;
-    const T *res = static_cast<const T *>(p.residual) + row * p.ldr;
-    float v[NV][V];
-    float ss = 0.0f;
+    const int lane = WARP ? threadIdx.x & 31 : threadIdx.x, step = WARP ? 32 : blockDim.x;
+    const int64_t row0 = WARP ? ((int64_t)blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5)) * R : blockIdx.x;
+    if (WARP && row0 >= p.rows) return;  // whole warps
+    uint4 h[R][NV], res[R][NV];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const int col = (lane + GT * j) * V, valid = p.F - col;
+    for (int k = 0; k < R; ++k)
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[j][i] = 0.0f;
-        if (valid > 0) {
-            load_chunk<T, VEC>(x + col, valid, v[j]);
+        for (int j = 0; j < NV; ++j) {
+            const int col = (lane + step * j) * V, valid = p.F - col;
+            const bool in = valid > 0 && (R == 1 || row0 + k < p.rows);
+            h[k][j] = res[k][j] = make_uint4(0, 0, 0, 0);
+            if (in) h[k][j] = load_raw<T, VEC>(static_cast<const T *>(p.x) + (row0 + k) * p.ldx + col, valid);
+            if (in && p.residual != nullptr)
+                res[k][j] = load_raw<T, VEC>(static_cast<const T *>(p.residual) + (row0 + k) * p.ldr + col, valid);
+        }
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+        const int64_t row = row0 + k;
+        if (R > 1 && row >= p.rows) break;
+        float ss = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            float v[V];
+            unpack16<T>(h[k][j], v);
             if (p.residual != nullptr) {
                 float r[V];
-                load_chunk<T, VEC>(res + col, valid, r);
+                unpack16<T>(res[k][j], r);
 #pragma unroll
-                for (int i = 0; i < V; ++i) v[j][i] = to_f32(from_f32<T>(v[j][i] + r[i]));
+                for (int i = 0; i < V; ++i) v[i] += r[i];
+                h[k][j] = pack16<T>(v);
+                unpack16<T>(h[k][j], v);  // the norm is of the rounded sum
+                const int col = (lane + step * j) * V, valid = p.F - col;
+                if (valid > 0) store_raw<T, VEC>(static_cast<T *>(p.h) + row * p.ldh + col, valid, h[k][j]);
             }
+#pragma unroll
+            for (int i = 0; i < V; ++i) ss = fmaf(v[i], v[i], ss);
         }
+        const float rstd = rsqrtf(row_sum<WARP>(ss, red) / (float)p.F + p.eps);
+        if (lane == 0 && p.rstd != nullptr) p.rstd[row] = rstd;
 #pragma unroll
-        for (int i = 0; i < V; ++i) ss = fmaf(v[j][i], v[j][i], ss);
-    }
-    const float rstd = rsqrtf(row_sum<GT>(ss, red) / (float)p.F + p.eps);
-    if (lane == 0 && p.rstd != nullptr) p.rstd[row] = rstd;
+        for (int j = 0; j < NV; ++j) {
+            const int col = (lane + step * j) * V, valid = p.F - col;
+            float v[V], w[V];
+            unpack16<T>(h[k][j], v);
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const int col = (lane + GT * j) * V, valid = p.F - col;
-        float w[V];
+            for (int i = 0; i < V; ++i) w[i] = 0.0f;
+            if (valid > 0) load_weight<T, VEC>(p.w, p.w_f32 != 0, col, valid, w);
+            if (!FP8) {
+                if (valid > 0) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) w[i] = 0.0f;
-        if (valid > 0) {
-            if (p.residual != nullptr)
-                store_chunk<T, VEC>(static_cast<T *>(p.h) + row * p.ldh + col, valid, v[j]);
-            load_weight<T, VEC>(p.w, p.w_f32 != 0, col, valid, w);
-        }
-        if (!FP8) {
-            if (valid > 0) {
+                    for (int i = 0; i < V; ++i) v[i] = v[i] * rstd * w[i];
+                    store_chunk<T, VEC>(static_cast<T *>(p.y) + row * p.ldy + col, valid, v);
+                }
+            } else {
+                uint32_t m = 0;
 #pragma unroll
-                for (int i = 0; i < V; ++i) v[j][i] = v[j][i] * rstd * w[i];
-                store_chunk<T, VEC>(static_cast<T *>(p.y) + row * p.ldy + col, valid, v[j]);
-            }
-        } else {
-            uint32_t m = 0;
+                for (int i = 0; i < V; ++i) {
+                    v[i] = __fmul_rn(v[i], w[i]);
+                    m = max(m, abs_bits(v[i]));
+                }
+                // 128 columns are 128 / V neighbouring threads: a whole or half a warp
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                v[j][i] = __fmul_rn(v[j][i], w[i]);
-                m = max(m, abs_bits(v[j][i]));
-            }
-            // 128 columns are 128 / V neighbouring threads: a whole or half a warp
+                for (int off = 64 / V; off > 0; off >>= 1) m = max(m, __shfl_xor_sync(kFullMask, m, off));
+                const float a = block_amax(m), f = block_factor(a);
+                if (valid > 0) {
+                    // code rows are padded to 16 bytes, so a whole chunk always fits; columns from F on are zeros
+                    uint32_t c[V / 4];
 #pragma unroll
-            for (int off = 64 / V; off > 0; off >>= 1) m = max(m, __shfl_xor_sync(kFullMask, m, off));
-            const float a = block_amax(m), f = block_factor(a);
-            if (valid > 0) {
-                // code rows are padded to 16 bytes, so a whole chunk always fits; columns from F on are zeros
-                uint32_t c[V / 4];
-#pragma unroll
-                for (int i = 0; i < V / 4; ++i)
-                    c[i] = e4m3x4(v[j][4 * i] * f, v[j][4 * i + 1] * f, v[j][4 * i + 2] * f, v[j][4 * i + 3] * f);
-                uint32_t *dst = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(p.y) + row * p.ldy + col);
-                if (V == 8)
-                    *reinterpret_cast<uint2 *>(dst) = make_uint2(c[0], c[V / 4 - 1]);
-                else
-                    *dst = c[0];
-                if ((col & 127) == 0) p.scales[(int64_t)(col >> 7) * p.lds + row] = block_scale(a) * rstd;
+                    for (int i = 0; i < V / 4; ++i)
+                        c[i] = e4m3x4(v[4 * i] * f, v[4 * i + 1] * f, v[4 * i + 2] * f, v[4 * i + 3] * f);
+                    uint32_t *dst = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(p.y) + row * p.ldy + col);
+                    if (V == 8)
+                        __stcs(reinterpret_cast<uint2 *>(dst), make_uint2(c[0], c[V / 4 - 1]));
+                    else
+                        __stcs(dst, c[0]);
+                    if ((col & 127) == 0) p.scales[(int64_t)(col >> 7) * p.lds + row] = block_scale(a) * rstd;
+                }
             }
         }
     }
@@ -156,64 +163,71 @@ struct BwdParams {
     int F, w_f32;
 };
 
-template <typename T, int GT, int NV, bool VEC>
-__global__ void __launch_bounds__(Shape<GT>::kThreads) rms_norm_bwd_kernel(const BwdParams p) {
+template <typename T, bool WARP, int NV, bool VEC>
+__global__ void __launch_bounds__(WARP ? kRowThreads : kBlockThreads) rms_norm_bwd_kernel(const BwdParams p) {
     constexpr int V = Vec<T>::N;
-    constexpr int kRows = Shape<GT>::kRows;
+    constexpr int kRows = WARP ? kRowThreads / 32 : 1;
     __shared__ float red[2][32];
-    __shared__ float cols[GT == 32 ? kRows * 32 * V : 1];
-    const int lane = threadIdx.x % GT, slot = threadIdx.x / GT;
+    __shared__ float cols[WARP ? kRows * 32 * V : 1];
+    const int lane = WARP ? threadIdx.x & 31 : threadIdx.x, step = WARP ? 32 : blockDim.x, slot = WARP ? threadIdx.x >> 5 : 0;
     const float inv_f = 1.0f / (float)p.F;
-    float w[NV][V], dw[NV][V];
+    float dw[NV][V];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const int col = (lane + GT * j) * V, valid = p.F - col;
+    for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int i = 0; i < V; ++i) w[j][i] = 0.0f, dw[j][i] = 0.0f;
-        if (valid > 0) load_weight<T, VEC>(p.w, p.w_f32 != 0, col, valid, w[j]);
-    }
+        for (int i = 0; i < V; ++i) dw[j][i] = 0.0f;
     int turn = 0;
     for (int64_t row = (int64_t)blockIdx.x * kRows + slot; row < p.rows; row += (int64_t)gridDim.x * kRows, turn ^= 1) {
+        uint4 h[NV], g[NV], gh[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int col = (lane + step * j) * V, valid = p.F - col;
+            h[j] = g[j] = gh[j] = make_uint4(0, 0, 0, 0);
+            if (valid > 0) {
+                h[j] = load_raw<T, VEC>(static_cast<const T *>(p.h) + row * p.ldh + col, valid);
+                g[j] = load_raw<T, VEC>(static_cast<const T *>(p.gy) + row * p.ldgy + col, valid);
+                if (p.gh != nullptr) gh[j] = load_raw<T, VEC>(static_cast<const T *>(p.gh) + row * p.ldgh + col, valid);
+            }
+        }
         const float rstd = __ldg(p.rstd + row);
-        float hat[NV][V], g[NV][V], gh[NV][V];
         float s = 0.0f;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int col = (lane + GT * j) * V, valid = p.F - col;
+            const int col = (lane + step * j) * V, valid = p.F - col;
+            float x[V], y[V], w[V];
+            unpack16<T>(h[j], x);
+            unpack16<T>(g[j], y);
 #pragma unroll
-            for (int i = 0; i < V; ++i) hat[j][i] = 0.0f, g[j][i] = 0.0f, gh[j][i] = 0.0f;
-            if (valid > 0) {
-                load_chunk<T, VEC>(static_cast<const T *>(p.h) + row * p.ldh + col, valid, hat[j]);
-                load_chunk<T, VEC>(static_cast<const T *>(p.gy) + row * p.ldgy + col, valid, g[j]);
-                if (p.gh != nullptr)
-                    load_chunk<T, VEC>(static_cast<const T *>(p.gh) + row * p.ldgh + col, valid, gh[j]);
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
+            for (int i = 0; i < V; ++i) w[i] = 0.0f;
+            if (valid > 0) load_weight<T, VEC>(p.w, p.w_f32 != 0, col, valid, w);  // from L1: cheaper than its registers
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                hat[j][i] *= rstd;
-                dw[j][i] = fmaf(g[j][i], hat[j][i], dw[j][i]);
-                g[j][i] *= w[j][i];
-                s = fmaf(g[j][i], hat[j][i], s);
+                const float hat = x[i] * rstd;
+                dw[j][i] = fmaf(y[i], hat, dw[j][i]);
+                s = fmaf(y[i] * w[i], hat, s);
             }
-        const float c = row_sum<GT>(s, red[turn]) * inv_f;  // two buffers: a warp may be a row ahead of another
+        }
+        const float c = row_sum<WARP>(s, red[turn]) * inv_f;  // two buffers: a warp may be a row ahead of another
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int col = (lane + GT * j) * V, valid = p.F - col;
+            const int col = (lane + step * j) * V, valid = p.F - col;
             if (valid > 0) {
+                float x[V], y[V], w[V], o[V];
+                unpack16<T>(h[j], x);
+                unpack16<T>(g[j], y);
+                unpack16<T>(gh[j], o);
+                load_weight<T, VEC>(p.w, p.w_f32 != 0, col, valid, w);
 #pragma unroll
-                for (int i = 0; i < V; ++i) gh[j][i] = fmaf(rstd, g[j][i] - hat[j][i] * c, gh[j][i]);
-                store_chunk<T, VEC>(static_cast<T *>(p.gx) + row * p.ldgx + col, valid, gh[j]);
+                for (int i = 0; i < V; ++i) o[i] = fmaf(rstd, y[i] * w[i] - x[i] * rstd * c, o[i]);
+                store_chunk<T, VEC>(static_cast<T *>(p.gx) + row * p.ldgx + col, valid, o);
             }
         }
     }
     float *out = p.partial + (int64_t)blockIdx.x * p.F;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const int col = (lane + GT * j) * V;
-        if (GT == 32) {  // the block's warps add up in warp order
+        const int col = (lane + step * j) * V;
+        if (WARP) {  // the block's warps add up in warp order
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < V; ++i) cols[(slot * V + i) * 32 + lane] = dw[j][i];
@@ -262,7 +276,7 @@ __global__ void __launch_bounds__(kWideThreads) rms_norm_bwd_wide_kernel(const B
                 s = fmaf(g[i] * w[i], hat[i], s);
             }
         }
-        const float c = row_sum<kWideThreads>(s, red[turn]) * inv_f;
+        const float c = row_sum<false>(s, red[turn]) * inv_f;
         for (int k = threadIdx.x; k < chunks; k += kWideThreads) {
             const int col = k * V, valid = p.F - col;
             float hat[V], g[V], w[V], gh[V];
@@ -284,44 +298,23 @@ __global__ void __launch_bounds__(kWideThreads) rms_norm_bwd_wide_kernel(const B
             if (k * V + i < p.F) out[k * V + i] = dw[i * chunks + k];
 }
 
-// dw[c] = sum of partial[b][c] over the blocks, in a fixed order: 16 threads take every 16th block of a column.
-template <typename T>
-__global__ void __launch_bounds__(512) rms_norm_dw_kernel(const float *__restrict__ partial, int blocks, int F, T *dw) {
-    __shared__ float red[16][33];
-    const int c = blockIdx.x * 32 + threadIdx.x;
-    float s = 0.0f;
-    if (c < F) {
-#pragma unroll 8
-        for (int b = threadIdx.y; b < blocks; b += 16) s += partial[(int64_t)b * F + c];
-    }
-    red[threadIdx.y][threadIdx.x] = s;
-    __syncthreads();
-    if (threadIdx.y == 0 && c < F) {
-#pragma unroll
-        for (int i = 1; i < 16; ++i) s += red[i][threadIdx.x];
-        dw[c] = from_f32<T>(s);
-    }
-}
-
-// How a row of F elements of `size` bytes is spread: threads per row and 16-byte chunks per thread.
+// How a row of F elements of `size` bytes is spread: over a warp (threads = 32) or a block, with nv 16-byte chunks a
+// thread; nv = 0: too wide for registers.
 struct Spread {
-    int gt, nv;
+    int threads, nv;
 };
 Spread spread_of(int F, int size) {
     const int chunks = (int)div_up(F, 16 / size);
-    if (chunks <= 32) return {32, 1};
-    if (chunks <= 64) return {32, 2};
-    if (chunks <= 128) return {32, 4};
-    if (chunks <= 256) return {256, 1};
-    if (chunks <= 512) return {256, 2};
-    if (chunks <= 1024) return {256, 4};
-    return {kWideThreads, 4};
+    if (chunks <= 128) return {32, chunks <= 32 ? 1 : chunks <= 64 ? 2 : 4};
+    const int nv = chunks <= 256 ? 1 : chunks <= 2 * kBlockThreads ? 2 : 4;
+    if (chunks > 4 * kBlockThreads) return {kWideThreads, 0};
+    return {(int)div_up(div_up(chunks, nv), 32) * 32, nv};
 }
 
 int bwd_blocks(int64_t rows, int F, int size) {
     const Spread s = spread_of(F, size);
-    const int64_t need = div_up(rows, s.gt == 32 ? kRowThreads / 32 : 1);
-    const int64_t cap = (int64_t)kNumSMs * (s.gt == kWideThreads ? 2 : 4);
+    const int64_t need = div_up(rows, s.threads == 32 ? kRowThreads / 32 : 1);
+    const int64_t cap = (int64_t)kNumSMs * (s.nv == 0 ? 2 : 4);
     return (int)(need < cap ? need : cap);
 }
 
@@ -333,30 +326,31 @@ int by_type(int type, F32 a, BF16 b, F16 c) {
 template <typename T, bool VEC, bool FP8>
 int launch_fwd(const FwdParams &p, cudaStream_t st) {
     const Spread s = spread_of(p.F, (int)sizeof(T));
-    const int64_t blocks = s.gt == 32 ? div_up(p.rows, kRowThreads / 32) : p.rows;
-    const dim3 grid((unsigned)blocks);
-#define RMS_LAUNCH(GT, NV) rms_norm_fwd_kernel<T, GT, NV, VEC, FP8><<<grid, Shape<GT>::kThreads, 0, st>>>(p)
-    if (s.gt == 32 && s.nv == 1) RMS_LAUNCH(32, 1);
-    else if (s.gt == 32 && s.nv == 2) RMS_LAUNCH(32, 2);
-    else if (s.gt == 32) RMS_LAUNCH(32, 4);
-    else if (s.gt == 256 && s.nv == 1) RMS_LAUNCH(256, 1);
-    else if (s.gt == 256 && s.nv == 2) RMS_LAUNCH(256, 2);
-    else if (s.gt == 256) RMS_LAUNCH(256, 4);
-    else RMS_LAUNCH(kWideThreads, 4);
-#undef RMS_LAUNCH
+#define RMS_WARP(NV, R) \
+    rms_norm_fwd_kernel<T, true, NV, R, VEC, FP8><<<(unsigned)div_up(p.rows, kRowThreads / 32 * R), kRowThreads, 0, st>>>(p)
+#define RMS_BLOCK(NV, THREADS) rms_norm_fwd_kernel<T, false, NV, 1, VEC, FP8><<<(unsigned)p.rows, THREADS, 0, st>>>(p)
+    if (s.threads == 32 && s.nv == 1) RMS_WARP(1, 2);
+    else if (s.threads == 32 && s.nv == 2) RMS_WARP(2, 1);
+    else if (s.threads == 32) RMS_WARP(4, 1);
+    else if (s.nv == 1) RMS_BLOCK(1, s.threads);
+    else if (s.nv == 2) RMS_BLOCK(2, s.threads);
+    else if (s.nv == 4) RMS_BLOCK(4, s.threads);
+    else RMS_BLOCK(8, kBlockThreads);  // fp32 rows above 8192 columns
+#undef RMS_WARP
+#undef RMS_BLOCK
     return check_launch("rms_norm_fwd_kernel");
 }
 
 template <typename T, bool VEC>
 int launch_bwd(const BwdParams &p, int blocks, cudaStream_t st) {
     const Spread s = spread_of(p.F, (int)sizeof(T));
-#define RMS_LAUNCH(GT, NV) rms_norm_bwd_kernel<T, GT, NV, VEC><<<blocks, Shape<GT>::kThreads, 0, st>>>(p)
-    if (s.gt == 32 && s.nv == 1) RMS_LAUNCH(32, 1);
-    else if (s.gt == 32 && s.nv == 2) RMS_LAUNCH(32, 2);
-    else if (s.gt == 32) RMS_LAUNCH(32, 4);
-    else if (s.gt == 256 && s.nv == 1) RMS_LAUNCH(256, 1);
-    else if (s.gt == 256 && s.nv == 2) RMS_LAUNCH(256, 2);
-    else if (s.gt == 256) RMS_LAUNCH(256, 4);
+#define RMS_LAUNCH(WARP, NV, THREADS) rms_norm_bwd_kernel<T, WARP, NV, VEC><<<blocks, THREADS, 0, st>>>(p)
+    if (s.threads == 32 && s.nv == 1) RMS_LAUNCH(true, 1, kRowThreads);
+    else if (s.threads == 32 && s.nv == 2) RMS_LAUNCH(true, 2, kRowThreads);
+    else if (s.threads == 32) RMS_LAUNCH(true, 4, kRowThreads);
+    else if (s.nv == 1) RMS_LAUNCH(false, 1, s.threads);
+    else if (s.nv == 2) RMS_LAUNCH(false, 2, s.threads);
+    else if (s.nv == 4) RMS_LAUNCH(false, 4, s.threads);
     else {
         static PerDeviceOnce attr_done;
         const cudaError_t e = attr_done.run([] {
@@ -373,8 +367,8 @@ int launch_bwd(const BwdParams &p, int blocks, cudaStream_t st) {
 
 template <typename T>
 int launch_dw(const float *partial, int blocks, int F, void *dw, cudaStream_t st) {
-    rms_norm_dw_kernel<T><<<(unsigned)div_up(F, 32), dim3(32, 16), 0, st>>>(partial, blocks, F, static_cast<T *>(dw));
-    return check_launch("rms_norm_dw_kernel");
+    column_sum_kernel<T><<<(unsigned)div_up(F, 32), dim3(32, 16), 0, st>>>(partial, blocks, F, static_cast<T *>(dw));
+    return check_launch("column_sum_kernel");
 }
 
 // 16-byte accesses of rows at p with a stride of ld elements

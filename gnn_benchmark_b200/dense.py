@@ -318,29 +318,33 @@ FP8 = torch.float8_e4m3fn
 FP8_BLOCK = 128
 
 
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """`t` itself when its rows are contiguous and do not overlap, else a copy."""
+    return t if t.stride(1) == 1 and t.stride(0) >= t.size(1) else t.contiguous()
+
+
 def _quantize(x: torch.Tensor, block_rows: int, rows: bool, cols: bool):
     """(codes, scales, codes_t, scales_t) of x from one read; the pair that is not asked for is None, None."""
     if x.dim() != 2 or x.dtype not in _lib.TYPES:
         raise RuntimeError(f"quantize_fp8: x must be a float32, bfloat16 or float16 matrix, not {tuple(x.shape)} {x.dtype}")
     _lib.require_cuda(x)
     m, k = x.shape
-    if x.stride(1) != 1 or x.stride(0) < k:
-        x = x.contiguous()
-    high = (m + 127) // 128 if block_rows == 128 else m
-    wide = (k + 127) // 128 if block_rows == 128 else k
+    x = _rows(x)
     codes = scales = codes_t = scales_t = None
     args, args_t = (0, 0, 0, 0), (0, 0, 0, 0)
     if rows:
         codes, scales = _lib.empty_codes(m, k, x.device)
-        scales = scales if high == m else torch.empty(((k + 127) // 128, high), dtype=torch.float32, device=x.device).t()
-        args = (codes.data_ptr(), codes.stride(0), scales.data_ptr(), high)
+        if block_rows == 128:
+            scales = _lib.empty_scales((m + 127) // 128, k, x.device)
+        args = (codes.data_ptr(), codes.stride(0), scales.data_ptr(), scales.stride(1))
     if cols:
         codes_t, scales_t = _lib.empty_codes(k, m, x.device)
-        scales_t = scales_t if wide == k else torch.empty(((m + 127) // 128, wide), dtype=torch.float32, device=x.device).t()
-        args_t = (codes_t.data_ptr(), codes_t.stride(0), scales_t.data_ptr(), wide)
+        if block_rows == 128:
+            scales_t = _lib.empty_scales((k + 127) // 128, m, x.device)
+        args_t = (codes_t.data_ptr(), codes_t.stride(0), scales_t.data_ptr(), scales_t.stride(1))
     with _lib.device_of(x):
         rc = _lib.lib().gnnagg_fp8_quantize(x.data_ptr(), max(x.stride(0), k), m, k, _lib.TYPES[x.dtype], block_rows, *args, *args_t,
-                                            _lib.stream_ptr(x.device))
+                                            0, _lib.stream_ptr(x.device))
     _lib.check(rc, "fp8_quantize")
     return codes, scales, codes_t, scales_t
 
@@ -359,20 +363,22 @@ def quantize_fp8(x: torch.Tensor, block=(1, 128), transpose: bool = False):
     return r[2:] if transpose else r[:2]
 
 
-def _operand(name: str, codes: torch.Tensor, scales: torch.Tensor, device):
+def _operand(name: str, codes: torch.Tensor, scales: torch.Tensor, index: int):
     """(rows that a scale covers, row stride) of a checked operand."""
-    if codes.dim() != 2 or codes.dtype != FP8 or codes.device != device:
+    if codes.dim() != 2 or codes.dtype != FP8 or codes.get_device() != index:
         raise RuntimeError(f"matmul_fp8: {name} must be a float8_e4m3fn matrix on the operands' device")
     rows, k = codes.shape
-    ld = codes.stride(0) if rows > 1 and k > 0 else (k + 15) // 16 * 16 + 16
-    if rows > 0 and k > 0 and (codes.stride(1) != 1 and k > 1 or ld < k or ld % 16 != 0 or codes.data_ptr() % 16 != 0):
+    high, kb = (rows + 127) // 128, (k + 127) // 128
+    ld, step = codes.stride()
+    if rows <= 1 or k == 0:  # torch may keep any stride
+        ld = kb * 128
+    if rows > 0 and k > 0 and (step != 1 and k > 1 or ld < k or ld % 16 != 0 or codes.data_ptr() % 16 != 0):
         raise RuntimeError(f"matmul_fp8: {name}'s rows must be contiguous and start on 16 bytes (as quantize_fp8 lays them)")
-    kb = (k + 127) // 128
-    if scales.dim() != 2 or scales.dtype != torch.float32 or scales.device != device or scales.size(1) != kb \
-            or scales.size(0) not in (rows, (rows + 127) // 128):
-        raise RuntimeError(f"matmul_fp8: {name}'s scales must be float32 ({rows} or {(rows + 127) // 128}, {kb}), "
-                           f"not {tuple(scales.shape)} {scales.dtype}")
-    return (1 if scales.size(0) == rows else 128), ld
+    shape = scales.shape
+    if scales.dtype != torch.float32 or scales.get_device() != index or (shape != (rows, kb) and shape != (high, kb)):
+        raise RuntimeError(f"matmul_fp8: {name}'s scales must be float32 ({rows} or {high}, {kb}) on the operands' device, "
+                           f"not {tuple(shape)} {scales.dtype}")
+    return (1 if shape[0] == rows else 128), ld
 
 
 def matmul_fp8(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor,
@@ -380,41 +386,51 @@ def matmul_fp8(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scale
                accumulate: bool = False) -> torch.Tensor:
     """out (M, N) (+)= (a * a_scales) @ (b * b_scales).T (+ bias): a (M, K) and b (N, K) float8_e4m3fn with float32
     scales for each block of 128 along K, one per row, (rows, ceil(K / 128)), or per 128 rows.  out_dtype float32,
-    bfloat16 or float16 (out's type when out is given); bias float32 (N,); accumulate needs a float32 out."""
-    _lib.require_cuda(a, a_scales, b, b_scales, bias, out)
-    device = a.device
-    a_block, lda = _operand("a", a, a_scales, device)
-    b_block, ldb = _operand("b", b, b_scales, device)
+    bfloat16 or float16 (out's type when out is given); bias (N,) of one of these; accumulate needs a float32 out."""
+    if not a.is_cuda:
+        _lib.require_cuda(a)
+    device, index = a.device, a.get_device()
+    a_block, lda = _operand("a", a, a_scales, index)
+    b_block, ldb = _operand("b", b, b_scales, index)
     m, k = a.shape
-    n = b.size(0)
-    if b.size(1) != k:
+    n, kb = b.shape
+    if kb != k:
         raise RuntimeError(f"matmul_fp8: shape mismatch a={tuple(a.shape)} b={tuple(b.shape)}")
-    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,) or not bias.is_contiguous()
-                             or bias.device != device):
-        raise RuntimeError("matmul_fp8: bias must be a contiguous float32 vector of N elements on the operands' device")
+    bias_ptr = bias_type = 0
+    if bias is not None:
+        if bias.dtype not in _lib.TYPES or bias.shape != (n,) or not bias.is_contiguous() or bias.get_device() != index:
+            raise RuntimeError("matmul_fp8: bias must be a contiguous float32, bfloat16 or float16 vector of N elements on the "
+                               "operands' device")
+        bias_ptr, bias_type = bias.data_ptr(), _lib.TYPES[bias.dtype]
     if out is None:
         if accumulate:
             raise RuntimeError("matmul_fp8: accumulate needs an output to accumulate into")
         if out_dtype not in _lib.TYPES:
             raise RuntimeError("matmul_fp8: out_dtype must be float32, bfloat16 or float16")
         out = torch.empty((m, n), dtype=out_dtype, device=device)
-    elif out.shape != (m, n) or out.dtype not in _lib.TYPES or out.device != device \
-            or (out.numel() > 0 and (out.stride(1) != 1 and n > 1 or out.stride(0) < n)):
-        raise RuntimeError("matmul_fp8: out must be (M, N) float32, bfloat16 or float16 with contiguous rows")
-    if accumulate and out.dtype != torch.float32:
-        raise RuntimeError("matmul_fp8: accumulate needs a float32 output")
+        ldc = n
+    else:
+        out_dtype, ldc = out.dtype, out.stride(0) if m > 1 else n
+        if out.shape != (m, n) or out_dtype not in _lib.TYPES or out.get_device() != index \
+                or (out.numel() > 0 and (out.stride(1) != 1 and n > 1 or ldc < n)):
+            raise RuntimeError("matmul_fp8: out must be (M, N) float32, bfloat16 or float16 with contiguous rows on the operands' "
+                               "device")
+        if accumulate and out_dtype != torch.float32:
+            raise RuntimeError("matmul_fp8: accumulate needs a float32 output")
     lib = _lib.lib()
-    ws_bytes = lib.gnnagg_fp8_matmul_workspace_bytes(m, n, k)
-    # from the caching allocator at every call: ordered with the stream, and a captured graph has its own
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes else None
-    _fp8_devices.add(device.index)
+    ws_ptr, ws_bytes = 0, lib.gnnagg_fp8_matmul_workspace_bytes(m, n, k)
+    if ws_bytes:
+        # from the caching allocator at every call: ordered with the stream, and a captured graph has its own
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
+        ws_ptr = ws.data_ptr()
+    _fp8_devices.add(index)
     with _lib.device_of(a):
-        rc = lib.gnnagg_fp8_matmul(a.data_ptr(), lda, a_scales.data_ptr(), a_scales.stride(0), a_scales.stride(1),
-                                   a_block, b.data_ptr(), ldb, b_scales.data_ptr(), b_scales.stride(0),
-                                   b_scales.stride(1), b_block, m, n, k, _lib.ptr(bias), 1 if accumulate else 0,
-                                   out.data_ptr(), max(out.stride(0), n), _lib.TYPES[out.dtype], _lib.ptr(ws), ws_bytes,
+        rc = lib.gnnagg_fp8_matmul(a.data_ptr(), lda, a_scales.data_ptr(), *a_scales.stride(), a_block, b.data_ptr(), ldb,
+                                   b_scales.data_ptr(), *b_scales.stride(), b_block, m, n, k, bias_ptr, bias_type,
+                                   1 if accumulate else 0, out.data_ptr(), ldc, _lib.TYPES[out_dtype], ws_ptr, ws_bytes,
                                    _lib.stream_ptr(device))
-    _lib.check(rc, "fp8_matmul")
+    if rc:
+        _lib.check(rc, "fp8_matmul")
     return out
 
 
@@ -425,27 +441,45 @@ class LinearFP8(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias):
-        need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        xq, xs, xt, xts = _quantize(x, 1, True, need_w)
-        wq, ws, wt, wts = _quantize(weight, 128, True, need_x)
-        ctx.save_for_backward(xt, xts, wt, wts)
-        ctx.types = x.dtype, weight.dtype, None if bias is None else bias.dtype
-        return matmul_fp8(xq, xs, wq, ws, bias=None if bias is None else bias.float(), out_dtype=x.dtype)
+        lib, device = _lib.lib(), x.device
+        (m, k), n = x.shape, weight.size(0)
+        x, weight = _rows(x), _rows(weight)
+        need_x, need_w = (1 if need else 0 for need in ctx.needs_input_grad[:2])
+        types = [_lib.TYPES[t.dtype] if t is not None else 0 for t in (x, weight, bias)]
+        kept_bytes = lib.gnnagg_fp8_linear_kept_bytes(m, n, k, need_x, need_w)
+        scratch_bytes = lib.gnnagg_fp8_linear_scratch_bytes(m, n, k, 0)
+        kept = torch.empty(kept_bytes, dtype=torch.uint8, device=device)
+        scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device=device)
+        y = torch.empty((m, n), dtype=x.dtype, device=device)
+        _fp8_devices.add(device.index)
+        with _lib.device_of(x):
+            rc = lib.gnnagg_fp8_linear_fwd(x.data_ptr(), max(x.stride(0), k), types[0], weight.data_ptr(),
+                                           max(weight.stride(0), k), types[1], _lib.ptr(bias), types[2], m, n, k, y.data_ptr(),
+                                           types[0], need_x, need_w, kept.data_ptr(), kept_bytes, scratch.data_ptr(),
+                                           scratch_bytes, _lib.stream_ptr(device))
+        _lib.check(rc, "fp8_linear_fwd")
+        ctx.save_for_backward(kept)
+        ctx.sizes, ctx.needs, ctx.types = (m, n, k), (need_x, need_w), types
+        ctx.dtypes = x.dtype, weight.dtype, None if bias is None else bias.dtype
+        return y
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        xt, xts, wt, wts = ctx.saved_tensors
-        x_type, w_type, b_type = ctx.types
-        need_x, need_w, need_b = ctx.needs_input_grad
-        gx = gw = gb = None
-        if need_b:
-            gb = g.sum(0, dtype=torch.float32).to(b_type)
-        if need_x or need_w:
-            gq, gs, gt, gts = _quantize(g, 1, need_x, need_w)
-        if need_x:
-            gx = matmul_fp8(gq, gs, wt, wts, out_dtype=x_type)
-        if need_w:
-            gw = matmul_fp8(gt, gts, xt, xts, out_dtype=w_type)
+        (kept,) = ctx.saved_tensors
+        (m, n, k), (need_x, need_w), types = ctx.sizes, ctx.needs, ctx.types
+        lib, device = _lib.lib(), g.device
+        g = _rows(g)
+        gx = torch.empty((m, k), dtype=ctx.dtypes[0], device=device) if need_x else None
+        gw = torch.empty((n, k), dtype=ctx.dtypes[1], device=device) if need_w else None
+        gb = torch.empty(n, dtype=ctx.dtypes[2], device=device) if ctx.needs_input_grad[2] else None
+        scratch_bytes = lib.gnnagg_fp8_linear_scratch_bytes(m, n, k, 1)
+        scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device=device)
+        with _lib.device_of(g):
+            rc = lib.gnnagg_fp8_linear_bwd(g.data_ptr(), max(g.stride(0), n), types[0], m, n, k, need_x, need_w,
+                                           kept.data_ptr(), kept.numel(), _lib.ptr(gx), types[0], _lib.ptr(gw), types[1],
+                                           _lib.ptr(gb), types[2], scratch.data_ptr(), scratch_bytes, _lib.stream_ptr(device))
+        _lib.check(rc, "fp8_linear_bwd")
         return gx, gw, gb
 
 
@@ -459,4 +493,4 @@ def linear_fp8(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor = None)
         raise RuntimeError("linear_fp8: x and weight must be float32, bfloat16 or float16 on one device")
     if bias is not None and (bias.shape != (weight.size(0),) or bias.dtype not in _lib.TYPES or bias.device != x.device):
         raise RuntimeError("linear_fp8: bias must be a float32, bfloat16 or float16 vector of N elements on x's device")
-    return LinearFP8.apply(x, weight, bias)
+    return LinearFP8.apply(x, weight, bias if bias is None or bias.is_contiguous() else bias.contiguous())

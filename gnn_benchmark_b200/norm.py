@@ -143,14 +143,15 @@ MAX_RMS_WIDTH = 16384
 
 
 def _check_rms(what: str, x: torch.Tensor, weight: torch.Tensor, residual) -> None:
-    if not (x.is_cuda and weight.is_cuda and (residual is None or residual.is_cuda)):
-        _lib.require_cuda(x, weight, residual)
-    if x.dim() != 2 or x.dtype not in _lib.TYPES or not 0 < x.size(1) <= MAX_RMS_WIDTH:
+    if not x.is_cuda:
+        _lib.require_cuda(x)
+    index, dtype, shape = x.get_device(), x.dtype, x.shape
+    if len(shape) != 2 or dtype not in _lib.TYPES or not 0 < shape[1] <= MAX_RMS_WIDTH:
         raise RuntimeError(f"{what}: x must be (rows, F) float32, bfloat16 or float16 with 1 <= F <= {MAX_RMS_WIDTH}, "
-                           f"not {tuple(x.shape)} {x.dtype}")
-    if weight.shape != x.shape[1:] or weight.dtype not in (x.dtype, torch.float32) or weight.device != x.device:
-        raise RuntimeError(f"{what}: weight must be a vector of {x.size(1)} elements of x's type or float32 on x's device")
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
+                           f"not {tuple(shape)} {dtype}")
+    if weight.shape != shape[1:] or weight.dtype not in (dtype, torch.float32) or weight.get_device() != index:
+        raise RuntimeError(f"{what}: weight must be a vector of {shape[1]} elements of x's type or float32 on x's device")
+    if residual is not None and (residual.shape != shape or residual.dtype != dtype or residual.get_device() != index):
         raise RuntimeError(f"{what}: residual must match x in shape, type and device")
 
 
@@ -171,8 +172,8 @@ def _vector(t: torch.Tensor) -> torch.Tensor:
 def _rms_forward(x, weight, residual, eps, need_rstd):
     rows, f = x.shape
     x, weight = _rows(x), _vector(weight)
-    y = torch.empty((rows, f), dtype=x.dtype, device=x.device)
-    rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if need_rstd else None
+    y = torch.empty_strided((rows, f), (f, 1), dtype=x.dtype, device=x.device)
+    rstd = torch.empty_strided((rows,), (1,), dtype=torch.float32, device=x.device) if need_rstd else None
     h, res_ptr, res_ld, h_ptr = x, 0, 0, 0
     if residual is not None:
         residual = _rows(residual)
@@ -182,7 +183,8 @@ def _rms_forward(x, weight, residual, eps, need_rstd):
         rc = _lib.lib().gnnagg_rms_norm_fwd(x.data_ptr(), _ld(x), res_ptr, res_ld, weight.data_ptr(),
                                             _lib.TYPES[weight.dtype], rows, f, _lib.TYPES[x.dtype], eps, h_ptr, f,
                                             y.data_ptr(), f, _lib.ptr(rstd), _lib.stream_ptr(x.device))
-    _lib.check(rc, "rms_norm_fwd")
+    if rc:
+        _lib.check(rc, "rms_norm_fwd")
     return y, h, rstd, weight
 
 
@@ -198,6 +200,7 @@ class _RMSNorm(torch.autograd.Function):
         return (y, h) if residual is not None else y
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, gy, gh=None):
         h, w, rstd = ctx.saved_tensors
         if gy is None:  # only the sum was used
@@ -205,16 +208,18 @@ class _RMSNorm(torch.autograd.Function):
         rows, f = h.shape
         gy = _rows(gy)
         gh = None if gh is None else _rows(gh)
-        gx = torch.empty((rows, f), dtype=h.dtype, device=h.device)
-        dw = torch.empty(f, dtype=w.dtype, device=h.device)
+        gx = torch.empty_strided((rows, f), (f, 1), dtype=h.dtype, device=h.device)
+        dw = torch.empty_like(w)
         lib, kind = _lib.lib(), _lib.TYPES[h.dtype]
-        partial = torch.empty(lib.gnnagg_rms_norm_partial_bytes(rows, f, kind), dtype=torch.uint8, device=h.device)
+        partial_bytes = lib.gnnagg_rms_norm_partial_bytes(rows, f, kind)
+        partial = torch.empty_strided((partial_bytes,), (1,), dtype=torch.uint8, device=h.device)
         with _lib.device_of(h):
             rc = lib.gnnagg_rms_norm_bwd(gy.data_ptr(), _ld(gy), _lib.ptr(gh), 0 if gh is None else _ld(gh),
                                          h.data_ptr(), _ld(h), rstd.data_ptr(), w.data_ptr(), _lib.TYPES[w.dtype],
                                          rows, f, kind, gx.data_ptr(), f, dw.data_ptr(), partial.data_ptr(),
-                                         partial.numel(), _lib.stream_ptr(h.device))
-        _lib.check(rc, "rms_norm_bwd")
+                                         partial_bytes, _lib.stream_ptr(h.device))
+        if rc:
+            _lib.check(rc, "rms_norm_bwd")
         return gx, dw, gx if ctx.has_residual else None, None
 
 
@@ -247,7 +252,7 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor =
     h, res_ptr, res_ld, h_ptr = None, 0, 0, 0
     if residual is not None:
         residual = _rows(residual)
-        h = torch.empty((rows, f), dtype=x.dtype, device=x.device)
+        h = torch.empty_strided((rows, f), (f, 1), dtype=x.dtype, device=x.device)
         res_ptr, res_ld, h_ptr = residual.data_ptr(), _ld(residual), h.data_ptr()
     with _lib.device_of(x):
         rc = _lib.lib().gnnagg_rms_norm_fp8(x.data_ptr(), _ld(x), res_ptr, res_ld, weight.data_ptr(),

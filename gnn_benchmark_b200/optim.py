@@ -7,7 +7,8 @@ tensors, `AdamW` the torch.optim.Optimizer around it.
 8-bit moments (`state_bits=8`) take 2.03 bytes a parameter instead of 8: e4m3 codes of the first moment and of the
 second moment's square root, in blocks of 256 elements with an fp32 scale each.
 """
-import ctypes
+from array import array
+from itertools import chain
 
 import torch
 
@@ -17,16 +18,15 @@ STATE_BLOCK = 256
 FP8 = torch.float8_e4m3fn
 
 
-class _Tensor(ctypes.Structure):
-    _fields_ = [("param", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("exp_avg", ctypes.c_void_p),
-                ("exp_avg_sq", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("master", ctypes.c_void_p),
-                ("n", ctypes.c_int64)]
-
-
-def _check(what, i, t, n, dtype, device):
-    if t.numel() != n or t.dtype != dtype or t.device != device or not t.is_contiguous():
-        raise RuntimeError(f"adamw_step: {what} {i} must be a contiguous {dtype} tensor of {n} elements on the "
-                           f"parameters' device, not {tuple(t.shape)} {t.dtype} on {t.device}")
+def _check(what, ts, sizes, dtype, index) -> None:
+    """The tensors of one list: their type, device, layout and number of elements."""
+    if {t.dtype for t in ts} == {dtype} and set(map(torch.Tensor.get_device, ts)) == {index} \
+            and all(map(torch.Tensor.is_contiguous, ts)) and list(map(torch.Tensor.numel, ts)) == sizes:
+        return
+    for i, (t, n) in enumerate(zip(ts, sizes)):
+        if t.dtype != dtype or t.get_device() != index or not t.is_contiguous() or t.numel() != n:
+            raise RuntimeError(f"adamw_step: {what} {i} must be a contiguous {dtype} tensor of {n} elements on the parameters' "
+                               f"device, not {tuple(t.shape)} {t.dtype} on {t.device}")
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr: float, betas=(0.9, 0.999), eps: float = 1e-8,
@@ -52,32 +52,34 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr: float, be
         raise RuntimeError("adamw_step: the first step is 1")
     if count == 0:
         return
-    device, dtype = params[0].device, params[0].dtype
+    device, dtype, index = params[0].device, params[0].dtype, params[0].get_device()
     _lib.require_cuda(params[0])
     if dtype not in _lib.TYPES:
         raise RuntimeError(f"adamw_step: parameters must be float32, bfloat16 or float16, not {dtype}")
     state = torch.float32 if scales is None else FP8
-    rows = []
-    for i in range(count):
-        p, g, m, v = params[i], grads[i], exp_avgs[i], exp_avg_sqs[i]
-        n = p.numel()
-        _check("parameter", i, p, n, dtype, device)
-        _check("gradient", i, g, n, dtype, device)
-        _check("exp_avg", i, m, n, state, device)
-        _check("exp_avg_sq", i, v, n, state, device)
-        s = w = 0
-        if scales is not None:
-            _check("scales", i, scales[i], (n + STATE_BLOCK - 1) // STATE_BLOCK * 2, torch.float32, device)
-            s = scales[i].data_ptr()
-        if masters is not None and masters[i] is not None:
-            _check("master", i, masters[i], n, torch.float32, device)
-            w = masters[i].data_ptr()
-        rows.append((p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), s, w, n))
-    table = (_Tensor * count)(*rows)
+    sizes = list(map(torch.Tensor.numel, params))
+    _check("parameter", params, sizes, dtype, index)
+    _check("gradient", grads, sizes, dtype, index)
+    _check("exp_avg", exp_avgs, sizes, state, index)
+    _check("exp_avg_sq", exp_avg_sqs, sizes, state, index)
+    pointers = torch.Tensor.data_ptr
+    scale_ptrs = master_ptrs = (0,) * count
+    if scales is not None:
+        _check("scales", scales, [-(-n // STATE_BLOCK) * 2 for n in sizes], torch.float32, index)
+        scale_ptrs = map(pointers, scales)
+    if masters is not None:
+        held = [(t, n) for t, n in zip(masters, sizes) if t is not None]
+        if held:
+            _check("master", [t for t, _ in held], [n for _, n in held], torch.float32, index)
+        master_ptrs = map(_lib.ptr, masters)
+    rows = zip(map(pointers, params), map(pointers, grads), map(pointers, exp_avgs), map(pointers, exp_avg_sqs), scale_ptrs,
+               master_ptrs, sizes)
+    table = array("q", chain.from_iterable(rows))  # entries of gnnagg_adamw_tensor: six pointers and a size
     with _lib.device_of(params[0]):
-        rc = _lib.lib().gnnagg_adamw_step(table, count, _lib.TYPES[dtype], 32 if scales is None else 8, lr, b1, b2, eps,
-                                          weight_decay, step, _lib.ptr(device_scalars), _lib.stream_ptr(device))
-    _lib.check(rc, "adamw_step")
+        rc = _lib.lib().gnnagg_adamw_step(table.buffer_info()[0], count, _lib.TYPES[dtype], 32 if scales is None else 8, lr, b1,
+                                          b2, eps, weight_decay, step, _lib.ptr(device_scalars), _lib.stream_ptr(device))
+    if rc:
+        _lib.check(rc, "adamw_step")
 
 
 def _zero_moment(bits: int, like: torch.Tensor) -> torch.Tensor:

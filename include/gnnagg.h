@@ -378,11 +378,12 @@ int gnnagg_rms_norm_bwd(const void *gy, int64_t ldgy, const void *gh, int64_t ld
  *   codes    [rows][ldc] with scales[i + j * lds] (i: row or row block, j: column group), and / or
  *   codes_t  [cols][ldt], the same for the transpose: blocks of 1 x 128 lie along x's columns.
  *   Code rows start on 16 bytes (ldc, ldt % 16 == 0); the padding behind a row is partly overwritten with zeros.
+ *   column_sums  optional [ceil(rows / 128)][cols]: sums of x over 128 rows each
  *
  * gnnagg_fp8_matmul: C[M,N] = sum_k A[m,k] sa[m,k/128] B[n,k] sb[n,k/128] (+ bias[N]) (+ C).
  *   a_block, b_block  rows that a scale covers: 1 or 128; the scale of (row or row block i, k-block j) is
  *             sa[i * sa_stride + j * sa_stride_k]
- *   out_type  GNNAGG_F32 / BF16 / F16; accumulate needs F32
+ *   out_type, bias_type  GNNAGG_F32 / BF16 / F16; accumulate needs an F32 output
  *   workspace gnnagg_fp8_matmul_workspace_bytes(M, N, K) bytes, 16-byte aligned; NULL when that is 0.  Its contents
  *             mean nothing between calls.
  * Sums are fp32: chains of 128 elements in tensor memory, their scaled sum in registers; a sum that is split over
@@ -393,15 +394,31 @@ int gnnagg_rms_norm_bwd(const void *gy, int64_t ldgy, const void *gh, int64_t ld
  * ---------------------------------------------------------------------------------- */
 int gnnagg_fp8_quantize(const void *x, int64_t ldx, int64_t rows, int64_t cols, int32_t type, int32_t block_rows,
                         uint8_t *codes, int64_t ldc, float *scales, int64_t lds, uint8_t *codes_t, int64_t ldt,
-                        float *scales_t, int64_t lds_t, void *stream);
+                        float *scales_t, int64_t lds_t, float *column_sums, void *stream);
 size_t gnnagg_fp8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int gnnagg_fp8_matmul(const uint8_t *A, int64_t lda, const float *sa, int64_t sa_stride, int64_t sa_stride_k,
                       int32_t a_block, const uint8_t *B, int64_t ldb, const float *sb, int64_t sb_stride,
-                      int64_t sb_stride_k, int32_t b_block, int64_t M, int64_t N, int64_t K, const float *bias,
-                      int32_t accumulate, void *C, int64_t ldc, int32_t out_type, void *workspace,
+                      int64_t sb_stride_k, int32_t b_block, int64_t M, int64_t N, int64_t K, const void *bias,
+                      int32_t bias_type, int32_t accumulate, void *C, int64_t ldc, int32_t out_type, void *workspace,
                       size_t workspace_bytes, void *stream);
 int gnnagg_fp8_matmul_status(void *stream);
 int gnnagg_fp8_matmul_status_clear(void *stream);
+
+/* A linear layer on these: y[M,N] = x[M,K] w[N,K]^T (+ bias[N]), with x rounded in blocks of 1 x 128 and w of
+ * 128 x 128, and its gradients gx = g w (g in blocks of 1 x 128), gw = g^T x (both in blocks of 128 rows), gb = column
+ * sums of g (unrounded).  What the backward needs of x (need_w) and of w (need_x) is left in `kept` as codes and
+ * scales; scratch means nothing after the call.  kept and scratch are 16-byte aligned, of the sizes that
+ * gnnagg_fp8_linear_kept_bytes and gnnagg_fp8_linear_scratch_bytes give.  Types as above, each of its own; y, gx, gw
+ * have contiguous rows; gx, gw, gb may be NULL (gx, gw need what was kept). */
+size_t gnnagg_fp8_linear_kept_bytes(int64_t M, int64_t N, int64_t K, int32_t need_x, int32_t need_w);
+size_t gnnagg_fp8_linear_scratch_bytes(int64_t M, int64_t N, int64_t K, int32_t backward);
+int gnnagg_fp8_linear_fwd(const void *x, int64_t ldx, int32_t x_type, const void *w, int64_t ldw, int32_t w_type,
+                          const void *bias, int32_t bias_type, int64_t M, int64_t N, int64_t K, void *y, int32_t y_type,
+                          int32_t need_x, int32_t need_w, void *kept, size_t kept_bytes, void *scratch,
+                          size_t scratch_bytes, void *stream);
+int gnnagg_fp8_linear_bwd(const void *g, int64_t ldg, int32_t g_type, int64_t M, int64_t N, int64_t K, int32_t need_x,
+                          int32_t need_w, const void *kept, size_t kept_bytes, void *gx, int32_t x_type, void *gw,
+                          int32_t w_type, void *gb, int32_t b_type, void *scratch, size_t scratch_bytes, void *stream);
 
 /* ------------------------------------------------------------------------------------
  * L3  AdamW over many tensors in one launch (no reference counterpart; the reference's optimiser is

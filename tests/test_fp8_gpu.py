@@ -292,7 +292,7 @@ def test_gpu_refusals():
                 lambda: dense.matmul_fp8(a, sa, b, sb, out=out, accumulate=True),
                 lambda: dense.matmul_fp8(a, sa, b, sb, out=out[:, :39]),
                 lambda: dense.matmul_fp8(a, sa, b, sb, bias=torch.zeros(39, device="cuda")),
-                lambda: dense.matmul_fp8(a, sa, b, sb, bias=torch.zeros(40, device="cuda").half()),
+                lambda: dense.matmul_fp8(a, sa, b, sb, bias=torch.zeros(40, device="cuda").double()),
                 lambda: dense.matmul_fp8(a, sa, b, sb, out_dtype=torch.float64), lambda: dense.matmul_fp8(a, sa.cpu(), b, sb),
                 lambda: dense.quantize_fp8(torch.zeros(4, 4, 4, device="cuda")), lambda: dense.quantize_fp8(out.double()),
                 lambda: dense.quantize_fp8(out, (1, 64)), lambda: dense.linear_fp8(out, out[:, :39])):

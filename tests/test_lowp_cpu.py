@@ -68,7 +68,7 @@ def test_product_status_codes(cuda_lib):
 
     def call(A=16, lda=256, sa=16, a_block=1, B=16, ldb=256, b_block=128, M=300, N=200, K=256, acc=0, C=16, ldc=200, t=1,
              ws=None, nb=0, stride=1):
-        return f(A, lda, sa, stride, 300, a_block, B, ldb, 16, 1, 2, b_block, M, N, K, None, acc, C, ldc, t, ws, nb, None)
+        return f(A, lda, sa, stride, 300, a_block, B, ldb, 16, 1, 2, b_block, M, N, K, None, 0, acc, C, ldc, t, ws, nb, None)
 
     assert call(M=-1) == -1 and call(a_block=64) == -1 and call(b_block=0) == -1 and call(t=5) == -1 and call(acc=2) == -1
     assert call(acc=1) == -2 and call(A=None) == -1 and call(C=None) == -1 and call(lda=255) == -1 and call(ldc=199) == -1
@@ -79,17 +79,36 @@ def test_product_status_codes(cuda_lib):
     assert call(M=40, N=200, K=20000, lda=20000, ldb=20000) == -4
     assert call(M=40, N=200, K=20000, lda=20000, ldb=20000, ws=16, nb=need - 1) == -4
     q = cuda_lib.gnnagg_fp8_quantize
-    assert q(16, 64, 4, 64, 0, 2, 16, 64, 16, 4, None, 0, None, 0, None) == -1
-    assert q(16, 64, 4, 64, 7, 1, 16, 64, 16, 4, None, 0, None, 0, None) == -1
-    assert q(16, 64, 4, 64, 0, 1, None, 0, None, 0, None, 0, None, 0, None) == -1
-    assert q(16, 63, 4, 64, 0, 1, 16, 64, 16, 4, None, 0, None, 0, None) == -1
-    assert q(16, 64, 4, 64, 0, 1, 16, 72, 16, 4, None, 0, None, 0, None) == -2
-    assert q(16, 64, 4, 64, 0, 1, 16, 64, 16, 3, None, 0, None, 0, None) == -1
-    assert q(16, 64, 0, 64, 0, 1, None, 0, None, 0, None, 0, None, 0, None) == 0
+    assert q(16, 64, 4, 64, 0, 2, 16, 64, 16, 4, None, 0, None, 0, None, None) == -1
+    assert q(16, 64, 4, 64, 7, 1, 16, 64, 16, 4, None, 0, None, 0, None, None) == -1
+    assert q(16, 64, 4, 64, 0, 1, None, 0, None, 0, None, 0, None, 0, None, None) == -1
+    assert q(16, 63, 4, 64, 0, 1, 16, 64, 16, 4, None, 0, None, 0, None, None) == -1
+    assert q(16, 64, 4, 64, 0, 1, 16, 72, 16, 4, None, 0, None, 0, None, None) == -2
+    assert q(16, 64, 4, 64, 0, 1, 16, 64, 16, 3, None, 0, None, 0, None, None) == -1
+    assert q(16, 64, 0, 64, 0, 1, None, 0, None, 0, None, 0, None, 0, None, None) == 0
+
+
+def test_linear_status_codes(cuda_lib):
+    kept, scratch = cuda_lib.gnnagg_fp8_linear_kept_bytes, cuda_lib.gnnagg_fp8_linear_scratch_bytes
+    assert kept(100, 50, 60, 0, 0) == 0 and 0 < kept(100, 50, 60, 1, 0) < kept(100, 50, 60, 1, 1)
+    assert scratch(100, 50, 60, 0) > 0 and scratch(100, 50, 60, 1) > 0 and kept(-1, 2, 3, 1, 1) == 0
+    nb, sb = kept(100, 50, 60, 1, 1), scratch(100, 50, 60, 0)
+
+    def fwd(M=100, kp=16, knb=nb, s=16, snb=sb, x=None):
+        return cuda_lib.gnnagg_fp8_linear_fwd(x, 60, 0, 16, 60, 0, None, 0, M, 50, 60, 16, 0, 1, 1, kp, knb, s, snb, None)
+
+    assert fwd(M=-1) == -1 and fwd(kp=None) == -4 and fwd(knb=nb - 1) == -4 and fwd(s=24) == -4 and fwd(snb=sb - 1) == -4
+    assert fwd() == -1  # x is null
+    b = cuda_lib.gnnagg_fp8_linear_bwd
+    assert b(16, 50, 0, 100, 50, 60, 0, 1, 16, nb, 16, 0, None, 0, None, 0, 16, 1 << 30, None) == -1  # gx, nothing kept for it
+    assert b(16, 50, 0, 100, 50, 60, 1, 1, 16, nb, 16, 0, None, 0, 16, 7, 16, 1 << 30, None) == -1
+    assert b(16, 50, 0, 100, 50, 60, 1, 1, 16, nb - 1, 16, 0, None, 0, None, 0, 16, 1 << 30, None) == -4
 
 
 def test_adamw_status_codes(cuda_lib):
-    from gnn_benchmark_b200.optim import _Tensor
+    class _Tensor(ctypes.Structure):
+        _fields_ = [(k, ctypes.c_void_p) for k in ("param", "grad", "exp_avg", "exp_avg_sq", "scales", "master")]
+        _fields_ += [("n", ctypes.c_int64)]
 
     f = cuda_lib.gnnagg_adamw_step
 
@@ -105,6 +124,5 @@ def test_adamw_status_codes(cuda_lib):
     assert call([(16, 16, 16, 16, None, None, -1)]) == -1
     assert call([good], bits=8) == -1 and call([(16, 16, 16, 16, 12, None, 8)], bits=8) == -2
     assert call([]) == 0 and call([(None, None, None, None, None, None, 0)]) == 0  # nothing to do, nothing launched
-    assert ctypes.sizeof(_Tensor) == 56
     assert cuda_lib.gnnagg_adamw_tick(None, None, 1e-3, 0.9, 0.999, 1e-8, 0.0, 16, None) == -1
     assert cuda_lib.gnnagg_adamw_tick(16, None, 1e-3, 1.0, 0.999, 1e-8, 0.0, 16, None) == -1
