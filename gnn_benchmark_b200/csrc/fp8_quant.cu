@@ -2,11 +2,14 @@
 // read: the operands of the 8-bit product.
 //
 // A block of the grid holds a 128 x 128 tile in registers, as it lies in memory: 256 threads, each V neighbouring
-// columns (16 bytes of input) of a run of neighbouring rows.  Largest magnitudes are maxima of bit patterns, by shuffles along a row and
-// by shared-memory atomics along columns (a maximum does not depend on the order).  Transposed codes go through a
-// 16 KB shared tile: 8 rows of a column are one 8-byte piece, at piece index XOR (column / V) so that a warp's
-// stores meet different banks, and leave as 16-byte stores.
-// Bound by memory: per element its bytes in and one byte out for each orientation.
+// columns (16 bytes of input) of a run of neighbouring rows.  Largest magnitudes are maxima of bit patterns, two 16-bit
+// elements an instruction; a run's rows are reduced across their 16 (32) threads by halving exchanges, so that a row's
+// reciprocal is taken once, and columns through a shared table of the runs' maxima.  Transposed codes go through a 16 KB
+// shared tile: 8 rows of a column are one 8-byte piece, at piece index XOR (column / V) so that a warp's stores meet
+// different banks, and leave as 16-byte stores.
+// Bound by memory: per element its bytes in and one byte out for each orientation.  What keeps it from the floor is
+// instruction issue: 7 instructions an element with both orientations (15 with a shuffle reduction per row and a
+// reciprocal per thread and column: 195 us at 16384 x 8192 bf16).
 #include "lowp.cuh"
 
 namespace gnnagg {
@@ -25,30 +28,50 @@ struct QuantParams {
     float *column_sums;            // [row blocks][cols] sums of x over a tile's rows, or null
 };
 
+// Magnitudes of a 32-bit word's elements (one fp32, or two 16-bit ones side by side) and their maxima, as bits.
+template <typename T>
+__device__ __forceinline__ uint32_t word_abs(uint32_t w) {
+    return sizeof(T) == 4 ? w & 0x7FFFFFFFu : w & 0x7FFF7FFFu;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t word_max(uint32_t a, uint32_t b) {
+    return sizeof(T) == 4 ? max(a, b) : __vmaxu2(a, b);
+}
+// A word's larger magnitude as fp32 bits.
+template <typename T>
+__device__ __forceinline__ uint32_t word_amax(uint32_t w) {
+    if (sizeof(T) == 4) return w;
+    const uint16_t m = (uint16_t)max(w & 0xFFFFu, w >> 16);
+    return __float_as_uint(to_f32(*reinterpret_cast<const T *>(&m)));
+}
+
 // BLOCK: one scale for the whole tile; otherwise one per row (ROWS) and one per column (COLS) of the tile.
 template <typename T, bool VEC, bool BLOCK, bool ROWS, bool COLS>
-__global__ void __launch_bounds__(kThreads) fp8_quantize_kernel(const QuantParams p) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2) fp8_quantize_kernel(const QuantParams p) {
     constexpr int V = Vec<T>::N;
-    constexpr int kLanes = kTile / V;             // threads along a row: 16 or 32
+    constexpr int kLanes = kTile / V;                // threads along a row: 16 or 32
     constexpr int kRun = kTile * kLanes / kThreads;  // neighbouring rows of a thread: 8 or 16
-    __shared__ uint32_t top[kTile];
+    constexpr int kRuns = kTile / kRun;
     __shared__ __align__(16) uint8_t tile[COLS ? kTile * kTile : 16];
+    __shared__ __align__(16) float factors[COLS && !BLOCK ? kTile : 4];
+    __shared__ uint32_t top;
     const int ch = threadIdx.x % kLanes, rg = threadIdx.x / kLanes;
     const int64_t row0 = (int64_t)blockIdx.x * kTile, col0 = (int64_t)blockIdx.y * kTile;
     const int64_t col = col0 + ch * V;
     const int valid = (int)(p.cols - col < V ? p.cols - col : V);
-    if (threadIdx.x < kTile) top[threadIdx.x] = 0;
-    __syncthreads();
     uint4 raw[kRun];
-    auto at = [&](int i, int e) { return to_f32(reinterpret_cast<const T *>(&raw[i])[e]); };
 #pragma unroll
     for (int i = 0; i < kRun; ++i) {
         const int64_t row = row0 + rg * kRun + i;
         raw[i] = make_uint4(0, 0, 0, 0);
         if (row < p.rows && valid > 0) raw[i] = load_raw<T, VEC>(static_cast<const T *>(p.x) + row * p.ldx + col, valid);
     }
+    auto at = [&raw](int i, int e) { return to_f32(reinterpret_cast<const T *>(&raw[i])[e]); };
+    if (BLOCK) {
+        if (threadIdx.x == 0) top = 0;
+        __syncthreads();
+    }
     if (p.column_sums != nullptr) {
-        constexpr int kRuns = kTile / kRun;
         __shared__ float red[kRuns][kTile];
 #pragma unroll
         for (int e = 0; e < V; ++e) {
@@ -65,65 +88,90 @@ __global__ void __launch_bounds__(kThreads) fp8_quantize_kernel(const QuantParam
             p.column_sums[blockIdx.x * p.cols + col0 + threadIdx.x] = s;
         }
     }
-    uint32_t whole = 0;
-    if (BLOCK) {
+    // maxima of the thread's rows (m) and columns (cm)
+    uint32_t m[kRun], cm[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < kRun; ++i)
+    for (int i = 0; i < kRun; ++i) {
+        const uint32_t w[4] = {word_abs<T>(raw[i].x), word_abs<T>(raw[i].y), word_abs<T>(raw[i].z), word_abs<T>(raw[i].w)};
+        m[i] = word_max<T>(word_max<T>(w[0], w[1]), word_max<T>(w[2], w[3]));
+        if (COLS && !BLOCK) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) whole = max(whole, abs_bits(at(i, e)));
-        whole = __reduce_max_sync(kFullMask, whole);
-        if ((threadIdx.x & 31) == 0) atomicMax(&top[0], whole);
-        __syncthreads();
-        whole = top[0];
-        if (threadIdx.x == 0) {
-            const float s = block_scale(block_amax(whole));
-            if (ROWS) p.scales[blockIdx.x + blockIdx.y * p.lds] = s;
-            if (COLS) p.scales_t[blockIdx.y + blockIdx.x * p.lds_t] = s;
+            for (int k = 0; k < 4; ++k) cm[k] = word_max<T>(cm[k], w[k]);
         }
     }
+    float whole = 0.0f;  // BLOCK: the tile's factor
+    if (BLOCK) {
+        uint32_t a = 0;
+#pragma unroll
+        for (int i = 0; i < kRun; ++i) a = word_max<T>(a, m[i]);
+        a = __reduce_max_sync(kFullMask, word_amax<T>(a));
+        if ((threadIdx.x & 31) == 0) atomicMax(&top, a);
+        __syncthreads();
+        const float amax = block_amax(top);
+        whole = block_factor(amax);
+        if (threadIdx.x == 0) {
+            if (ROWS) p.scales[blockIdx.x + blockIdx.y * p.lds] = block_scale(amax);
+            if (COLS) p.scales_t[blockIdx.y + blockIdx.x * p.lds_t] = block_scale(amax);
+        }
+    }
+    if (COLS && !BLOCK) {
+        // the runs' column maxima side by side (in the tile's memory), then one thread a column
+        uint32_t *table = reinterpret_cast<uint32_t *>(tile);  // [kRuns][kTile / elements per word]
+        *reinterpret_cast<uint4 *>(table + rg * kLanes * 4 + ch * 4) = make_uint4(cm[0], cm[1], cm[2], cm[3]);
+        __syncthreads();
+        if (threadIdx.x < kTile) {
+            const T *column = reinterpret_cast<const T *>(tile) + threadIdx.x;
+            uint32_t a = 0;
+#pragma unroll
+            for (int i = 0; i < kRuns; ++i) a = max(a, __float_as_uint(to_f32(column[i * kTile])));
+            const float amax = block_amax(a);
+            factors[threadIdx.x] = block_factor(amax);
+            if (col0 + threadIdx.x < p.cols) p.scales_t[col0 + threadIdx.x + blockIdx.x * p.lds_t] = block_scale(amax);
+        }
+        __syncthreads();
+    }
     if (ROWS) {
+        float f = whole;
+        if (!BLOCK) {
+            // halving exchange: after each step a thread holds half as many rows, with twice the columns in each
+#pragma unroll
+            for (int n = kRun / 2, off = kLanes / 2; n > 0; n /= 2, off /= 2) {
+                const bool upper = (ch & off) != 0;
+#pragma unroll
+                for (int k = 0; k < n; ++k) {
+                    const uint32_t other = __shfl_xor_sync(kFullMask, upper ? m[k] : m[k + n], off);
+                    m[k] = word_max<T>(upper ? m[k + n] : m[k], other);
+                }
+            }
+            const uint32_t a = word_max<T>(m[0], __shfl_xor_sync(kFullMask, m[0], 1));
+            const float amax = block_amax(word_amax<T>(a));  // of row ch / 2 of the run
+            f = block_factor(amax);
+            const int64_t row = row0 + rg * kRun + ch / 2;
+            if ((ch & 1) == 0 && row < p.rows) p.scales[row + blockIdx.y * p.lds] = block_scale(amax);
+        }
 #pragma unroll
         for (int i = 0; i < kRun; ++i) {
             const int64_t row = row0 + rg * kRun + i;
-            uint32_t m = whole;
-            if (!BLOCK) {
-#pragma unroll
-                for (int e = 0; e < V; ++e) m = max(m, abs_bits(at(i, e)));
-#pragma unroll
-                for (int off = kLanes / 2; off > 0; off >>= 1) m = max(m, __shfl_xor_sync(kFullMask, m, off));
-            }
-            const float a = block_amax(m), f = block_factor(a);
+            const float fi = BLOCK ? whole : __shfl_sync(kFullMask, f, 2 * i, kLanes);
             if (row < p.rows && valid > 0) {
                 uint32_t c[V / 4];
 #pragma unroll
                 for (int k = 0; k < V / 4; ++k)
-                    c[k] = e4m3x4(__fmul_rn(at(i, 4 * k), f), __fmul_rn(at(i, 4 * k + 1), f), __fmul_rn(at(i, 4 * k + 2), f),
-                                  __fmul_rn(at(i, 4 * k + 3), f));
+                    c[k] = e4m3x4(__fmul_rn(at(i, 4 * k), fi), __fmul_rn(at(i, 4 * k + 1), fi), __fmul_rn(at(i, 4 * k + 2), fi),
+                                  __fmul_rn(at(i, 4 * k + 3), fi));
                 // code rows are padded to 16 bytes, so a whole chunk always fits
                 uint32_t *dst = reinterpret_cast<uint32_t *>(p.codes + row * p.ldc + col);
                 if (V == 8)
                     *reinterpret_cast<uint2 *>(dst) = make_uint2(c[0], c[V / 4 - 1]);
                 else
                     *dst = c[0];
-                if (!BLOCK && ch == 0) p.scales[row + blockIdx.y * p.lds] = block_scale(a);
             }
         }
     }
     if (COLS) {
-        if (!BLOCK) {
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                uint32_t m = 0;
-#pragma unroll
-                for (int i = 0; i < kRun; ++i) m = max(m, abs_bits(at(i, e)));
-                if (V == 8) m = max(m, __shfl_xor_sync(kFullMask, m, 16));  // the warp's other run of rows
-                if (V == 4 || (threadIdx.x & 16) == 0) atomicMax(&top[ch * V + e], m);
-            }
-            __syncthreads();
-        }
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            const float f = block_factor(block_amax(BLOCK ? whole : top[ch * V + e]));
+            const float f = BLOCK ? whole : factors[ch * V + e];
 #pragma unroll
             for (int k = 0; k < kRun / 8; ++k) {
                 uint2 u;
@@ -145,8 +193,6 @@ __global__ void __launch_bounds__(kThreads) fp8_quantize_kernel(const QuantParam
                 *reinterpret_cast<uint4 *>(p.codes_t + out * p.ldt + r) = make_uint4(a.x, a.y, b.x, b.y);
             }
         }
-        if (!BLOCK && threadIdx.x < kTile && col0 + threadIdx.x < p.cols)
-            p.scales_t[col0 + threadIdx.x + blockIdx.x * p.lds_t] = block_scale(block_amax(top[threadIdx.x]));
     }
 }
 
