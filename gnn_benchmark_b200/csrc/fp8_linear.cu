@@ -86,8 +86,8 @@ int multiply(const Piece &a, bool a_block, const Piece &b, bool b_block, int64_t
 
 int check(const char *what, int64_t M, int64_t N, int64_t K, const void *kept, size_t kept_bytes, size_t kept_need,
           const void *scratch, size_t scratch_bytes, size_t scratch_need) {
-    if (M > 0x7FFFFFFF - 256 || N > 65535ll * 128 || K > 65535ll * 128)
-        return fail(GNNAGG_ERR_UNSUPPORTED, "%s: more than 2^31 rows or %d columns", what, 65535 * 128);
+    if (M > 0x7FFFFFFF - 256 || N > 0x7FFFFFFF - 256 || K > 0x7FFFFFFF - 256)
+        return fail(GNNAGG_ERR_UNSUPPORTED, "%s: a size exceeds 2^31", what);
     if (kept_need > 0 && (kept == nullptr || !aligned16(kept) || kept_bytes < kept_need))
         return fail(GNNAGG_ERR_SCRATCH, "%s: the buffer that is kept is too small or misaligned (need %zu bytes)", what, kept_need);
     if (scratch_need > 0 && (scratch == nullptr || !aligned16(scratch) || scratch_bytes < scratch_need))

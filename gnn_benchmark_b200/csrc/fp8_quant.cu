@@ -25,6 +25,7 @@ struct QuantParams {
     int64_t ldc, ldt;
     float *scales, *scales_t;      // scale of (row or row block i, column group j) at i + j * lds, likewise for the
     int64_t lds, lds_t;            // transpose
+    uint32_t col_tiles;
     float *column_sums;            // [row blocks][cols] sums of x over a tile's rows, or null
 };
 
@@ -56,7 +57,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2) fp8_quantize
     __shared__ __align__(16) float factors[COLS && !BLOCK ? kTile : 4];
     __shared__ uint32_t top;
     const int ch = threadIdx.x % kLanes, rg = threadIdx.x / kLanes;
-    const int64_t row0 = (int64_t)blockIdx.x * kTile, col0 = (int64_t)blockIdx.y * kTile;
+    // neighbouring blocks read neighbouring columns of the same rows
+    const int64_t rt = blockIdx.x / p.col_tiles, ct = blockIdx.x - rt * p.col_tiles;
+    const int64_t row0 = rt * kTile, col0 = ct * kTile;
     const int64_t col = col0 + ch * V;
     const int valid = (int)(p.cols - col < V ? p.cols - col : V);
     uint4 raw[kRun];
@@ -85,7 +88,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2) fp8_quantize
             float s = 0.0f;
 #pragma unroll
             for (int i = 0; i < kRuns; ++i) s += red[i][threadIdx.x];
-            p.column_sums[blockIdx.x * p.cols + col0 + threadIdx.x] = s;
+            p.column_sums[rt * p.cols + col0 + threadIdx.x] = s;
         }
     }
     // maxima of the thread's rows (m) and columns (cm)
@@ -110,8 +113,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2) fp8_quantize
         const float amax = block_amax(top);
         whole = block_factor(amax);
         if (threadIdx.x == 0) {
-            if (ROWS) p.scales[blockIdx.x + blockIdx.y * p.lds] = block_scale(amax);
-            if (COLS) p.scales_t[blockIdx.y + blockIdx.x * p.lds_t] = block_scale(amax);
+            if (ROWS) p.scales[rt + ct * p.lds] = block_scale(amax);
+            if (COLS) p.scales_t[ct + rt * p.lds_t] = block_scale(amax);
         }
     }
     if (COLS && !BLOCK) {
@@ -126,7 +129,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2) fp8_quantize
             for (int i = 0; i < kRuns; ++i) a = max(a, __float_as_uint(to_f32(column[i * kTile])));
             const float amax = block_amax(a);
             factors[threadIdx.x] = block_factor(amax);
-            if (col0 + threadIdx.x < p.cols) p.scales_t[col0 + threadIdx.x + blockIdx.x * p.lds_t] = block_scale(amax);
+            if (col0 + threadIdx.x < p.cols) p.scales_t[col0 + threadIdx.x + rt * p.lds_t] = block_scale(amax);
         }
         __syncthreads();
     }
@@ -147,7 +150,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2) fp8_quantize
             const float amax = block_amax(word_amax<T>(a));  // of row ch / 2 of the run
             f = block_factor(amax);
             const int64_t row = row0 + rg * kRun + ch / 2;
-            if ((ch & 1) == 0 && row < p.rows) p.scales[row + blockIdx.y * p.lds] = block_scale(amax);
+            if ((ch & 1) == 0 && row < p.rows) p.scales[row + ct * p.lds] = block_scale(amax);
         }
 #pragma unroll
         for (int i = 0; i < kRun; ++i) {
@@ -198,7 +201,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2) fp8_quantize
 
 template <typename T, bool VEC, bool BLOCK>
 int launch(const QuantParams &p, cudaStream_t st) {
-    const dim3 grid((unsigned)div_up(p.rows, kTile), (unsigned)div_up(p.cols, kTile));
+    const unsigned grid = (unsigned)(div_up(p.rows, kTile) * p.col_tiles);
     if (p.codes != nullptr && p.codes_t != nullptr)
         fp8_quantize_kernel<T, VEC, BLOCK, true, true><<<grid, kThreads, 0, st>>>(p);
     else if (p.codes != nullptr)
@@ -230,8 +233,8 @@ extern "C" int gnnagg_fp8_quantize(const void *x, int64_t ldx, int64_t rows, int
     if (codes == nullptr && codes_t == nullptr) return fail(GNNAGG_ERR_ARG, "fp8_quantize: no output");
     if (x == nullptr || (codes != nullptr && scales == nullptr) || (codes_t != nullptr && scales_t == nullptr))
         return fail(GNNAGG_ERR_ARG, "fp8_quantize: null pointer");
-    if (rows > 0x7FFFFFFF - 256 || cols > (int64_t)65535 * kTile)
-        return fail(GNNAGG_ERR_UNSUPPORTED, "fp8_quantize: more than 2^31 rows or %d columns", 65535 * kTile);
+    if (rows > 0x7FFFFFFF - 256 || cols > 0x7FFFFFFF - 256 || div_up(rows, kTile) * div_up(cols, kTile) > 0x7FFFFFFF)
+        return fail(GNNAGG_ERR_UNSUPPORTED, "fp8_quantize: more than 2^31 rows, columns or tiles");
     if (ldx < cols || (codes != nullptr && ldc < cols) || (codes_t != nullptr && ldt < rows))
         return fail(GNNAGG_ERR_ARG, "fp8_quantize: a stride is smaller than its rows");
     if ((codes != nullptr && (!aligned16(codes) || ldc % 16 != 0)) ||
@@ -240,7 +243,7 @@ extern "C" int gnnagg_fp8_quantize(const void *x, int64_t ldx, int64_t rows, int
     const int64_t r = block_rows == 1 ? rows : div_up(rows, kTile), c = block_rows == 1 ? cols : div_up(cols, kTile);
     if ((codes != nullptr && lds < r) || (codes_t != nullptr && lds_t < c))
         return fail(GNNAGG_ERR_ARG, "fp8_quantize: a stride of the scales is too small");
-    const QuantParams p{x, ldx, rows, cols, codes, codes_t, ldc, ldt, scales, scales_t, lds, lds_t, column_sums};
+    const QuantParams p{x, ldx, rows, cols, codes, codes_t, ldc, ldt, scales, scales_t, lds, lds_t, (uint32_t)div_up(cols, kTile), column_sums};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool block = block_rows == 128;
     return type == kTypeF32    ? launch_type<float>(p, block, st)
