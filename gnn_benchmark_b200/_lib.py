@@ -11,7 +11,10 @@ import torch
 _PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG_DIR, "libgnnagg.so")
 
+OPS_PATH = os.path.join(_PKG_DIR, "_torch_ops.so")
+
 _lib = None
+_ops = None
 
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -111,6 +114,23 @@ def lib():
     return _lib
 
 
+def ops():
+    """The torch front end of the low-precision operators (csrc/torch/ops.cpp): the same C ABI, with argument checks,
+    allocation and autograd nodes in C++.  Raises if _torch_ops.so has not been built."""
+    global _ops
+    if _ops is None:
+        import importlib.util
+
+        lib()
+        if not os.path.isfile(OPS_PATH):
+            raise RuntimeError(f"{OPS_PATH} is missing: build it with `python -m gnn_benchmark_b200.build`")
+        spec = importlib.util.spec_from_file_location("_torch_ops", OPS_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _ops = module
+    return _ops
+
+
 def check(rc: int, what: str) -> None:
     if rc != 0:
         msg = lib().gnnagg_error_string(rc).decode()
@@ -145,18 +165,6 @@ class device_of:
     def __exit__(self, *exc):
         if self.before != self.index:
             torch.cuda.set_device(self.before)
-
-
-def empty_codes(rows: int, cols: int, device):
-    """Uninitialised e4m3 codes (rows, cols) whose rows start on 16 bytes, and their scales (`empty_scales`)."""
-    ld = (cols + 15) // 16 * 16
-    codes = torch.empty_strided((rows, cols) if ld == cols else (rows, ld), (ld, 1), dtype=torch.float8_e4m3fn, device=device)
-    return codes if ld == cols else codes[:, :cols], empty_scales(rows, cols, device)
-
-
-def empty_scales(rows: int, cols: int, device):
-    """Uninitialised scales, one per row and 128 columns, lying column by column, each column on 16 bytes."""
-    return torch.empty_strided((rows, (cols + 127) // 128), (1, (rows + 3) // 4 * 4), dtype=torch.float32, device=device)
 
 
 def require_cuda(*tensors) -> None:

@@ -132,7 +132,7 @@ def wgrad(g: torch.Tensor, x: torch.Tensor, out: torch.Tensor = None) -> torch.T
 def _matmul_tn(g: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
     """g.T @ x, tensor-core kernel when it takes the shapes, cuBLAS otherwise."""
     if MODE == "fp8":
-        return matmul_fp8(*_quantize(g, 1, False, True)[2:], *_quantize(x, 1, False, True)[2:], out_dtype=torch.float32)
+        return matmul_fp8(*quantize_fp8(g, transpose=True), *quantize_fp8(x, transpose=True), out_dtype=torch.float32)
     if enabled() and wgrad_supported(g, x):
         return wgrad(g, x)
     _library_path("wgrad", (g.size(1), x.size(1)))
@@ -314,40 +314,6 @@ class SageDense(torch.autograd.Function):
 
 # ---------------------------------------------------------------------------------------------- 8-bit products
 
-FP8 = torch.float8_e4m3fn
-FP8_BLOCK = 128
-
-
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """`t` itself when its rows are contiguous and do not overlap, else a copy."""
-    return t if t.stride(1) == 1 and t.stride(0) >= t.size(1) else t.contiguous()
-
-
-def _quantize(x: torch.Tensor, block_rows: int, rows: bool, cols: bool):
-    """(codes, scales, codes_t, scales_t) of x from one read; the pair that is not asked for is None, None."""
-    if x.dim() != 2 or x.dtype not in _lib.TYPES:
-        raise RuntimeError(f"quantize_fp8: x must be a float32, bfloat16 or float16 matrix, not {tuple(x.shape)} {x.dtype}")
-    _lib.require_cuda(x)
-    m, k = x.shape
-    x = _rows(x)
-    codes = scales = codes_t = scales_t = None
-    args, args_t = (0, 0, 0, 0), (0, 0, 0, 0)
-    if rows:
-        codes, scales = _lib.empty_codes(m, k, x.device)
-        if block_rows == 128:
-            scales = _lib.empty_scales((m + 127) // 128, k, x.device)
-        args = (codes.data_ptr(), codes.stride(0), scales.data_ptr(), scales.stride(1))
-    if cols:
-        codes_t, scales_t = _lib.empty_codes(k, m, x.device)
-        if block_rows == 128:
-            scales_t = _lib.empty_scales((k + 127) // 128, m, x.device)
-        args_t = (codes_t.data_ptr(), codes_t.stride(0), scales_t.data_ptr(), scales_t.stride(1))
-    with _lib.device_of(x):
-        rc = _lib.lib().gnnagg_fp8_quantize(x.data_ptr(), max(x.stride(0), k), m, k, _lib.TYPES[x.dtype], block_rows, *args, *args_t,
-                                            0, _lib.stream_ptr(x.device))
-    _lib.check(rc, "fp8_quantize")
-    return codes, scales, codes_t, scales_t
-
 
 def quantize_fp8(x: torch.Tensor, block=(1, 128), transpose: bool = False):
     """(codes, scales) of x (rows, cols) float32, bfloat16 or float16.
@@ -359,26 +325,7 @@ def quantize_fp8(x: torch.Tensor, block=(1, 128), transpose: bool = False):
     that holds a NaN or an infinity reads back as NaN."""
     if tuple(block) not in ((1, 128), (128, 128)):
         raise RuntimeError(f"quantize_fp8: block must be (1, 128) or (128, 128), not {block}")
-    r = _quantize(x, block[0], not transpose, transpose)
-    return r[2:] if transpose else r[:2]
-
-
-def _operand(name: str, codes: torch.Tensor, scales: torch.Tensor, index: int):
-    """(rows that a scale covers, row stride) of a checked operand."""
-    if codes.dim() != 2 or codes.dtype != FP8 or codes.get_device() != index:
-        raise RuntimeError(f"matmul_fp8: {name} must be a float8_e4m3fn matrix on the operands' device")
-    rows, k = codes.shape
-    high, kb = (rows + 127) // 128, (k + 127) // 128
-    ld, step = codes.stride()
-    if rows <= 1 or k == 0:  # torch may keep any stride
-        ld = kb * 128
-    if rows > 0 and k > 0 and (step != 1 and k > 1 or ld < k or ld % 16 != 0 or codes.data_ptr() % 16 != 0):
-        raise RuntimeError(f"matmul_fp8: {name}'s rows must be contiguous and start on 16 bytes (as quantize_fp8 lays them)")
-    shape = scales.shape
-    if scales.dtype != torch.float32 or scales.get_device() != index or (shape != (rows, kb) and shape != (high, kb)):
-        raise RuntimeError(f"matmul_fp8: {name}'s scales must be float32 ({rows} or {high}, {kb}) on the operands' device, "
-                           f"not {tuple(shape)} {scales.dtype}")
-    return (1 if shape[0] == rows else 128), ld
+    return tuple(_lib.ops().quantize_fp8(x, block[0], not transpose, transpose))
 
 
 def matmul_fp8(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor,
@@ -386,111 +333,19 @@ def matmul_fp8(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scale
                accumulate: bool = False) -> torch.Tensor:
     """out (M, N) (+)= (a * a_scales) @ (b * b_scales).T (+ bias): a (M, K) and b (N, K) float8_e4m3fn with float32
     scales for each block of 128 along K, one per row, (rows, ceil(K / 128)), or per 128 rows.  out_dtype float32,
-    bfloat16 or float16 (out's type when out is given); bias (N,) of one of these; accumulate needs a float32 out."""
-    if not a.is_cuda:
-        _lib.require_cuda(a)
-    device, index = a.device, a.get_device()
-    a_block, lda = _operand("a", a, a_scales, index)
-    b_block, ldb = _operand("b", b, b_scales, index)
-    m, k = a.shape
-    n, kb = b.shape
-    if kb != k:
-        raise RuntimeError(f"matmul_fp8: shape mismatch a={tuple(a.shape)} b={tuple(b.shape)}")
-    bias_ptr = bias_type = 0
-    if bias is not None:
-        if bias.dtype not in _lib.TYPES or bias.shape != (n,) or not bias.is_contiguous() or bias.get_device() != index:
-            raise RuntimeError("matmul_fp8: bias must be a contiguous float32, bfloat16 or float16 vector of N elements on the "
-                               "operands' device")
-        bias_ptr, bias_type = bias.data_ptr(), _lib.TYPES[bias.dtype]
-    if out is None:
-        if accumulate:
-            raise RuntimeError("matmul_fp8: accumulate needs an output to accumulate into")
-        if out_dtype not in _lib.TYPES:
-            raise RuntimeError("matmul_fp8: out_dtype must be float32, bfloat16 or float16")
-        out = torch.empty((m, n), dtype=out_dtype, device=device)
-        ldc = n
-    else:
-        out_dtype, ldc = out.dtype, out.stride(0) if m > 1 else n
-        if out.shape != (m, n) or out_dtype not in _lib.TYPES or out.get_device() != index \
-                or (out.numel() > 0 and (out.stride(1) != 1 and n > 1 or ldc < n)):
-            raise RuntimeError("matmul_fp8: out must be (M, N) float32, bfloat16 or float16 with contiguous rows on the operands' "
-                               "device")
-        if accumulate and out_dtype != torch.float32:
-            raise RuntimeError("matmul_fp8: accumulate needs a float32 output")
-    lib = _lib.lib()
-    ws_ptr, ws_bytes = 0, lib.gnnagg_fp8_matmul_workspace_bytes(m, n, k)
-    if ws_bytes:
-        # from the caching allocator at every call: ordered with the stream, and a captured graph has its own
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
-        ws_ptr = ws.data_ptr()
-    _fp8_devices.add(index)
-    with _lib.device_of(a):
-        rc = lib.gnnagg_fp8_matmul(a.data_ptr(), lda, a_scales.data_ptr(), *a_scales.stride(), a_block, b.data_ptr(), ldb,
-                                   b_scales.data_ptr(), *b_scales.stride(), b_block, m, n, k, bias_ptr, bias_type,
-                                   1 if accumulate else 0, out.data_ptr(), ldc, _lib.TYPES[out_dtype], ws_ptr, ws_bytes,
-                                   _lib.stream_ptr(device))
-    if rc:
-        _lib.check(rc, "fp8_matmul")
+    bfloat16 or float16 (out's type when out is given); bias (N,) of one of these; accumulate needs a float32 out.
+    Not differentiable."""
+    out = _lib.ops().matmul_fp8(a, a_scales, b, b_scales, bias, out, out_dtype, accumulate)
+    _fp8_devices.add(out.get_device())
     return out
-
-
-class LinearFP8(torch.autograd.Function):
-    """y = x @ W^T (+ b) with e4m3 operands in all three products.  x and the output's gradient are rounded in blocks
-    of 1 x 128 along the sum they enter (columns for y and the input gradient, rows for the weight gradient), the
-    weight in blocks of 128 x 128.  What is kept for the backward is 8-bit: x's transposed codes and the weight's."""
-
-    @staticmethod
-    def forward(ctx, x, weight, bias):
-        lib, device = _lib.lib(), x.device
-        (m, k), n = x.shape, weight.size(0)
-        x, weight = _rows(x), _rows(weight)
-        need_x, need_w = (1 if need else 0 for need in ctx.needs_input_grad[:2])
-        types = [_lib.TYPES[t.dtype] if t is not None else 0 for t in (x, weight, bias)]
-        kept_bytes = lib.gnnagg_fp8_linear_kept_bytes(m, n, k, need_x, need_w)
-        scratch_bytes = lib.gnnagg_fp8_linear_scratch_bytes(m, n, k, 0)
-        kept = torch.empty(kept_bytes, dtype=torch.uint8, device=device)
-        scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device=device)
-        y = torch.empty((m, n), dtype=x.dtype, device=device)
-        _fp8_devices.add(device.index)
-        with _lib.device_of(x):
-            rc = lib.gnnagg_fp8_linear_fwd(x.data_ptr(), max(x.stride(0), k), types[0], weight.data_ptr(),
-                                           max(weight.stride(0), k), types[1], _lib.ptr(bias), types[2], m, n, k, y.data_ptr(),
-                                           types[0], need_x, need_w, kept.data_ptr(), kept_bytes, scratch.data_ptr(),
-                                           scratch_bytes, _lib.stream_ptr(device))
-        _lib.check(rc, "fp8_linear_fwd")
-        ctx.save_for_backward(kept)
-        ctx.sizes, ctx.needs, ctx.types = (m, n, k), (need_x, need_w), types
-        ctx.dtypes = x.dtype, weight.dtype, None if bias is None else bias.dtype
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g):
-        (kept,) = ctx.saved_tensors
-        (m, n, k), (need_x, need_w), types = ctx.sizes, ctx.needs, ctx.types
-        lib, device = _lib.lib(), g.device
-        g = _rows(g)
-        gx = torch.empty((m, k), dtype=ctx.dtypes[0], device=device) if need_x else None
-        gw = torch.empty((n, k), dtype=ctx.dtypes[1], device=device) if need_w else None
-        gb = torch.empty(n, dtype=ctx.dtypes[2], device=device) if ctx.needs_input_grad[2] else None
-        scratch_bytes = lib.gnnagg_fp8_linear_scratch_bytes(m, n, k, 1)
-        scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device=device)
-        with _lib.device_of(g):
-            rc = lib.gnnagg_fp8_linear_bwd(g.data_ptr(), max(g.stride(0), n), types[0], m, n, k, need_x, need_w,
-                                           kept.data_ptr(), kept.numel(), _lib.ptr(gx), types[0], _lib.ptr(gw), types[1],
-                                           _lib.ptr(gb), types[2], scratch.data_ptr(), scratch_bytes, _lib.stream_ptr(device))
-        _lib.check(rc, "fp8_linear_bwd")
-        return gx, gw, gb
 
 
 def linear_fp8(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor = None) -> torch.Tensor:
     """x (M, K) @ weight (N, K).T (+ bias (N,)) with operands rounded to e4m3 in blocks of 128, in the forward and in
-    both gradients; sums in float32, the output in x's type.  float32, bfloat16 or float16."""
-    _lib.require_cuda(x, weight, bias)
-    if x.dim() != 2 or weight.dim() != 2 or x.size(1) != weight.size(1):
-        raise RuntimeError(f"linear_fp8: shape mismatch x={tuple(x.shape)} weight={tuple(weight.shape)}")
-    if x.dtype not in _lib.TYPES or weight.dtype not in _lib.TYPES or weight.device != x.device:
-        raise RuntimeError("linear_fp8: x and weight must be float32, bfloat16 or float16 on one device")
-    if bias is not None and (bias.shape != (weight.size(0),) or bias.dtype not in _lib.TYPES or bias.device != x.device):
-        raise RuntimeError("linear_fp8: bias must be a float32, bfloat16 or float16 vector of N elements on x's device")
-    return LinearFP8.apply(x, weight, bias if bias is None or bias.is_contiguous() else bias.contiguous())
+    both gradients; sums in float32, the output in x's type.  float32, bfloat16 or float16.
+
+    x and the output's gradient are rounded in blocks of 1 x 128 along the sum they enter, the weight in blocks of
+    128 x 128.  What is kept for the backward is 8-bit.  Differentiable once."""
+    y = _lib.ops().linear_fp8(x, weight, bias)
+    _fp8_devices.add(y.get_device())
+    return y

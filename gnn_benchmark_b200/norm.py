@@ -139,102 +139,14 @@ def relu_dropout_(x: torch.Tensor, p: float, training: bool) -> torch.Tensor:
     return F.dropout(x, p=p, training=training) if p > 0 else x
 
 
-MAX_RMS_WIDTH = 16384
-
-
-def _check_rms(what: str, x: torch.Tensor, weight: torch.Tensor, residual) -> None:
-    if not x.is_cuda:
-        _lib.require_cuda(x)
-    index, dtype, shape = x.get_device(), x.dtype, x.shape
-    if len(shape) != 2 or dtype not in _lib.TYPES or not 0 < shape[1] <= MAX_RMS_WIDTH:
-        raise RuntimeError(f"{what}: x must be (rows, F) float32, bfloat16 or float16 with 1 <= F <= {MAX_RMS_WIDTH}, "
-                           f"not {tuple(shape)} {dtype}")
-    if weight.shape != shape[1:] or weight.dtype not in (dtype, torch.float32) or weight.get_device() != index:
-        raise RuntimeError(f"{what}: weight must be a vector of {shape[1]} elements of x's type or float32 on x's device")
-    if residual is not None and (residual.shape != shape or residual.dtype != dtype or residual.get_device() != index):
-        raise RuntimeError(f"{what}: residual must match x in shape, type and device")
-
-
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """`t` itself when its rows are contiguous and do not overlap, else a copy."""
-    return t if t.stride(1) == 1 and t.stride(0) >= t.size(1) else t.contiguous()
-
-
-def _ld(t: torch.Tensor) -> int:
-    """Row stride of `_rows(t)`; of a single row, or rows of one element, torch may keep any stride."""
-    return max(t.stride(0), t.size(1))
-
-
-def _vector(t: torch.Tensor) -> torch.Tensor:
-    return t if t.is_contiguous() else t.contiguous()
-
-
-def _rms_forward(x, weight, residual, eps, need_rstd):
-    rows, f = x.shape
-    x, weight = _rows(x), _vector(weight)
-    y = torch.empty_strided((rows, f), (f, 1), dtype=x.dtype, device=x.device)
-    rstd = torch.empty_strided((rows,), (1,), dtype=torch.float32, device=x.device) if need_rstd else None
-    h, res_ptr, res_ld, h_ptr = x, 0, 0, 0
-    if residual is not None:
-        residual = _rows(residual)
-        h = torch.empty_like(y)
-        res_ptr, res_ld, h_ptr = residual.data_ptr(), _ld(residual), h.data_ptr()
-    with _lib.device_of(x):
-        rc = _lib.lib().gnnagg_rms_norm_fwd(x.data_ptr(), _ld(x), res_ptr, res_ld, weight.data_ptr(),
-                                            _lib.TYPES[weight.dtype], rows, f, _lib.TYPES[x.dtype], eps, h_ptr, f,
-                                            y.data_ptr(), f, _lib.ptr(rstd), _lib.stream_ptr(x.device))
-    if rc:
-        _lib.check(rc, "rms_norm_fwd")
-    return y, h, rstd, weight
-
-
-class _RMSNorm(torch.autograd.Function):
-    """(y, h) = norm of h = x + residual; without a residual h is x itself and only y is an output."""
-
-    @staticmethod
-    def forward(ctx, x, weight, residual, eps):
-        y, h, rstd, w = _rms_forward(x, weight, residual, eps, True)
-        ctx.save_for_backward(h, w, rstd)
-        ctx.has_residual = residual is not None
-        ctx.set_materialize_grads(False)
-        return (y, h) if residual is not None else y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, gy, gh=None):
-        h, w, rstd = ctx.saved_tensors
-        if gy is None:  # only the sum was used
-            return gh, None, gh if ctx.has_residual else None, None
-        rows, f = h.shape
-        gy = _rows(gy)
-        gh = None if gh is None else _rows(gh)
-        gx = torch.empty_strided((rows, f), (f, 1), dtype=h.dtype, device=h.device)
-        dw = torch.empty_like(w)
-        lib, kind = _lib.lib(), _lib.TYPES[h.dtype]
-        partial_bytes = lib.gnnagg_rms_norm_partial_bytes(rows, f, kind)
-        partial = torch.empty_strided((partial_bytes,), (1,), dtype=torch.uint8, device=h.device)
-        with _lib.device_of(h):
-            rc = lib.gnnagg_rms_norm_bwd(gy.data_ptr(), _ld(gy), _lib.ptr(gh), 0 if gh is None else _ld(gh),
-                                         h.data_ptr(), _ld(h), rstd.data_ptr(), w.data_ptr(), _lib.TYPES[w.dtype],
-                                         rows, f, kind, gx.data_ptr(), f, dw.data_ptr(), partial.data_ptr(),
-                                         partial_bytes, _lib.stream_ptr(h.device))
-        if rc:
-            _lib.check(rc, "rms_norm_bwd")
-        return gx, dw, gx if ctx.has_residual else None, None
-
-
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor = None, eps: float = 1e-6):
     """y = h * rsqrt(mean(h^2) + eps) * weight over the last dimension, with h = x + residual.
 
-    x and residual (rows, F) float32, bfloat16 or float16; weight (F,) of the same type or float32.  With a
-    residual the result is (y, h): h, rounded to x's type, is the stream that the next layer adds to, and the
-    norm is of that rounded h.  Without one it is y alone.  Differentiable in x, weight and residual."""
-    _check_rms("rms_norm", x, weight, residual)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
-                                    or (residual is not None and residual.requires_grad)):
-        return _RMSNorm.apply(x, weight, residual, float(eps))
-    y, h, _, _ = _rms_forward(x, weight, residual, eps, False)
-    return y if residual is None else (y, h)
+    x and residual (rows, F) float32, bfloat16 or float16, F at most 16384; weight (F,) of the same type or float32.
+    With a residual the result is (y, h): h, rounded to x's type, is the stream that the next layer adds to, and the
+    norm is of that rounded h.  Without one it is y alone.  Differentiable (once) in x, weight and residual."""
+    r = _lib.ops().rms_norm(x, weight, residual, eps)
+    return r[0] if residual is None else tuple(r)
 
 
 def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor = None, eps: float = 1e-6):
@@ -242,22 +154,4 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor =
     (rows, ceil(F / 128)) float32, the value of an element being codes * scales[row, column // 128].  They are
     laid out as `dense.matmul_fp8` takes them.  With a residual the result is (codes, scales, h).  Inference
     only: there is no gradient through the rounding."""
-    _check_rms("rms_norm_fp8", x, weight, residual)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
-                                    or (residual is not None and residual.requires_grad)):
-        raise RuntimeError("rms_norm_fp8 has no gradient: call it under torch.no_grad(), or use rms_norm")
-    rows, f = x.shape
-    x, weight = _rows(x), _vector(weight)
-    codes, scales = _lib.empty_codes(rows, f, x.device)
-    h, res_ptr, res_ld, h_ptr = None, 0, 0, 0
-    if residual is not None:
-        residual = _rows(residual)
-        h = torch.empty_strided((rows, f), (f, 1), dtype=x.dtype, device=x.device)
-        res_ptr, res_ld, h_ptr = residual.data_ptr(), _ld(residual), h.data_ptr()
-    with _lib.device_of(x):
-        rc = _lib.lib().gnnagg_rms_norm_fp8(x.data_ptr(), _ld(x), res_ptr, res_ld, weight.data_ptr(),
-                                            _lib.TYPES[weight.dtype], rows, f, _lib.TYPES[x.dtype], eps, h_ptr, f,
-                                            codes.data_ptr(), codes.stride(0), scales.data_ptr(), scales.stride(1),
-                                            _lib.stream_ptr(x.device))
-    _lib.check(rc, "rms_norm_fp8")
-    return (codes, scales) if residual is None else (codes, scales, h)
+    return tuple(_lib.ops().rms_norm_fp8(x, weight, residual, eps))

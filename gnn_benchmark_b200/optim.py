@@ -7,26 +7,12 @@ tensors, `AdamW` the torch.optim.Optimizer around it.
 8-bit moments (`state_bits=8`) take 2.03 bytes a parameter instead of 8: e4m3 codes of the first moment and of the
 second moment's square root, in blocks of 256 elements with an fp32 scale each.
 """
-from array import array
-from itertools import chain
-
 import torch
 
 from . import _lib
 
 STATE_BLOCK = 256
 FP8 = torch.float8_e4m3fn
-
-
-def _check(what, ts, sizes, dtype, index) -> None:
-    """The tensors of one list: their type, device, layout and number of elements."""
-    if {t.dtype for t in ts} == {dtype} and set(map(torch.Tensor.get_device, ts)) == {index} \
-            and all(map(torch.Tensor.is_contiguous, ts)) and list(map(torch.Tensor.numel, ts)) == sizes:
-        return
-    for i, (t, n) in enumerate(zip(ts, sizes)):
-        if t.dtype != dtype or t.get_device() != index or not t.is_contiguous() or t.numel() != n:
-            raise RuntimeError(f"adamw_step: {what} {i} must be a contiguous {dtype} tensor of {n} elements on the parameters' "
-                               f"device, not {tuple(t.shape)} {t.dtype} on {t.device}")
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr: float, betas=(0.9, 0.999), eps: float = 1e-8,
@@ -41,45 +27,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr: float, be
     masters: for 16-bit parameters, float32 copies (None where there is none) that are updated and that the
     parameters are rounded from.  step: t, from 1.  device_scalars: what `AdamW(capturable=True)` keeps on the device
     instead of step and lr.  No two tensors may overlap."""
-    count = len(params)
-    if not (len(grads) == len(exp_avgs) == len(exp_avg_sqs) == count) or (scales is not None and len(scales) != count) \
-            or (masters is not None and len(masters) != count):
-        raise RuntimeError("adamw_step: the lists must have one entry per parameter")
-    b1, b2 = betas
-    if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
-        raise RuntimeError(f"adamw_step: betas must be in [0, 1), not {betas}")
-    if device_scalars is None and step < 1:
-        raise RuntimeError("adamw_step: the first step is 1")
-    if count == 0:
-        return
-    device, dtype, index = params[0].device, params[0].dtype, params[0].get_device()
-    _lib.require_cuda(params[0])
-    if dtype not in _lib.TYPES:
-        raise RuntimeError(f"adamw_step: parameters must be float32, bfloat16 or float16, not {dtype}")
-    state = torch.float32 if scales is None else FP8
-    sizes = list(map(torch.Tensor.numel, params))
-    _check("parameter", params, sizes, dtype, index)
-    _check("gradient", grads, sizes, dtype, index)
-    _check("exp_avg", exp_avgs, sizes, state, index)
-    _check("exp_avg_sq", exp_avg_sqs, sizes, state, index)
-    pointers = torch.Tensor.data_ptr
-    scale_ptrs = master_ptrs = (0,) * count
-    if scales is not None:
-        _check("scales", scales, [-(-n // STATE_BLOCK) * 2 for n in sizes], torch.float32, index)
-        scale_ptrs = map(pointers, scales)
-    if masters is not None:
-        held = [(t, n) for t, n in zip(masters, sizes) if t is not None]
-        if held:
-            _check("master", [t for t, _ in held], [n for _, n in held], torch.float32, index)
-        master_ptrs = map(_lib.ptr, masters)
-    rows = zip(map(pointers, params), map(pointers, grads), map(pointers, exp_avgs), map(pointers, exp_avg_sqs), scale_ptrs,
-               master_ptrs, sizes)
-    table = array("q", chain.from_iterable(rows))  # entries of gnnagg_adamw_tensor: six pointers and a size
-    with _lib.device_of(params[0]):
-        rc = _lib.lib().gnnagg_adamw_step(table.buffer_info()[0], count, _lib.TYPES[dtype], 32 if scales is None else 8, lr, b1,
-                                          b2, eps, weight_decay, step, _lib.ptr(device_scalars), _lib.stream_ptr(device))
-    if rc:
-        _lib.check(rc, "adamw_step")
+    _lib.ops().adamw_step(params, grads, exp_avgs, exp_avg_sqs, scales, masters, device_scalars, step, lr, *betas, eps,
+                          weight_decay)
 
 
 def _zero_moment(bits: int, like: torch.Tensor) -> torch.Tensor:
