@@ -21,6 +21,8 @@
 //               lane quarter w % 4 and one half of the columns.
 // What bounds a block is the hand-over and scaling: per scheduler 256 FMAs, 180 cycles of tensor-memory reads and a
 // round trip between the warps, against 512 cycles of MMA.  So the scaling loop holds nothing that another warp can do.
+// Where one column of tiles and few k-blocks make up the product (tall activations, a small weight), Q stays in shared
+// memory and only P's blocks go round: a third of the loads, and twice the blocks on their way.
 // Output tiles leave through shared memory by TMA stores, which run under the next tile's MMAs; rows that TMA cannot
 // address, and outputs that are added to, by plain stores.
 // A tile's sum may be split along k over several CTAs (few tiles, long sums): each writes an fp32 partial product
@@ -40,6 +42,7 @@ constexpr int kTmemCols = 512;
 constexpr int P_BYTES = BP * BK;
 constexpr int kPanel = 32 * 128;               // 32 rows of 128 bytes of the output, as a warp stages them
 constexpr int kRing = 3;                       // a scale warp's blocks: in use and on their way
+constexpr int kMaxStages = 10;
 constexpr int kBarBytes = 256;
 constexpr int kSmemLimit = 227 * 1024;
 // Registers per thread of the widest tiles after the launch: the control warpgroup gives up what the scaling ones
@@ -62,9 +65,9 @@ struct Tile {
     static constexpr int kWarpBytes = kPanels * kPanel + kCols * 4;
     static constexpr int kFixed = 1024 + kBarBytes + kWarps * kWarpBytes + (2 * kRing * kRaw + kBufs * kSlot) * 4;
     static constexpr int kFit = (kSmemLimit - kFixed) / kStageBytes;
-    static constexpr int kStages = kFit > 10 ? 10 : kFit;
+    static constexpr int kStages = kFit > kMaxStages ? kMaxStages : kFit;
     static constexpr int kSmem = kFixed + kStages * kStageBytes;
-    static constexpr int kBarriers = 2 * kStages + 2 * kBufs + 1;
+    static constexpr int kBarriers = 2 * kMaxStages + 2 * kBufs + 2;
     static_assert(kSmem <= kSmemLimit && kStages >= 3 && kBarriers * 8 + 8 <= kBarBytes, "shared memory budget");
     static constexpr bool kSplitRegs = BN == 256;
     static constexpr int kRegsNeeded = 128 * kRegsControl + 32 * kWarps * kRegsScaling;
@@ -96,6 +99,8 @@ struct Params {
     int p_block;         // P's scales are per 128 rows
     int kblocks, splits, kb_per_split;
     int tiles_p, tiles_q, items;
+    int stages;          // of the ring; with keep_q they hold P alone, behind Q's k-blocks
+    int keep_q;
     int accumulate;
     int vec_out;         // 16-byte stores of the output's rows
     int tma_out;         // the output leaves by TMA
@@ -177,13 +182,14 @@ __device__ __forceinline__ Item item_of(const Params &p, int i) {
     return w;
 }
 
-// Place and phase parity in a ring of N barriers.
-template <int N>
+// Place and phase parity in a ring of n barriers.
 struct Ring {
+    int n;
     int i = 0;
     uint32_t phase = 0;
+    __device__ __forceinline__ explicit Ring(int size) : n(size) {}
     __device__ __forceinline__ void next() {
-        if (++i == N) i = 0, phase ^= 1u;
+        if (++i == n) i = 0, phase ^= 1u;
     }
 };
 
@@ -193,11 +199,11 @@ __global__ void __launch_bounds__((Tile<BN, QROW>::kThreads), 1)
 fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
                   const __grid_constant__ CUtensorMap map_c, const Params p) {
     using S = Tile<BN, QROW>;
-    constexpr int kStages = S::kStages, kBufs = S::kBufs, kCols = S::kCols, kWarps = S::kWarps;
+    constexpr int kBufs = S::kBufs, kCols = S::kCols, kWarps = S::kWarps;
     extern __shared__ uint8_t smem_raw[];
     // 1024-byte alignment: the swizzle pattern and the descriptors assume it
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    uint8_t *staging = smem + kStages * S::kStageBytes;
+    uint8_t *staging = smem + S::kStages * S::kStageBytes;
     float *bias_s = reinterpret_cast<float *>(staging + kWarps * S::kPanels * kPanel);  // kCols per warp
     float *raw = bias_s + kWarps * kCols;                                                // kRing * kRaw per scale warp
     float *slots = raw + 2 * kRing * S::kRaw;                                                // one per partial product
@@ -206,14 +212,18 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_consta
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const uint32_t bar0 = smem_u32(bars);
     auto bar_full = [&](int s) { return bar0 + 8u * (uint32_t)s; };
-    auto bar_empty = [&](int s) { return bar0 + 8u * (uint32_t)(kStages + s); };
-    auto bar_acc_full = [&](int b) { return bar0 + 8u * (uint32_t)(2 * kStages + b); };
-    auto bar_acc_empty = [&](int b) { return bar0 + 8u * (uint32_t)(2 * kStages + kBufs + b); };
-    const uint32_t bar_drain = bar0 + 8u * (uint32_t)(2 * kStages + 2 * kBufs);
+    auto bar_empty = [&](int s) { return bar0 + 8u * (uint32_t)(kMaxStages + s); };
+    auto bar_acc_full = [&](int b) { return bar0 + 8u * (uint32_t)(2 * kMaxStages + b); };
+    auto bar_acc_empty = [&](int b) { return bar0 + 8u * (uint32_t)(2 * kMaxStages + kBufs + b); };
+    const uint32_t bar_drain = bar0 + 8u * (uint32_t)(2 * kMaxStages + 2 * kBufs);
+    const uint32_t bar_q = bar_drain + 8u;  // Q has landed, where it stays
+    // where a stage's P and Q begin
+    const uint32_t stage0 = smem_u32(smem) + (p.keep_q ? (uint32_t)(p.kblocks * BN * BK) : 0u);
+    const uint32_t stage_step = p.keep_q ? P_BYTES : S::kStageBytes;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kStages; ++s) {
+        for (int s = 0; s < p.stages; ++s) {
             mbar_init(bar_full(s), 1);
             mbar_init(bar_empty(s), 1);
         }
@@ -222,6 +232,7 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_consta
             mbar_init(bar_acc_empty(b), kWarps);
         }
         mbar_init(bar_drain, 1);
+        mbar_init(bar_q, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -240,9 +251,15 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_consta
         if (S::kSplitRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
         if (warp == 0) {
             // ---------------- TMA issuer ----------------
-            Ring<kStages> st;
+            Ring st(p.stages);
             uint32_t it = 0;
             bool ok = true;
+            if (p.keep_q && elect_one()) {
+                mbar_arrive_expect_tx(bar_q, (uint32_t)(p.kblocks * BN * BK));
+                for (int kb = 0; kb < p.kblocks; ++kb)
+                    tma_load_2d(smem_u32(smem) + (uint32_t)(kb * BN * BK), &map_q, bar_q, kb * BK, 0);
+            }
+            __syncwarp();
             for (int i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
                 const Item w = item_of(p, i);
                 for (int kb = w.kb0; kb < w.kb1; ++kb, ++it, st.next()) {
@@ -251,20 +268,22 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_consta
                         break;
                     }
                     if (elect_one()) {
-                        const uint32_t sp = smem_u32(smem) + (uint32_t)(st.i * S::kStageBytes);
-                        mbar_arrive_expect_tx(bar_full(st.i), (uint32_t)S::kStageBytes + p.tx_excess);
+                        const uint32_t sp = stage0 + (uint32_t)st.i * stage_step;
+                        mbar_arrive_expect_tx(bar_full(st.i), stage_step + p.tx_excess);
                         tma_load_2d(sp, &map_p, bar_full(st.i), kb * BK, w.tp * BP);
-                        tma_load_2d(sp + P_BYTES, &map_q, bar_full(st.i), kb * BK, w.tq * BN);
+                        if (!p.keep_q) tma_load_2d(sp + P_BYTES, &map_q, bar_full(st.i), kb * BK, w.tq * BN);
                     }
                     __syncwarp();
                 }
             }
             if (!ok) {
                 // copies of the last k-blocks issued may still be landing: wait for them, bounded
-                for (uint32_t back = 1; back <= (uint32_t)kStages && back <= it; ++back) {
-                    const uint32_t j = it - back;
+                const uint32_t n = (uint32_t)p.stages;
+                for (uint32_t back = 0; back <= n && back <= it; ++back) {
+                    if (back == 0 && !p.keep_q) continue;
+                    const uint32_t j = it - back, bar = back == 0 ? bar_q : bar_full((int)(j % n));
                     const unsigned long long t0 = globaltimer_ns();
-                    while (!mbar_try_wait(bar_full(j % kStages), (j / kStages) & 1u)) {
+                    while (!mbar_try_wait(bar, back == 0 ? 0u : (j / n) & 1u)) {
                         if (globaltimer_ns() - t0 > p.wait_ns) {
                             atomicCAS(&g_status, 0, (int)kErrDrain);
                             break;
@@ -274,9 +293,9 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_consta
             }
         } else if (warp == 1) {
             // ---------------- MMA issuer ----------------
-            Ring<kStages> st;
-            Ring<kBufs> ac;
-            bool ok = true;
+            Ring st(p.stages);
+            Ring ac(kBufs);
+            bool ok = !p.keep_q || mbar_wait(bar_q, 0, abort_flag, &g_status, kErrWaitFull, p.wait_ns);
             for (int i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
                 const Item w = item_of(p, i);
                 for (int kb = w.kb0; kb < w.kb1; ++kb, st.next(), ac.next()) {
@@ -287,8 +306,9 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_consta
                     }
                     tc_fence_after();
                     if (elect_one()) {
-                        const uint32_t sp = smem_u32(smem) + (uint32_t)(st.i * S::kStageBytes);
-                        const uint64_t dp = make_smem_desc(sp), dq = make_smem_desc(sp + P_BYTES);
+                        const uint32_t sp = stage0 + (uint32_t)st.i * stage_step;
+                        const uint32_t sq = p.keep_q ? smem_u32(smem) + (uint32_t)(kb * BN * BK) : sp + P_BYTES;
+                        const uint64_t dp = make_smem_desc(sp), dq = make_smem_desc(sq);
                         const uint32_t d = tmem_base + (uint32_t)(ac.i * BN);
 #pragma unroll
                         for (int k = 0; k < BK / UMMA_K; ++k)  // 32 bytes further inside the swizzled row
@@ -315,7 +335,7 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_consta
         } else {
             // ---------------- scales ----------------
             float *mine = raw + (warp - 2) * kRing * S::kRaw;
-            Ring<kBufs> ac;
+            Ring ac(kBufs);
             uint32_t it = 0;  // of all blocks; this warp has every second
             bool ok = true;
             for (int i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
@@ -382,7 +402,7 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_consta
             if (lane == 0) mbar_arrive(bar);
         };
         constexpr int kChunk = kCols > 32 ? (QROW ? 8 : 16) : kCols;
-        Ring<kBufs> ac;
+        Ring ac(kBufs);
         float *bias = bias_s + (warp - 4) * kCols;
         int64_t bias_at = -1;  // first column of the bias that is there
         uint32_t limit = 1u << 22;
@@ -632,7 +652,7 @@ int make_map_out(CUtensorMap *map, void *base, int type, int splits, int64_t M, 
 }
 
 template <int BN, bool QROW, bool SWAP, typename TOut>
-int launch(const CUtensorMap &mp, const CUtensorMap &mq, const CUtensorMap &mc, const Params &p, cudaStream_t st) {
+int launch(const CUtensorMap &mp, const CUtensorMap &mq, const CUtensorMap &mc, Params p, cudaStream_t st) {
     using S = Tile<BN, QROW>;
     static PerDeviceOnce attr_done;
     const cudaError_t e = attr_done.run([] {
@@ -649,6 +669,10 @@ int launch(const CUtensorMap &mp, const CUtensorMap &mq, const CUtensorMap &mc, 
         return fail(GNNAGG_ERR_CUDA, "fp8_matmul: cannot reserve %d bytes of shared memory and the registers: %s", S::kSmem,
                     cudaGetErrorString(e));
     const int grid = p.items < kNumSMs ? p.items : kNumSMs;
+    // Q stays where every CTA has several tiles of one column, and all of its k-blocks and three of P's fit
+    const int left = S::kStages * S::kStageBytes - p.kblocks * BN * BK;
+    p.keep_q = p.tiles_q == 1 && p.splits == 1 && p.items > grid && left >= 3 * P_BYTES;
+    p.stages = p.keep_q ? (left / P_BYTES < kMaxStages ? left / P_BYTES : kMaxStages) : S::kStages;
     fp8_matmul_kernel<BN, QROW, SWAP, TOut><<<grid, S::kThreads, S::kSmem, st>>>(mp, mq, mc, p);
     return check_launch("fp8_matmul_kernel");
 }
