@@ -26,7 +26,8 @@
 // Output tiles leave through shared memory by TMA stores, which run under the next tile's MMAs; rows that TMA cannot
 // address, and outputs that are added to, by plain stores.
 // A tile's sum may be split along k over several CTAs (few tiles, long sums): each writes an fp32 partial product
-// to the workspace and a second kernel adds them in a fixed order.
+// to the workspace and a second kernel adds them in a fixed order; up to eight small ones (few rows) are CTAs of a
+// cluster, and the first adds the others' from its own shared memory, which saves the second launch.
 // Every wait is bounded (about a second); on a time-out the kernel records a code in the library's status word,
 // drains its own copies and MMAs, frees tensor memory and returns.
 #include "lowp.cuh"
@@ -120,6 +121,22 @@ __device__ __forceinline__ void tc_mma_f8(uint32_t tmem_d, uint64_t adesc, uint6
         : "memory");
 }
 
+__device__ __forceinline__ void cluster_sync() {
+    __syncwarp();  // the barrier's aligned form wants whole warps
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Stores to the shared memory of the cluster's first CTA, at the place of this CTA's address `addr`.
+__device__ __forceinline__ void st_first(uint32_t addr, float v) {
+    asm volatile(
+        "{\n"
+        ".reg .b32 r;\n"
+        "mapa.shared::cluster.u32 r, %0, 0;\n"
+        "st.shared::cluster.f32 [r], %1;\n"
+        "}\n" ::"r"(addr), "f"(v)
+        : "memory");
+}
+
 // 4 bytes global -> shared, or zero when !ok.
 __device__ __forceinline__ void cp_async_4_or_zero(uint32_t dst, const float *src, bool ok) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(ok ? 4 : 0) : "memory");
@@ -193,8 +210,8 @@ struct Ring {
     }
 };
 
-// SWAP: the output is stored transposed, C[column][lane].
-template <int BN, bool QROW, bool SWAP, typename TOut>
+// SWAP: the output is stored transposed, C[column][lane].  JOIN (with SWAP): the splits of a tile are a cluster.
+template <int BN, bool QROW, bool SWAP, bool JOIN, typename TOut>
 __global__ void __launch_bounds__((Tile<BN, QROW>::kThreads), 1)
 fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
                   const __grid_constant__ CUtensorMap map_c, const Params p) {
@@ -391,6 +408,10 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_consta
                 __syncwarp();
             }
         }
+        if (JOIN) {  // the two barriers of the scaling warps
+            cluster_sync();
+            cluster_sync();
+        }
     } else {
         // ---------------- scaling warps ----------------
         if (S::kSplitRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsScaling));
@@ -459,13 +480,33 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_consta
             if (__any_sync(kFullMask, limit == 0)) {
                 *abort_flag = 1;
                 atomicCAS(&g_status, 0, (int)kErrWaitAccFull);
+                if (JOIN) {
+                    cluster_sync();
+                    cluster_sync();
+                }
                 break;
+            }
+            if (JOIN) {
+                // one tile per cluster: its CTAs' sums go to the first one, into stages that its MMAs have left, and
+                // are added there in rank order
+                cluster_sync();
+                float *sums = reinterpret_cast<float *>(smem) + (warp - 4) * kCols * 32 + lane;
+                if (w.split > 0) {
+#pragma unroll
+                    for (int j = 0; j < kCols; ++j)
+                        st_first(smem_u32(sums + ((w.split - 1) * kWarps * kCols + j) * 32), acc[j]);
+                }
+                cluster_sync();
+                if (w.split > 0) break;
+                for (int r = 1; r < p.splits; ++r)
+#pragma unroll
+                    for (int j = 0; j < kCols; ++j) acc[j] += sums[((r - 1) * kWarps * kCols + j) * 32];
             }
             if (SWAP) {
                 // lane = column of the output: 32 neighbouring columns of one output row per store
                 const int64_t row = row0 + lane;
                 const float bias = p.bias != nullptr && row < p.rows_p ? load_as_f32(p.bias, p.bias_type, row) : 0.0f;
-                TOut *dst = static_cast<TOut *>(p.C) + w.split * p.split_stride + col0 * p.ldc + row;
+                TOut *dst = static_cast<TOut *>(p.C) + (JOIN ? 0 : w.split * p.split_stride) + col0 * p.ldc + row;
 #pragma unroll
                 for (int j = 0; j < kCols; ++j, dst += p.ldc) {
                     if (row < p.rows_p && col0 + j < p.rows_q) {
@@ -594,9 +635,17 @@ struct Plan {
     bool swap;
     int bn, tiles_p, tiles_q, splits, kb_per_split, kblocks;
     int64_t ldp;  // row stride of a partial product
-    size_t bytes() const { return splits > 1 ? (size_t)splits * rows * ldp * sizeof(float) : 0; }
+    size_t bytes() const { return splits > 1 && !join ? (size_t)splits * rows * ldp * sizeof(float) : 0; }
     int64_t rows;
+    bool join;    // the splits of a tile are a cluster
 };
+
+// Shared memory of the stages of a tile of few rows.
+int stage_bytes(int bn) {
+    return bn == 16   ? Tile<16, true>::kStages * Tile<16, true>::kStageBytes
+           : bn == 32 ? Tile<32, true>::kStages * Tile<32, true>::kStageBytes
+                      : Tile<64, true>::kStages * Tile<64, true>::kStageBytes;
+}
 
 Plan plan_of(int64_t M, int64_t N, int64_t K) {
     Plan p;
@@ -614,6 +663,8 @@ Plan plan_of(int64_t M, int64_t N, int64_t K) {
     if (splits < 1) splits = 1;
     p.kb_per_split = (int)div_up(p.kblocks, splits);
     p.splits = p.kb_per_split > 0 ? (int)div_up(p.kblocks, p.kb_per_split) : 1;
+    // a cluster has at most eight CTAs; their tiles' sums have to fit behind one another in the first one's stages
+    p.join = p.swap && p.splits > 1 && p.splits <= 8 && (p.splits - 1) * BP * p.bn * 4 <= stage_bytes(p.bn);
     p.rows = M;
     p.ldp = div_up(N, 4) * 4;
     return p;
@@ -651,18 +702,18 @@ int make_map_out(CUtensorMap *map, void *base, int type, int splits, int64_t M, 
     return GNNAGG_OK;
 }
 
-template <int BN, bool QROW, bool SWAP, typename TOut>
+template <int BN, bool QROW, bool SWAP, bool JOIN, typename TOut>
 int launch(const CUtensorMap &mp, const CUtensorMap &mq, const CUtensorMap &mc, Params p, cudaStream_t st) {
     using S = Tile<BN, QROW>;
     static PerDeviceOnce attr_done;
     const cudaError_t e = attr_done.run([] {
         cudaFuncAttributes a;
-        const cudaError_t r = cudaFuncGetAttributes(&a, fp8_matmul_kernel<BN, QROW, SWAP, TOut>);
+        const cudaError_t r = cudaFuncGetAttributes(&a, fp8_matmul_kernel<BN, QROW, SWAP, JOIN, TOut>);
         if (r != cudaSuccess) return r;
         // a register split above what the launch allocates would wait forever
         if (S::kSplitRegs && (a.numRegs > kRegsScaling || a.numRegs * S::kThreads < S::kRegsNeeded))
             return cudaErrorInvalidConfiguration;
-        return cudaFuncSetAttribute(fp8_matmul_kernel<BN, QROW, SWAP, TOut>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        return cudaFuncSetAttribute(fp8_matmul_kernel<BN, QROW, SWAP, JOIN, TOut>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     S::kSmem);
     });
     if (e != cudaSuccess)
@@ -673,22 +724,43 @@ int launch(const CUtensorMap &mp, const CUtensorMap &mq, const CUtensorMap &mc, 
     const int left = S::kStages * S::kStageBytes - p.kblocks * BN * BK;
     p.keep_q = p.tiles_q == 1 && p.splits == 1 && p.items > grid && left >= 3 * P_BYTES;
     p.stages = p.keep_q ? (left / P_BYTES < kMaxStages ? left / P_BYTES : kMaxStages) : S::kStages;
-    fp8_matmul_kernel<BN, QROW, SWAP, TOut><<<grid, S::kThreads, S::kSmem, st>>>(mp, mq, mc, p);
+    if (JOIN) {  // one item per CTA: all of them are resident
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)p.items);
+        cfg.blockDim = dim3(S::kThreads);
+        cfg.dynamicSmemBytes = S::kSmem;
+        cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = (unsigned)p.splits;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        const cudaError_t le = cudaLaunchKernelEx(&cfg, fp8_matmul_kernel<BN, QROW, SWAP, JOIN, TOut>, mp, mq, mc, p);
+        if (le != cudaSuccess) return fail(GNNAGG_ERR_CUDA, "fp8_matmul_kernel: %s", cudaGetErrorString(le));
+    } else {
+        fp8_matmul_kernel<BN, QROW, SWAP, JOIN, TOut><<<grid, S::kThreads, S::kSmem, st>>>(mp, mq, mc, p);
+    }
     return check_launch("fp8_matmul_kernel");
 }
 
 template <bool QROW, typename TOut>
 int launch_tile(const Plan &plan, const CUtensorMap &mp, const CUtensorMap &mq, const CUtensorMap &mc, const Params &p,
                 cudaStream_t st) {
+    if (plan.join)
+        return plan.bn == 16   ? launch<16, QROW, true, true, TOut>(mp, mq, mc, p, st)
+               : plan.bn == 32 ? launch<32, QROW, true, true, TOut>(mp, mq, mc, p, st)
+                               : launch<64, QROW, true, true, TOut>(mp, mq, mc, p, st);
     if (plan.swap)
-        return plan.bn == 16   ? launch<16, QROW, true, TOut>(mp, mq, mc, p, st)
-               : plan.bn == 32 ? launch<32, QROW, true, TOut>(mp, mq, mc, p, st)
-                               : launch<64, QROW, true, TOut>(mp, mq, mc, p, st);
-    return plan.bn == 16    ? launch<16, QROW, false, TOut>(mp, mq, mc, p, st)
-           : plan.bn == 32  ? launch<32, QROW, false, TOut>(mp, mq, mc, p, st)
-           : plan.bn == 64  ? launch<64, QROW, false, TOut>(mp, mq, mc, p, st)
-           : plan.bn == 128 ? launch<128, QROW, false, TOut>(mp, mq, mc, p, st)
-                            : launch<256, QROW, false, TOut>(mp, mq, mc, p, st);
+        return plan.bn == 16   ? launch<16, QROW, true, false, TOut>(mp, mq, mc, p, st)
+               : plan.bn == 32 ? launch<32, QROW, true, false, TOut>(mp, mq, mc, p, st)
+                               : launch<64, QROW, true, false, TOut>(mp, mq, mc, p, st);
+    return plan.bn == 16    ? launch<16, QROW, false, false, TOut>(mp, mq, mc, p, st)
+           : plan.bn == 32  ? launch<32, QROW, false, false, TOut>(mp, mq, mc, p, st)
+           : plan.bn == 64  ? launch<64, QROW, false, false, TOut>(mp, mq, mc, p, st)
+           : plan.bn == 128 ? launch<128, QROW, false, false, TOut>(mp, mq, mc, p, st)
+                            : launch<256, QROW, false, false, TOut>(mp, mq, mc, p, st);
 }
 
 template <typename TOut>
@@ -751,7 +823,7 @@ extern "C" int gnnagg_fp8_matmul(const uint8_t *A, int64_t lda, const float *sa,
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const Plan plan = plan_of(M, N, K);
     if (K == 0) return join_out(out_type, plan, nullptr, 0, M, N, bias, bias_type, accumulate, C, ldc, st);
-    const bool split = plan.splits > 1;
+    const bool split = plan.splits > 1 && !plan.join;  // through the workspace
     if (split && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < plan.bytes()))
         return fail(GNNAGG_ERR_SCRATCH, "fp8_matmul: workspace too small or misaligned (need %zu bytes)", plan.bytes());
     if ((int64_t)plan.tiles_p * plan.tiles_q * plan.splits > 0x7FFFFFFF)
