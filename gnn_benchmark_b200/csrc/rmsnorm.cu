@@ -5,8 +5,8 @@
 //     dh = gh + r * (w gy - hat * mean(w gy hat)),  hat = h r;   dw = sum over rows of gy hat
 //
 // Forward is one pass: a row stays in registers, as it lies in memory, between the sum of squares and the scaling.  A
-// row of up to 128 16-byte chunks belongs to a warp (short ones two at a time, so that a warp has 1 to 2 KB on their
-// way), a longer one to a block of as many threads as it fills.  Backward reads h and the two gradients once, writes dh
+// row of up to 16 16-byte chunks belongs to half a warp, of up to 128 to a warp (short ones two at a time, so that a warp
+// has 1 to 2 KB on their way), a longer one to a block of as many threads as it fills.  Backward reads h and the two gradients once, writes dh
 // once and keeps the column sums of dw in registers over all rows of a persistent block; a second kernel adds the
 // blocks' sums in a fixed order (no atomics).
 //
@@ -23,12 +23,13 @@ constexpr int kBlockThreads = 512;  // largest block of the block-per-row forms
 constexpr int kWideThreads = 1024;  // block of rows too wide for these
 constexpr int kMaxWidth = 16384;
 
-// Sum over the threads of a row (WARP: a warp, else the block); every thread gets it.  `red` holds a value per warp.
-template <bool WARP>
+// Threads of a row: L = 32 or 16 lanes of a warp, or (L = 0) the block.
+// Sum over them; every one gets it.  `red` holds a value per warp.
+template <int L>
 __device__ __forceinline__ float row_sum(float v, float *red) {
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(kFullMask, v, off);
-    if (WARP) return v;
+    for (int off = L == 16 ? 8 : 16; off > 0; off >>= 1) v += __shfl_xor_sync(kFullMask, v, off);
+    if (L > 0) return v;
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
     float s = 0.0f;
@@ -66,21 +67,21 @@ struct FwdParams {
     float eps;
 };
 
-// NV chunks a thread and row, R rows a warp at once.
-template <typename T, bool WARP, int NV, int R, bool VEC, bool FP8>
-__global__ void __launch_bounds__(WARP ? kRowThreads : kBlockThreads) rms_norm_fwd_kernel(const FwdParams p) {
+// NV chunks a thread and row, R rows a group of threads at once.
+template <typename T, int L, int NV, int R, bool VEC, bool FP8>
+__global__ void __launch_bounds__(L > 0 ? kRowThreads : kBlockThreads) rms_norm_fwd_kernel(const FwdParams p) {
     constexpr int V = Vec<T>::N;
     __shared__ float red[32];
-    const int lane = WARP ? threadIdx.x & 31 : threadIdx.x, step = WARP ? 32 : blockDim.x;
-    const int64_t row0 = WARP ? ((int64_t)blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5)) * R : blockIdx.x;
-    if (WARP && row0 >= p.rows) return;  // whole warps
+    const int lane = L > 0 ? threadIdx.x & (L - 1) : threadIdx.x, step = L > 0 ? L : blockDim.x;
+    const int64_t row0 = L > 0 ? ((int64_t)blockIdx.x * (kRowThreads / (L + !L)) + threadIdx.x / (L + !L)) * R : blockIdx.x;
+    if (L == 32 && row0 >= p.rows) return;  // whole warps; half a warp stays for the other half's exchanges
     uint4 h[R][NV], res[R][NV];
 #pragma unroll
     for (int k = 0; k < R; ++k)
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int col = (lane + step * j) * V, valid = p.F - col;
-            const bool in = valid > 0 && (R == 1 || row0 + k < p.rows);
+            const bool in = valid > 0 && ((L != 16 && R == 1) || row0 + k < p.rows);
             h[k][j] = res[k][j] = make_uint4(0, 0, 0, 0);
             if (in) h[k][j] = load_raw<T, VEC>(static_cast<const T *>(p.x) + (row0 + k) * p.ldx + col, valid);
             if (in && p.residual != nullptr)
@@ -89,7 +90,8 @@ __global__ void __launch_bounds__(WARP ? kRowThreads : kBlockThreads) rms_norm_f
 #pragma unroll
     for (int k = 0; k < R; ++k) {
         const int64_t row = row0 + k;
-        if (R > 1 && row >= p.rows) break;
+        if (L != 16 && R > 1 && row >= p.rows) break;
+        const bool live = L != 16 || row < p.rows;
         float ss = 0.0f;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
@@ -103,13 +105,13 @@ __global__ void __launch_bounds__(WARP ? kRowThreads : kBlockThreads) rms_norm_f
                 h[k][j] = pack16<T>(v);
                 unpack16<T>(h[k][j], v);  // the norm is of the rounded sum
                 const int col = (lane + step * j) * V, valid = p.F - col;
-                if (valid > 0) store_raw<T, VEC>(static_cast<T *>(p.h) + row * p.ldh + col, valid, h[k][j]);
+                if (valid > 0 && live) store_raw<T, VEC>(static_cast<T *>(p.h) + row * p.ldh + col, valid, h[k][j]);
             }
 #pragma unroll
             for (int i = 0; i < V; ++i) ss = fmaf(v[i], v[i], ss);
         }
-        const float rstd = rsqrtf(row_sum<WARP>(ss, red) / (float)p.F + p.eps);
-        if (lane == 0 && p.rstd != nullptr) p.rstd[row] = rstd;
+        const float rstd = rsqrtf(row_sum<L>(ss, red) / (float)p.F + p.eps);
+        if (lane == 0 && live && p.rstd != nullptr) p.rstd[row] = rstd;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int col = (lane + step * j) * V, valid = p.F - col;
@@ -119,7 +121,7 @@ __global__ void __launch_bounds__(WARP ? kRowThreads : kBlockThreads) rms_norm_f
             for (int i = 0; i < V; ++i) w[i] = 0.0f;
             if (valid > 0) load_weight<T, VEC>(p.w, p.w_f32 != 0, col, valid, w);
             if (!FP8) {
-                if (valid > 0) {
+                if (valid > 0 && live) {
 #pragma unroll
                     for (int i = 0; i < V; ++i) v[i] = v[i] * rstd * w[i];
                     store_chunk<T, VEC>(static_cast<T *>(p.y) + row * p.ldy + col, valid, v);
@@ -131,11 +133,11 @@ __global__ void __launch_bounds__(WARP ? kRowThreads : kBlockThreads) rms_norm_f
                     v[i] = __fmul_rn(v[i], w[i]);
                     m = max(m, abs_bits(v[i]));
                 }
-                // 128 columns are 128 / V neighbouring threads: a whole or half a warp
+                // 128 columns are 128 / V neighbouring threads: a whole or half a warp (or all of the row)
 #pragma unroll
-                for (int off = 64 / V; off > 0; off >>= 1) m = max(m, __shfl_xor_sync(kFullMask, m, off));
+                for (int off = L == 16 ? 8 : 64 / V; off > 0; off >>= 1) m = max(m, __shfl_xor_sync(kFullMask, m, off));
                 const float a = block_amax(m), f = block_factor(a);
-                if (valid > 0) {
+                if (valid > 0 && live) {
                     // code rows are padded to 16 bytes, so a whole chunk always fits; columns from F on are zeros
                     uint32_t c[V / 4];
 #pragma unroll
@@ -163,13 +165,16 @@ struct BwdParams {
     int F, w_f32;
 };
 
-template <typename T, bool WARP, int NV, bool VEC>
-__global__ void __launch_bounds__(WARP ? kRowThreads : kBlockThreads) rms_norm_bwd_kernel(const BwdParams p) {
+// Blocks per SM that the register limit is set for, as measured: more rows on their way against registers that spill.
+template <typename T, int L, int NV, bool VEC>
+__global__ void __launch_bounds__(L > 0 ? kRowThreads : kBlockThreads, L > 0 ? (NV == 1 ? 4 : NV == 2 ? 3 : 2) : NV == 4 ? 1 : 2)
+rms_norm_bwd_kernel(const BwdParams p) {
     constexpr int V = Vec<T>::N;
-    constexpr int kRows = WARP ? kRowThreads / 32 : 1;
+    constexpr int kRows = L > 0 ? kRowThreads / (L + !L) : 1, kWarpRows = L == 16 ? 2 : 1;
     __shared__ float red[2][32];
-    __shared__ float cols[WARP ? kRows * 32 * V : 1];
-    const int lane = WARP ? threadIdx.x & 31 : threadIdx.x, step = WARP ? 32 : blockDim.x, slot = WARP ? threadIdx.x >> 5 : 0;
+    __shared__ float cols[L > 0 ? kRowThreads * V : 1];
+    const int lane = L > 0 ? threadIdx.x & (L - 1) : threadIdx.x, step = L > 0 ? L : blockDim.x;
+    const int slot = L > 0 ? threadIdx.x / (L + !L) : 0;
     const float inv_f = 1.0f / (float)p.F;
     float dw[NV][V];
 #pragma unroll
@@ -177,19 +182,23 @@ __global__ void __launch_bounds__(WARP ? kRowThreads : kBlockThreads) rms_norm_b
 #pragma unroll
         for (int i = 0; i < V; ++i) dw[j][i] = 0.0f;
     int turn = 0;
-    for (int64_t row = (int64_t)blockIdx.x * kRows + slot; row < p.rows; row += (int64_t)gridDim.x * kRows, turn ^= 1) {
+    // a warp's rows go round together: its halves meet in the exchanges
+    for (int64_t base = (int64_t)blockIdx.x * kRows + slot / kWarpRows * kWarpRows; base < p.rows;
+         base += (int64_t)gridDim.x * kRows, turn ^= 1) {
+        const int64_t row = base + slot % kWarpRows;
+        const bool live = L != 16 || row < p.rows;
         uint4 h[NV], g[NV], gh[NV];
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int col = (lane + step * j) * V, valid = p.F - col;
             h[j] = g[j] = gh[j] = make_uint4(0, 0, 0, 0);
-            if (valid > 0) {
+            if (valid > 0 && live) {
                 h[j] = load_raw<T, VEC>(static_cast<const T *>(p.h) + row * p.ldh + col, valid);
                 g[j] = load_raw<T, VEC>(static_cast<const T *>(p.gy) + row * p.ldgy + col, valid);
                 if (p.gh != nullptr) gh[j] = load_raw<T, VEC>(static_cast<const T *>(p.gh) + row * p.ldgh + col, valid);
             }
         }
-        const float rstd = __ldg(p.rstd + row);
+        const float rstd = live ? __ldg(p.rstd + row) : 0.0f;
         float s = 0.0f;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
@@ -207,11 +216,11 @@ __global__ void __launch_bounds__(WARP ? kRowThreads : kBlockThreads) rms_norm_b
                 s = fmaf(y[i] * w[i], hat, s);
             }
         }
-        const float c = row_sum<WARP>(s, red[turn]) * inv_f;  // two buffers: a warp may be a row ahead of another
+        const float c = row_sum<L>(s, red[turn]) * inv_f;  // two buffers: a warp may be a row ahead of another
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int col = (lane + step * j) * V, valid = p.F - col;
-            if (valid > 0) {
+            if (valid > 0 && live) {
                 float x[V], y[V], w[V], o[V];
                 unpack16<T>(h[j], x);
                 unpack16<T>(g[j], y);
@@ -227,16 +236,16 @@ __global__ void __launch_bounds__(WARP ? kRowThreads : kBlockThreads) rms_norm_b
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const int col = (lane + step * j) * V;
-        if (WARP) {  // the block's warps add up in warp order
+        if (L > 0) {  // the block's rows add up in their order
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < V; ++i) cols[(slot * V + i) * 32 + lane] = dw[j][i];
+            for (int i = 0; i < V; ++i) cols[(slot * V + i) * L + lane] = dw[j][i];
             __syncthreads();
-            for (int e = threadIdx.x; e < 32 * V; e += kRowThreads) {
+            for (int e = threadIdx.x; e < L * V; e += kRowThreads) {
                 float s = 0.0f;
 #pragma unroll
-                for (int r = 0; r < kRows; ++r) s += cols[r * 32 * V + e];
-                const int c = ((e & 31) + 32 * j) * V + (e >> 5);
+                for (int r = 0; r < kRows; ++r) s += cols[r * L * V + e];
+                const int c = (e % (L + !L) + L * j) * V + e / (L + !L);
                 if (c < p.F) out[c] = s;
             }
         } else {
@@ -276,7 +285,7 @@ __global__ void __launch_bounds__(kWideThreads) rms_norm_bwd_wide_kernel(const B
                 s = fmaf(g[i] * w[i], hat[i], s);
             }
         }
-        const float c = row_sum<false>(s, red[turn]) * inv_f;
+        const float c = row_sum<0>(s, red[turn]) * inv_f;
         for (int k = threadIdx.x; k < chunks; k += kWideThreads) {
             const int col = k * V, valid = p.F - col;
             float hat[V], g[V], w[V], gh[V];
@@ -298,24 +307,42 @@ __global__ void __launch_bounds__(kWideThreads) rms_norm_bwd_wide_kernel(const B
             if (k * V + i < p.F) out[k * V + i] = dw[i * chunks + k];
 }
 
-// How a row of F elements of `size` bytes is spread: over a warp (threads = 32) or a block, with nv 16-byte chunks a
-// thread; nv = 0: too wide for registers.
+// How a row of F elements of `size` bytes is spread: over half a warp, a warp (lanes = 16, 32) or a block (lanes = 0) of
+// `threads`, with nv 16-byte chunks a thread; nv = 0: too wide for registers.
 struct Spread {
-    int threads, nv;
+    int lanes, threads, nv;
 };
 Spread spread_of(int F, int size) {
     const int chunks = (int)div_up(F, 16 / size);
-    if (chunks <= 128) return {32, chunks <= 32 ? 1 : chunks <= 64 ? 2 : 4};
+    if (chunks <= 16) return {16, kRowThreads, 1};
+    if (chunks <= 128) return {32, kRowThreads, chunks <= 32 ? 1 : chunks <= 64 ? 2 : 4};
     const int nv = chunks <= 256 ? 1 : chunks <= 2 * kBlockThreads ? 2 : 4;
-    if (chunks > 4 * kBlockThreads) return {kWideThreads, 0};
-    return {(int)div_up(div_up(chunks, nv), 32) * 32, nv};
+    if (chunks > 4 * kBlockThreads) return {0, kWideThreads, 0};
+    return {0, (int)div_up(div_up(chunks, nv), 32) * 32, nv};
 }
 
+// Most blocks a backward launch has: the partial sums' rows.
+constexpr int kMostPerSm = 6;
 int bwd_blocks(int64_t rows, int F, int size) {
     const Spread s = spread_of(F, size);
-    const int64_t need = div_up(rows, s.threads == 32 ? kRowThreads / 32 : 1);
-    const int64_t cap = (int64_t)kNumSMs * (s.nv == 0 ? 2 : 4);
+    const int64_t need = div_up(rows, s.lanes > 0 ? kRowThreads / s.lanes : 1);
+    const int64_t cap = (int64_t)kNumSMs * (s.nv == 0 ? 2 : kMostPerSm);
     return (int)(need < cap ? need : cap);
+}
+
+// Blocks of `threads` threads that an SM holds of KERNEL: a persistent grid is one full wave (with a block too many or
+// too few per SM the backward takes up to a third longer).
+template <auto KERNEL>
+int resident(int threads) {
+    static int known[PerDeviceOnce::kMaxDevices][kWideThreads / 32 + 1];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= PerDeviceOnce::kMaxDevices) return 1;
+    int n = __atomic_load_n(&known[dev][threads / 32], __ATOMIC_RELAXED);
+    if (n == 0) {
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, KERNEL, threads, 0) != cudaSuccess || n < 1) n = 1;
+        __atomic_store_n(&known[dev][threads / 32], n, __ATOMIC_RELAXED);
+    }
+    return n < kMostPerSm ? n : kMostPerSm;
 }
 
 template <typename F32, typename BF16, typename F16>
@@ -326,12 +353,13 @@ int by_type(int type, F32 a, BF16 b, F16 c) {
 template <typename T, bool VEC, bool FP8>
 int launch_fwd(const FwdParams &p, cudaStream_t st) {
     const Spread s = spread_of(p.F, (int)sizeof(T));
-#define RMS_WARP(NV, R) \
-    rms_norm_fwd_kernel<T, true, NV, R, VEC, FP8><<<(unsigned)div_up(p.rows, kRowThreads / 32 * R), kRowThreads, 0, st>>>(p)
-#define RMS_BLOCK(NV, THREADS) rms_norm_fwd_kernel<T, false, NV, 1, VEC, FP8><<<(unsigned)p.rows, THREADS, 0, st>>>(p)
-    if (s.threads == 32 && s.nv == 1) RMS_WARP(1, 2);
-    else if (s.threads == 32 && s.nv == 2) RMS_WARP(2, 1);
-    else if (s.threads == 32) RMS_WARP(4, 1);
+#define RMS_WARP(L, NV, R) \
+    rms_norm_fwd_kernel<T, L, NV, R, VEC, FP8><<<(unsigned)div_up(p.rows, kRowThreads / L * R), kRowThreads, 0, st>>>(p)
+#define RMS_BLOCK(NV, THREADS) rms_norm_fwd_kernel<T, 0, NV, 1, VEC, FP8><<<(unsigned)p.rows, THREADS, 0, st>>>(p)
+    if (s.lanes == 16) RMS_WARP(16, 1, 2);
+    else if (s.lanes == 32 && s.nv == 1) RMS_WARP(32, 1, 2);
+    else if (s.lanes == 32 && s.nv == 2) RMS_WARP(32, 2, 1);
+    else if (s.lanes == 32) RMS_WARP(32, 4, 1);
     else if (s.nv == 1) RMS_BLOCK(1, s.threads);
     else if (s.nv == 2) RMS_BLOCK(2, s.threads);
     else if (s.nv == 4) RMS_BLOCK(4, s.threads);
@@ -341,16 +369,23 @@ int launch_fwd(const FwdParams &p, cudaStream_t st) {
     return check_launch("rms_norm_fwd_kernel");
 }
 
+// `blocks`: at most this many; becomes the number of blocks (rows of partial sums).
 template <typename T, bool VEC>
-int launch_bwd(const BwdParams &p, int blocks, cudaStream_t st) {
+int launch_bwd(const BwdParams &p, int &blocks, cudaStream_t st) {
     const Spread s = spread_of(p.F, (int)sizeof(T));
-#define RMS_LAUNCH(WARP, NV, THREADS) rms_norm_bwd_kernel<T, WARP, NV, VEC><<<blocks, THREADS, 0, st>>>(p)
-    if (s.threads == 32 && s.nv == 1) RMS_LAUNCH(true, 1, kRowThreads);
-    else if (s.threads == 32 && s.nv == 2) RMS_LAUNCH(true, 2, kRowThreads);
-    else if (s.threads == 32) RMS_LAUNCH(true, 4, kRowThreads);
-    else if (s.nv == 1) RMS_LAUNCH(false, 1, s.threads);
-    else if (s.nv == 2) RMS_LAUNCH(false, 2, s.threads);
-    else if (s.nv == 4) RMS_LAUNCH(false, 4, s.threads);
+#define RMS_LAUNCH(L, NV)                                                                    \
+    do {                                                                                     \
+        const int wave = kNumSMs * resident<rms_norm_bwd_kernel<T, L, NV, VEC>>(s.threads);  \
+        if (blocks > wave) blocks = wave;                                                    \
+        rms_norm_bwd_kernel<T, L, NV, VEC><<<blocks, s.threads, 0, st>>>(p);                 \
+    } while (0)
+    if (s.lanes == 16) RMS_LAUNCH(16, 1);
+    else if (s.lanes == 32 && s.nv == 1) RMS_LAUNCH(32, 1);
+    else if (s.lanes == 32 && s.nv == 2) RMS_LAUNCH(32, 2);
+    else if (s.lanes == 32) RMS_LAUNCH(32, 4);
+    else if (s.nv == 1) RMS_LAUNCH(0, 1);
+    else if (s.nv == 2) RMS_LAUNCH(0, 2);
+    else if (s.nv == 4) RMS_LAUNCH(0, 4);
     else {
         static PerDeviceOnce attr_done;
         const cudaError_t e = attr_done.run([] {
@@ -447,7 +482,8 @@ extern "C" int gnnagg_rms_norm_bwd(const void *gy, int64_t ldgy, const void *gh,
         return fail(GNNAGG_ERR_ARG, "rms_norm_bwd: null pointer");
     if (rows > 0 && (ldgy < F || ldh < F || ldgx < F || (gh != nullptr && ldgh < F)))
         return fail(GNNAGG_ERR_ARG, "rms_norm_bwd: a stride is smaller than its rows");
-    const int size = type_size(type), blocks = bwd_blocks(rows, F, size);
+    const int size = type_size(type);
+    int blocks = bwd_blocks(rows, F, size);
     if (partial_bytes < gnnagg_rms_norm_partial_bytes(rows, F, type))
         return fail(GNNAGG_ERR_SCRATCH, "rms_norm_bwd: partial-sum scratch too small");
     cudaStream_t st = static_cast<cudaStream_t>(stream);

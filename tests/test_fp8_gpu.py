@@ -75,6 +75,10 @@ CASES = [  # m, n, k: one row, few rows (weight rows along the lanes), ragged ed
     (1, 1, 1), (1, 128, 128), (1, 4096, 512), (7, 300, 1000), (16, 256, 4096), (17, 130, 200), (33, 1000, 640), (64, 64, 64),
     (65, 16, 128), (100, 17, 256), (128, 47, 100), (200, 100, 300), (300, 129, 1500), (257, 256, 129), (1000, 700, 260),
     (5003, 47, 100), (256, 256, 40000), (47, 100, 30001), (2500, 2048, 384), (20000, 256, 100), (3000, 1500, 1111),
+    # a weight that stays in shared memory (one to three k-blocks, narrow and wide), clusters of two to eight splits with
+    # 16, 32 and 64 columns, and splits too many or too large for a cluster
+    (20000, 200, 384), (20000, 47, 300), (19000, 128, 128), (38000, 16, 129), (20, 500, 4000), (50, 500, 3000), (3, 200, 1100),
+    (50, 500, 4000), (9, 130, 9000),
 ]
 
 
@@ -257,12 +261,14 @@ def test_linear_without_rows_and_broadcast_gradient():
     assert all(torch.equal(s, t) for s, t in zip(a, c))
 
 
-def test_bounded_wait_gives_up_and_reports():
-    """A launch that waits for bytes which never come returns by itself, leaves its code, and the next is right."""
+@pytest.mark.parametrize("m,n,k", [(300, 200, 256), (300, 100, 256), (20000, 200, 200), (5, 2000, 4096), (40, 200, 20000)])
+def test_bounded_wait_gives_up_and_reports(m, n, k):
+    """A launch that waits for bytes which never come returns by itself, leaves its code, and the next is right: wide and
+    narrow tiles, a weight that stays, a cluster, splits through the workspace."""
     from gnn_benchmark_b200 import _lib, dense
 
     lib = _lib.lib()
-    qa, qb = dense.quantize_fp8(_matrix(300, 256, 1)), dense.quantize_fp8(_matrix(200, 256, 2), (128, 128))
+    qa, qb = dense.quantize_fp8(_matrix(m, k, 1)), dense.quantize_fp8(_matrix(n, k, 2), (128, 128))
     want = dense.matmul_fp8(*qa, *qb)
     dense.check_status()
     _lib.check(lib.gnnagg_dense_stall_test(16, 3000), "stall_test")
