@@ -69,7 +69,14 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2) fp8_quantize
         raw[i] = make_uint4(0, 0, 0, 0);
         if (row < p.rows && valid > 0) raw[i] = load_raw<T, VEC>(static_cast<const T *>(p.x) + row * p.ldx + col, valid);
     }
-    auto at = [&raw](int i, int e) { return to_f32(reinterpret_cast<const T *>(&raw[i])[e]); };
+    auto at = [&raw](int i, int e) {
+        const uint32_t words[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+        if (sizeof(T) == 4) return __uint_as_float(words[e]);
+        const uint32_t w = words[e / 2 % 4];
+        if (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(e % 2 ? w & 0xFFFF0000u : w << 16);
+        const uint16_t h = (uint16_t)(e % 2 ? w >> 16 : w);
+        return to_f32(*reinterpret_cast<const T *>(&h));
+    };
     if (BLOCK) {
         if (threadIdx.x == 0) top = 0;
         __syncthreads();

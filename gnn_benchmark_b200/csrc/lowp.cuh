@@ -6,6 +6,8 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace gnnagg {
@@ -65,19 +67,41 @@ struct Vec {
     static constexpr int N = 16 / (int)sizeof(T);  // elements of one 16-byte access
 };
 
+// A 16-byte vector as fp32 values and back, one instruction an element and one for two (element by element the
+// compiler takes two each).
 template <typename T>
 __device__ __forceinline__ void unpack16(const uint4 &u, float (&f)[Vec<T>::N]) {
-    const T *e = reinterpret_cast<const T *>(&u);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-    for (int i = 0; i < Vec<T>::N; ++i) f[i] = to_f32(e[i]);
+    for (int i = 0; i < 4; ++i) {
+        if (std::is_same<T, float>::value) {
+            f[i] = __uint_as_float(w[i]);
+        } else if (std::is_same<T, __nv_bfloat16>::value) {  // the upper half of an fp32
+            f[2 * i % Vec<T>::N] = __uint_as_float(w[i] << 16);
+            f[(2 * i + 1) % Vec<T>::N] = __uint_as_float(w[i] & 0xFFFF0000u);
+        } else {
+            const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+            f[2 * i % Vec<T>::N] = v.x, f[(2 * i + 1) % Vec<T>::N] = v.y;
+        }
+    }
 }
 template <typename T>
 __device__ __forceinline__ uint4 pack16(const float (&f)[Vec<T>::N]) {
-    uint4 u;
-    T *e = reinterpret_cast<T *>(&u);
+    uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < Vec<T>::N; ++i) e[i] = from_f32<T>(f[i]);
-    return u;
+    for (int i = 0; i < 4; ++i) {
+        const float a = f[2 * i % Vec<T>::N], b = f[(2 * i + 1) % Vec<T>::N];
+        if (std::is_same<T, float>::value) {
+            w[i] = __float_as_uint(f[i]);
+        } else if (std::is_same<T, __nv_bfloat16>::value) {
+            const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+            w[i] = *reinterpret_cast<const uint32_t *>(&v);
+        } else {
+            const __half2 v = __floats2half2_rn(a, b);
+            w[i] = *reinterpret_cast<const uint32_t *>(&v);
+        }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // Vec<T>::N consecutive elements at p, of which `valid` exist (the others read as zero), as they lie in memory: a

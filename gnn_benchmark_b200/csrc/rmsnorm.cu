@@ -24,7 +24,13 @@ constexpr int kWideThreads = 1024;  // block of rows too wide for these
 constexpr int kMaxWidth = 16384;
 
 // Threads of a row: L = 32 or 16 lanes of a warp, or (L = 0) the block.
-// Sum over them; every one gets it.  `red` holds a value per warp.
+// Sum over them; every one gets it.  `red` holds a value per warp of up to 32, zero for those that the block lacks
+// (clear_sums), and is on 16 bytes.
+template <int N>
+__device__ __forceinline__ void clear_sums(float (&red)[N][32]) {
+    for (int i = threadIdx.x; i < N * 32; i += blockDim.x) red[i / 32][i % 32] = 0.0f;
+    __syncthreads();
+}
 template <int L>
 __device__ __forceinline__ float row_sum(float v, float *red) {
 #pragma unroll
@@ -32,9 +38,15 @@ __device__ __forceinline__ float row_sum(float v, float *red) {
     if (L > 0) return v;
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
-    float s = 0.0f;
-    for (int i = 0; i < (int)blockDim.x / 32; ++i) s += red[i];
-    return s;
+    const float4 *r = reinterpret_cast<const float4 *>(red);
+    float4 s = r[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+        if (i >= 4 && blockDim.x <= 512) break;
+        const float4 u = r[i];
+        s.x += u.x, s.y += u.y, s.z += u.z, s.w += u.w;
+    }
+    return (s.x + s.y) + (s.z + s.w);
 }
 
 template <typename T, bool VEC>
@@ -71,7 +83,8 @@ struct FwdParams {
 template <typename T, int L, int NV, int R, bool VEC, bool FP8>
 __global__ void __launch_bounds__(L > 0 ? kRowThreads : kBlockThreads) rms_norm_fwd_kernel(const FwdParams p) {
     constexpr int V = Vec<T>::N;
-    __shared__ float red[32];
+    __shared__ __align__(16) float red[1][32];
+    if (L == 0) clear_sums(red);
     const int lane = L > 0 ? threadIdx.x & (L - 1) : threadIdx.x, step = L > 0 ? L : blockDim.x;
     const int64_t row0 = L > 0 ? ((int64_t)blockIdx.x * (kRowThreads / (L + !L)) + threadIdx.x / (L + !L)) * R : blockIdx.x;
     if (L == 32 && row0 >= p.rows) return;  // whole warps; half a warp stays for the other half's exchanges
@@ -110,7 +123,7 @@ __global__ void __launch_bounds__(L > 0 ? kRowThreads : kBlockThreads) rms_norm_
 #pragma unroll
             for (int i = 0; i < V; ++i) ss = fmaf(v[i], v[i], ss);
         }
-        const float rstd = rsqrtf(row_sum<L>(ss, red) / (float)p.F + p.eps);
+        const float rstd = rsqrtf(row_sum<L>(ss, red[0]) / (float)p.F + p.eps);
         if (lane == 0 && live && p.rstd != nullptr) p.rstd[row] = rstd;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
@@ -171,10 +184,11 @@ __global__ void __launch_bounds__(L > 0 ? kRowThreads : kBlockThreads, L > 0 ? (
 rms_norm_bwd_kernel(const BwdParams p) {
     constexpr int V = Vec<T>::N;
     constexpr int kRows = L > 0 ? kRowThreads / (L + !L) : 1, kWarpRows = L == 16 ? 2 : 1;
-    __shared__ float red[2][32];
+    __shared__ __align__(16) float red[2][32];
     __shared__ float cols[L > 0 ? kRowThreads * V : 1];
     const int lane = L > 0 ? threadIdx.x & (L - 1) : threadIdx.x, step = L > 0 ? L : blockDim.x;
     const int slot = L > 0 ? threadIdx.x / (L + !L) : 0;
+    if (L == 0) clear_sums(red);
     const float inv_f = 1.0f / (float)p.F;
     float dw[NV][V];
 #pragma unroll
@@ -216,7 +230,7 @@ rms_norm_bwd_kernel(const BwdParams p) {
                 s = fmaf(y[i] * w[i], hat, s);
             }
         }
-        const float c = row_sum<L>(s, red[turn]) * inv_f;  // two buffers: a warp may be a row ahead of another
+        const float minus = -rstd * row_sum<L>(s, red[turn]) * inv_f;  // two buffers: a warp may be a row ahead of another
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int col = (lane + step * j) * V, valid = p.F - col;
@@ -227,7 +241,7 @@ rms_norm_bwd_kernel(const BwdParams p) {
                 unpack16<T>(gh[j], o);
                 load_weight<T, VEC>(p.w, p.w_f32 != 0, col, valid, w);
 #pragma unroll
-                for (int i = 0; i < V; ++i) o[i] = fmaf(rstd, y[i] * w[i] - x[i] * rstd * c, o[i]);
+                for (int i = 0; i < V; ++i) o[i] = fmaf(rstd, fmaf(x[i], minus, y[i] * w[i]), o[i]);
                 store_chunk<T, VEC>(static_cast<T *>(p.gx) + row * p.ldgx + col, valid, o);
             }
         }
@@ -256,17 +270,102 @@ rms_norm_bwd_kernel(const BwdParams p) {
     }
 }
 
+// The block-per-row form on 16-byte rows: the next row's chunks are copied to shared memory (cp.async, every thread its
+// own, so that no barrier is needed for them) while the block works on this one.  Without, a block's three loads, its
+// reduction and its store follow one another: 78 us instead of MEASURED at 8191 x 5000 bf16.
+template <typename T, int NV>
+__global__ void __launch_bounds__(kBlockThreads, NV == 4 ? 1 : 2) rms_norm_bwd_ahead_kernel(const BwdParams p) {
+    constexpr int V = Vec<T>::N;
+    extern __shared__ __align__(16) uint4 ahead[];  // [2][3 * NV][threads]
+    __shared__ __align__(16) float red[2][32];
+    const int tid = threadIdx.x, step = blockDim.x;
+    clear_sums(red);
+    const float inv_f = 1.0f / (float)p.F;
+    auto slot = [&](int turn, int k) -> uint4 * { return ahead + (turn * 3 * NV + k) * step + tid; };
+    auto fetch = [&](int64_t row, int turn) {
+        if (row < p.rows) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int col = (tid + step * j) * V;
+                if (col < p.F) {
+                    cp_async_16(slot(turn, 3 * j), static_cast<const T *>(p.h) + row * p.ldh + col);
+                    cp_async_16(slot(turn, 3 * j + 1), static_cast<const T *>(p.gy) + row * p.ldgy + col);
+                    if (p.gh != nullptr) cp_async_16(slot(turn, 3 * j + 2), static_cast<const T *>(p.gh) + row * p.ldgh + col);
+                }
+            }
+        }
+        cp_async_commit();
+    };
+    float dw[NV][V];
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) dw[j][i] = 0.0f;
+    fetch(blockIdx.x, 0);
+    float next = __ldg(p.rstd + blockIdx.x);  // there are no more blocks than rows
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
+        const float rstd = next;
+        if (row + gridDim.x < p.rows) next = __ldg(p.rstd + row + gridDim.x);
+        fetch(row + gridDim.x, turn ^ 1);
+        cp_async_wait<1>();
+        float s = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int col = (tid + step * j) * V;
+            if (col < p.F) {
+                float x[V], y[V], w[V];
+                unpack16<T>(*slot(turn, 3 * j), x);
+                unpack16<T>(*slot(turn, 3 * j + 1), y);
+                load_weight<T, true>(p.w, p.w_f32 != 0, col, V, w);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float hat = x[i] * rstd;
+                    dw[j][i] = fmaf(y[i], hat, dw[j][i]);
+                    s = fmaf(y[i] * w[i], hat, s);
+                }
+            }
+        }
+        const float minus = -rstd * row_sum<0>(s, red[turn]) * inv_f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int col = (tid + step * j) * V;
+            if (col < p.F) {
+                float x[V], y[V], w[V], o[V];
+                unpack16<T>(*slot(turn, 3 * j), x);
+                unpack16<T>(*slot(turn, 3 * j + 1), y);
+#pragma unroll
+                for (int i = 0; i < V; ++i) o[i] = 0.0f;
+                if (p.gh != nullptr) unpack16<T>(*slot(turn, 3 * j + 2), o);
+                load_weight<T, true>(p.w, p.w_f32 != 0, col, V, w);
+#pragma unroll
+                for (int i = 0; i < V; ++i) o[i] = fmaf(rstd, fmaf(x[i], minus, y[i] * w[i]), o[i]);
+                store_chunk<T, true>(static_cast<T *>(p.gx) + row * p.ldgx + col, V, o);
+            }
+        }
+    }
+    cp_async_wait<0>();
+    float *out = p.partial + (int64_t)blockIdx.x * p.F;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int col = (tid + step * j) * V;
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (col + i < p.F) out[col + i] = dw[j][i];
+    }
+}
+
 // Rows too wide for the registers of a block: two sweeps over the row (the second finds it in L1 / L2), and the
 // column sums of dw in shared memory, where every thread adds to columns of its own.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kWideThreads) rms_norm_bwd_wide_kernel(const BwdParams p) {
     constexpr int V = Vec<T>::N;
     extern __shared__ float dw[];  // [V][chunks]
-    __shared__ float red[2][32];
+    __shared__ __align__(16) float red[2][32];
     const int chunks = (p.F + V - 1) / V;
     const float inv_f = 1.0f / (float)p.F;
     for (int i = threadIdx.x; i < chunks * V; i += kWideThreads) dw[i] = 0.0f;
-    __syncthreads();
+    clear_sums(red);
     int turn = 0;
     for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
         const float rstd = __ldg(p.rstd + row);
@@ -285,7 +384,7 @@ __global__ void __launch_bounds__(kWideThreads) rms_norm_bwd_wide_kernel(const B
                 s = fmaf(g[i] * w[i], hat[i], s);
             }
         }
-        const float c = row_sum<0>(s, red[turn]) * inv_f;
+        const float minus = -rstd * row_sum<0>(s, red[turn]) * inv_f;
         for (int k = threadIdx.x; k < chunks; k += kWideThreads) {
             const int col = k * V, valid = p.F - col;
             float hat[V], g[V], w[V], gh[V];
@@ -296,7 +395,7 @@ __global__ void __launch_bounds__(kWideThreads) rms_norm_bwd_wide_kernel(const B
             for (int i = 0; i < V; ++i) gh[i] = 0.0f;
             if (p.gh != nullptr) load_chunk<T, VEC>(static_cast<const T *>(p.gh) + row * p.ldgh + col, valid, gh);
 #pragma unroll
-            for (int i = 0; i < V; ++i) gh[i] = fmaf(rstd, g[i] * w[i] - hat[i] * rstd * c, gh[i]);
+            for (int i = 0; i < V; ++i) gh[i] = fmaf(rstd, fmaf(hat[i], minus, g[i] * w[i]), gh[i]);
             store_chunk<T, VEC>(static_cast<T *>(p.gx) + row * p.ldgx + col, valid, gh);
         }
     }
@@ -330,16 +429,16 @@ int bwd_blocks(int64_t rows, int F, int size) {
     return (int)(need < cap ? need : cap);
 }
 
-// Blocks of `threads` threads that an SM holds of KERNEL: a persistent grid is one full wave (with a block too many or
+// Blocks of `threads` threads (and of their shared memory) that an SM holds of KERNEL: a persistent grid is one full wave (with a block too many or
 // too few per SM the backward takes up to a third longer).
 template <auto KERNEL>
-int resident(int threads) {
+int resident(int threads, size_t smem = 0) {
     static int known[PerDeviceOnce::kMaxDevices][kWideThreads / 32 + 1];
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= PerDeviceOnce::kMaxDevices) return 1;
     int n = __atomic_load_n(&known[dev][threads / 32], __ATOMIC_RELAXED);
     if (n == 0) {
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, KERNEL, threads, 0) != cudaSuccess || n < 1) n = 1;
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, KERNEL, threads, smem) != cudaSuccess || n < 1) n = 1;
         __atomic_store_n(&known[dev][threads / 32], n, __ATOMIC_RELAXED);
     }
     return n < kMostPerSm ? n : kMostPerSm;
@@ -379,11 +478,27 @@ int launch_bwd(const BwdParams &p, int &blocks, cudaStream_t st) {
         if (blocks > wave) blocks = wave;                                                    \
         rms_norm_bwd_kernel<T, L, NV, VEC><<<blocks, s.threads, 0, st>>>(p);                 \
     } while (0)
-    if (s.lanes == 16) RMS_LAUNCH(16, 1);
+#define RMS_AHEAD(NV)                                                                                            \
+    do {                                                                                                         \
+        static PerDeviceOnce attr_done;                                                                          \
+        const size_t smem = (size_t)2 * 3 * NV * s.threads * 16;                                                 \
+        const cudaError_t e = attr_done.run([] {                                                                 \
+            return cudaFuncSetAttribute(rms_norm_bwd_ahead_kernel<T, NV>,                                        \
+                                        cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * 3 * NV * kBlockThreads * 16); \
+        });                                                                                                      \
+        if (e != cudaSuccess) return fail(GNNAGG_ERR_CUDA, "rms_norm_bwd: %s", cudaGetErrorString(e));           \
+        const int wave = kNumSMs * resident<rms_norm_bwd_ahead_kernel<T, NV>>(s.threads, smem);                  \
+        if (blocks > wave) blocks = wave;                                                                        \
+        rms_norm_bwd_ahead_kernel<T, NV><<<blocks, s.threads, smem, st>>>(p);                                    \
+    } while (0)
+    if (VEC && s.lanes == 0 && s.nv == 1) RMS_AHEAD(1);
+    else if (VEC && s.lanes == 0 && s.nv == 2) RMS_AHEAD(2);
+    else if (VEC && s.lanes == 0 && s.nv == 4) RMS_AHEAD(4);
+    else if (s.lanes == 16) RMS_LAUNCH(16, 1);
     else if (s.lanes == 32 && s.nv == 1) RMS_LAUNCH(32, 1);
     else if (s.lanes == 32 && s.nv == 2) RMS_LAUNCH(32, 2);
     else if (s.lanes == 32) RMS_LAUNCH(32, 4);
-    else if (s.nv == 1) RMS_LAUNCH(0, 1);
+    else if (s.nv == 1) RMS_LAUNCH(0, 1);  // rows off 16 bytes
     else if (s.nv == 2) RMS_LAUNCH(0, 2);
     else if (s.nv == 4) RMS_LAUNCH(0, 4);
     else {
@@ -397,6 +512,7 @@ int launch_bwd(const BwdParams &p, int &blocks, cudaStream_t st) {
         rms_norm_bwd_wide_kernel<T, VEC><<<blocks, kWideThreads, smem, st>>>(p);
     }
 #undef RMS_LAUNCH
+#undef RMS_AHEAD
     return check_launch("rms_norm_bwd_kernel");
 }
 
