@@ -137,6 +137,42 @@ __device__ __forceinline__ void store_chunk(T *p, int valid, const float (&f)[Ve
     store_raw<T, VEC>(p, valid, pack16<T>(f));
 }
 
+// A thread's 16 bytes of a row as pieces of P neighbouring elements, one access each: piece q starts at column first +
+// q * step (columns from F on read as zero and are not written).  P = Vec<T>::N is a 16-byte vector; with smaller P, for
+// rows that do not allow it, neighbouring threads take neighbouring pieces, so that a warp's access is contiguous.
+template <int BYTES>
+struct Access;
+template <>
+struct Access<16> {
+    using type = uint4;
+};
+template <>
+struct Access<4> {
+    using type = uint32_t;
+};
+template <>
+struct Access<2> {
+    using type = uint16_t;
+};
+template <typename T, int P>
+__device__ __forceinline__ uint4 load_pieces(const T *row, int first, int step, int F) {
+    using A = typename Access<P * (int)sizeof(T)>::type;
+    uint4 u = make_uint4(0, 0, 0, 0);
+    A *piece = reinterpret_cast<A *>(&u);
+#pragma unroll
+    for (int q = 0; q < Vec<T>::N / P; ++q)
+        if (first + q * step < F) piece[q] = __ldcs(reinterpret_cast<const A *>(row + first + q * step));
+    return u;
+}
+template <typename T, int P>
+__device__ __forceinline__ void store_pieces(T *row, int first, int step, int F, const uint4 &u) {
+    using A = typename Access<P * (int)sizeof(T)>::type;
+    const A *piece = reinterpret_cast<const A *>(&u);
+#pragma unroll
+    for (int q = 0; q < Vec<T>::N / P; ++q)
+        if (first + q * step < F) __stcs(reinterpret_cast<A *>(row + first + q * step), piece[q]);
+}
+
 // out[c] = sum of partial[b][c] over the blocks, in a fixed order: 16 threads take every 16th block of a column.
 template <typename T>
 __global__ void __launch_bounds__(512) column_sum_kernel(const float *__restrict__ partial, int64_t blocks, int64_t F, T *out) {

@@ -49,25 +49,42 @@ __device__ __forceinline__ float row_sum(float v, float *red) {
     return (s.x + s.y) + (s.z + s.w);
 }
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void load_weight(const void *w, bool w_f32, int col, int valid, float (&f)[Vec<T>::N]) {
-    constexpr int V = Vec<T>::N;
-    if (VEC && !w_f32) {
-        unpack16<T>(__ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(w) + col)), f);
-    } else if (VEC) {
+// The weights of a thread's pieces (see load_pieces), of the rows' type or fp32.
+template <typename T, int P>
+__device__ __forceinline__ void load_weight(const void *w, bool w_f32, int first, int step, int F, float (&f)[Vec<T>::N]) {
 #pragma unroll
-        for (int i = 0; i < V; i += 4) {
-            const float4 v = __ldg(reinterpret_cast<const float4 *>(static_cast<const float *>(w) + col + i));
-            f[i] = v.x, f[i + 1] = v.y, f[i + 2] = v.z, f[i + 3] = v.w;
+    for (int q = 0; q < Vec<T>::N / P; ++q) {
+        const int c = first + q * step;
+#pragma unroll
+        for (int i = 0; i < P; ++i) f[q * P + i] = 0.0f;
+        if (c >= F) continue;
+        if (P == Vec<T>::N && !w_f32) {
+            unpack16<T>(__ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(w) + c)), f);
+        } else if (P >= 4) {
+#pragma unroll
+            for (int i = 0; i < P; i += 4) {
+                const float4 v = __ldg(reinterpret_cast<const float4 *>(static_cast<const float *>(w) + c + i));
+                f[q * P + i] = v.x, f[q * P + i + 1] = v.y, f[q * P + i + 2] = v.z, f[q * P + i + 3] = v.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+                f[q * P + i] = w_f32 ? __ldg(static_cast<const float *>(w) + c + i) : to_f32(static_cast<const T *>(w)[c + i]);
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            f[i] = i < valid ? (w_f32 ? __ldg(static_cast<const float *>(w) + col + i)
-                                      : to_f32(static_cast<const T *>(w)[col + i]))
-                             : 0.0f;
     }
 }
+
+// Where a thread's chunks of a row begin: a warp (half a warp) covers neighbouring columns.
+template <typename T, int L, int NV, int P>
+struct Columns {
+    static constexpr int V = Vec<T>::N, kLanes = L == 16 ? 16 : 32, kStep = P * kLanes;
+    int base;
+    __device__ __forceinline__ Columns()
+        : base((L == 0 ? (int)(threadIdx.x >> 5) * kLanes * V * NV : 0) + (int)(threadIdx.x & (kLanes - 1)) * P) {}
+    __device__ __forceinline__ int first(int j) const { return base + j * V * kLanes; }
+    // element i of chunk j
+    __device__ __forceinline__ int at(int j, int i) const { return first(j) + i / P * kStep + i % P; }
+};
 
 struct FwdParams {
     const void *x, *residual, *w;
@@ -80,12 +97,14 @@ struct FwdParams {
 };
 
 // NV chunks a thread and row, R rows a group of threads at once.
-template <typename T, int L, int NV, int R, bool VEC, bool FP8>
+template <typename T, int L, int NV, int R, int P, bool FP8>
 __global__ void __launch_bounds__(L > 0 ? kRowThreads : kBlockThreads) rms_norm_fwd_kernel(const FwdParams p) {
     constexpr int V = Vec<T>::N;
     __shared__ __align__(16) float red[1][32];
     if (L == 0) clear_sums(red);
-    const int lane = L > 0 ? threadIdx.x & (L - 1) : threadIdx.x, step = L > 0 ? L : blockDim.x;
+    const Columns<T, L, NV, P> cols;
+    constexpr int kStep = cols.kStep;
+    const int lane = L > 0 ? threadIdx.x & (L - 1) : threadIdx.x;
     const int64_t row0 = L > 0 ? ((int64_t)blockIdx.x * (kRowThreads / (L + !L)) + threadIdx.x / (L + !L)) * R : blockIdx.x;
     if (L == 32 && row0 >= p.rows) return;  // whole warps; half a warp stays for the other half's exchanges
     uint4 h[R][NV], res[R][NV];
@@ -93,12 +112,11 @@ __global__ void __launch_bounds__(L > 0 ? kRowThreads : kBlockThreads) rms_norm_
     for (int k = 0; k < R; ++k)
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int col = (lane + step * j) * V, valid = p.F - col;
-            const bool in = valid > 0 && ((L != 16 && R == 1) || row0 + k < p.rows);
+            const bool in = (L != 16 && R == 1) || row0 + k < p.rows;
             h[k][j] = res[k][j] = make_uint4(0, 0, 0, 0);
-            if (in) h[k][j] = load_raw<T, VEC>(static_cast<const T *>(p.x) + (row0 + k) * p.ldx + col, valid);
+            if (in) h[k][j] = load_pieces<T, P>(static_cast<const T *>(p.x) + (row0 + k) * p.ldx, cols.first(j), kStep, p.F);
             if (in && p.residual != nullptr)
-                res[k][j] = load_raw<T, VEC>(static_cast<const T *>(p.residual) + (row0 + k) * p.ldr + col, valid);
+                res[k][j] = load_pieces<T, P>(static_cast<const T *>(p.residual) + (row0 + k) * p.ldr, cols.first(j), kStep, p.F);
         }
 #pragma unroll
     for (int k = 0; k < R; ++k) {
@@ -117,8 +135,7 @@ __global__ void __launch_bounds__(L > 0 ? kRowThreads : kBlockThreads) rms_norm_
                 for (int i = 0; i < V; ++i) v[i] += r[i];
                 h[k][j] = pack16<T>(v);
                 unpack16<T>(h[k][j], v);  // the norm is of the rounded sum
-                const int col = (lane + step * j) * V, valid = p.F - col;
-                if (valid > 0 && live) store_raw<T, VEC>(static_cast<T *>(p.h) + row * p.ldh + col, valid, h[k][j]);
+                if (live) store_pieces<T, P>(static_cast<T *>(p.h) + row * p.ldh, cols.first(j), kStep, p.F, h[k][j]);
             }
 #pragma unroll
             for (int i = 0; i < V; ++i) ss = fmaf(v[i], v[i], ss);
@@ -127,41 +144,63 @@ __global__ void __launch_bounds__(L > 0 ? kRowThreads : kBlockThreads) rms_norm_
         if (lane == 0 && live && p.rstd != nullptr) p.rstd[row] = rstd;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int col = (lane + step * j) * V, valid = p.F - col;
+            const int first = cols.first(j);
             float v[V], w[V];
             unpack16<T>(h[k][j], v);
-#pragma unroll
-            for (int i = 0; i < V; ++i) w[i] = 0.0f;
-            if (valid > 0) load_weight<T, VEC>(p.w, p.w_f32 != 0, col, valid, w);
+            load_weight<T, P>(p.w, p.w_f32 != 0, first, kStep, p.F, w);
             if (!FP8) {
-                if (valid > 0 && live) {
 #pragma unroll
-                    for (int i = 0; i < V; ++i) v[i] = v[i] * rstd * w[i];
-                    store_chunk<T, VEC>(static_cast<T *>(p.y) + row * p.ldy + col, valid, v);
-                }
-            } else {
+                for (int i = 0; i < V; ++i) v[i] = v[i] * rstd * w[i];
+                if (live) store_pieces<T, P>(static_cast<T *>(p.y) + row * p.ldy, first, kStep, p.F, pack16<T>(v));
+                continue;
+            }
+            uint8_t *codes = static_cast<uint8_t *>(p.y) + row * p.ldy;
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = __fmul_rn(v[i], w[i]);
+            if (P == V) {
+                // 128 columns are 128 / V neighbouring threads: a whole or half a warp (or all of the row)
                 uint32_t m = 0;
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    v[i] = __fmul_rn(v[i], w[i]);
-                    m = max(m, abs_bits(v[i]));
-                }
-                // 128 columns are 128 / V neighbouring threads: a whole or half a warp (or all of the row)
+                for (int i = 0; i < V; ++i) m = max(m, abs_bits(v[i]));
 #pragma unroll
                 for (int off = L == 16 ? 8 : 64 / V; off > 0; off >>= 1) m = max(m, __shfl_xor_sync(kFullMask, m, off));
                 const float a = block_amax(m), f = block_factor(a);
-                if (valid > 0 && live) {
-                    // code rows are padded to 16 bytes, so a whole chunk always fits; columns from F on are zeros
+                if (first < p.F && live) {
                     uint32_t c[V / 4];
 #pragma unroll
                     for (int i = 0; i < V / 4; ++i)
                         c[i] = e4m3x4(v[4 * i] * f, v[4 * i + 1] * f, v[4 * i + 2] * f, v[4 * i + 3] * f);
-                    uint32_t *dst = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(p.y) + row * p.ldy + col);
+                    uint32_t *dst = reinterpret_cast<uint32_t *>(codes + first);
                     if (V == 8)
                         __stcs(reinterpret_cast<uint2 *>(dst), make_uint2(c[0], c[V / 4 - 1]));
                     else
                         __stcs(dst, c[0]);
-                    if ((col & 127) == 0) p.scales[(int64_t)(col >> 7) * p.lds + row] = block_scale(a) * rstd;
+                    if ((first & 127) == 0) p.scales[(int64_t)(first >> 7) * p.lds + row] = block_scale(a) * rstd;
+                }
+            } else {
+                // 128 columns are E elements of every lane
+                constexpr int E = V * cols.kLanes >= 128 ? 128 / cols.kLanes : V;
+#pragma unroll
+                for (int e = 0; e < V; e += E) {
+                    uint32_t m = 0;
+#pragma unroll
+                    for (int i = e; i < e + E; ++i) m = max(m, abs_bits(v[i]));
+#pragma unroll
+                    for (int off = cols.kLanes / 2; off > 0; off >>= 1) m = max(m, __shfl_xor_sync(kFullMask, m, off));
+                    const float a = block_amax(m), f = block_factor(a);
+#pragma unroll
+                    for (int i = e; i < e + E; i += P) {
+                        const int c = cols.at(j, i);
+                        if (c < p.F && live) {
+                            const uint32_t b = e4m3x4(v[i] * f, v[i + P - 1] * f, 0.0f, 0.0f);
+                            if (P == 2)
+                                *reinterpret_cast<uint16_t *>(codes + c) = (uint16_t)b;
+                            else
+                                codes[c] = (uint8_t)b;
+                        }
+                    }
+                    const int c0 = cols.at(j, e);
+                    if ((c0 & 127) == 0 && c0 < p.F && live) p.scales[(int64_t)(c0 >> 7) * p.lds + row] = block_scale(a) * rstd;
                 }
             }
         }
@@ -179,14 +218,16 @@ struct BwdParams {
 };
 
 // Blocks per SM that the register limit is set for, as measured: more rows on their way against registers that spill.
-template <typename T, int L, int NV, bool VEC>
+template <typename T, int L, int NV, int P>
 __global__ void __launch_bounds__(L > 0 ? kRowThreads : kBlockThreads, L > 0 ? (NV == 1 ? 4 : NV == 2 ? 3 : 2) : NV == 4 ? 1 : 2)
 rms_norm_bwd_kernel(const BwdParams p) {
     constexpr int V = Vec<T>::N;
     constexpr int kRows = L > 0 ? kRowThreads / (L + !L) : 1, kWarpRows = L == 16 ? 2 : 1;
     __shared__ __align__(16) float red[2][32];
-    __shared__ float cols[L > 0 ? kRowThreads * V : 1];
-    const int lane = L > 0 ? threadIdx.x & (L - 1) : threadIdx.x, step = L > 0 ? L : blockDim.x;
+    __shared__ float sums[L > 0 ? kRowThreads * V : 1];
+    const Columns<T, L, NV, P> cols;
+    constexpr int kStep = cols.kStep;
+    const int lane = L > 0 ? threadIdx.x & (L - 1) : threadIdx.x;
     const int slot = L > 0 ? threadIdx.x / (L + !L) : 0;
     if (L == 0) clear_sums(red);
     const float inv_f = 1.0f / (float)p.F;
@@ -204,25 +245,22 @@ rms_norm_bwd_kernel(const BwdParams p) {
         uint4 h[NV], g[NV], gh[NV];
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int col = (lane + step * j) * V, valid = p.F - col;
             h[j] = g[j] = gh[j] = make_uint4(0, 0, 0, 0);
-            if (valid > 0 && live) {
-                h[j] = load_raw<T, VEC>(static_cast<const T *>(p.h) + row * p.ldh + col, valid);
-                g[j] = load_raw<T, VEC>(static_cast<const T *>(p.gy) + row * p.ldgy + col, valid);
-                if (p.gh != nullptr) gh[j] = load_raw<T, VEC>(static_cast<const T *>(p.gh) + row * p.ldgh + col, valid);
+            if (live) {
+                const int first = cols.first(j);
+                h[j] = load_pieces<T, P>(static_cast<const T *>(p.h) + row * p.ldh, first, kStep, p.F);
+                g[j] = load_pieces<T, P>(static_cast<const T *>(p.gy) + row * p.ldgy, first, kStep, p.F);
+                if (p.gh != nullptr) gh[j] = load_pieces<T, P>(static_cast<const T *>(p.gh) + row * p.ldgh, first, kStep, p.F);
             }
         }
         const float rstd = live ? __ldg(p.rstd + row) : 0.0f;
         float s = 0.0f;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int col = (lane + step * j) * V, valid = p.F - col;
             float x[V], y[V], w[V];
             unpack16<T>(h[j], x);
             unpack16<T>(g[j], y);
-#pragma unroll
-            for (int i = 0; i < V; ++i) w[i] = 0.0f;
-            if (valid > 0) load_weight<T, VEC>(p.w, p.w_f32 != 0, col, valid, w);  // from L1: cheaper than its registers
+            load_weight<T, P>(p.w, p.w_f32 != 0, cols.first(j), kStep, p.F, w);  // from L1: cheaper than its registers
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const float hat = x[i] * rstd;
@@ -233,48 +271,44 @@ rms_norm_bwd_kernel(const BwdParams p) {
         const float minus = -rstd * row_sum<L>(s, red[turn]) * inv_f;  // two buffers: a warp may be a row ahead of another
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int col = (lane + step * j) * V, valid = p.F - col;
-            if (valid > 0 && live) {
-                float x[V], y[V], w[V], o[V];
-                unpack16<T>(h[j], x);
-                unpack16<T>(g[j], y);
-                unpack16<T>(gh[j], o);
-                load_weight<T, VEC>(p.w, p.w_f32 != 0, col, valid, w);
+            float x[V], y[V], w[V], o[V];
+            unpack16<T>(h[j], x);
+            unpack16<T>(g[j], y);
+            unpack16<T>(gh[j], o);
+            load_weight<T, P>(p.w, p.w_f32 != 0, cols.first(j), kStep, p.F, w);
 #pragma unroll
-                for (int i = 0; i < V; ++i) o[i] = fmaf(rstd, fmaf(x[i], minus, y[i] * w[i]), o[i]);
-                store_chunk<T, VEC>(static_cast<T *>(p.gx) + row * p.ldgx + col, valid, o);
-            }
+            for (int i = 0; i < V; ++i) o[i] = fmaf(rstd, fmaf(x[i], minus, y[i] * w[i]), o[i]);
+            if (live) store_pieces<T, P>(static_cast<T *>(p.gx) + row * p.ldgx, cols.first(j), kStep, p.F, pack16<T>(o));
         }
     }
     float *out = p.partial + (int64_t)blockIdx.x * p.F;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const int col = (lane + step * j) * V;
         if (L > 0) {  // the block's rows add up in their order
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < V; ++i) cols[(slot * V + i) * L + lane] = dw[j][i];
+            for (int i = 0; i < V; ++i) sums[(slot * V + i) * L + lane] = dw[j][i];
             __syncthreads();
             for (int e = threadIdx.x; e < L * V; e += kRowThreads) {
                 float s = 0.0f;
 #pragma unroll
-                for (int r = 0; r < kRows; ++r) s += cols[r * L * V + e];
-                const int c = (e % (L + !L) + L * j) * V + e / (L + !L);
+                for (int r = 0; r < kRows; ++r) s += sums[r * L * V + e];
+                const int i = e / (L + !L), c = (e % (L + !L)) * P + j * V * L + i / P * kStep + i % P;
                 if (c < p.F) out[c] = s;
             }
         } else {
 #pragma unroll
             for (int i = 0; i < V; ++i)
-                if (col + i < p.F) out[col + i] = dw[j][i];
+                if (cols.at(j, i) < p.F) out[cols.at(j, i)] = dw[j][i];
         }
     }
 }
 
 // The block-per-row form on 16-byte rows: the next row's chunks are copied to shared memory (cp.async, every thread its
 // own, so that no barrier is needed for them) while the block works on this one.  Without, a block's three loads, its
-// reduction and its store follow one another: 78 us instead of MEASURED at 8191 x 5000 bf16.
+// reduction and its store follow one another: 16384 x 4096 bf16 in 116 us instead of 104.
 template <typename T, int NV>
-__global__ void __launch_bounds__(kBlockThreads, NV == 4 ? 1 : 2) rms_norm_bwd_ahead_kernel(const BwdParams p) {
+__global__ void __launch_bounds__(kBlockThreads) rms_norm_bwd_ahead_kernel(const BwdParams p) {
     constexpr int V = Vec<T>::N;
     extern __shared__ __align__(16) uint4 ahead[];  // [2][3 * NV][threads]
     __shared__ __align__(16) float red[2][32];
@@ -317,7 +351,7 @@ __global__ void __launch_bounds__(kBlockThreads, NV == 4 ? 1 : 2) rms_norm_bwd_a
                 float x[V], y[V], w[V];
                 unpack16<T>(*slot(turn, 3 * j), x);
                 unpack16<T>(*slot(turn, 3 * j + 1), y);
-                load_weight<T, true>(p.w, p.w_f32 != 0, col, V, w);
+                load_weight<T, V>(p.w, p.w_f32 != 0, col, V, p.F, w);
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     const float hat = x[i] * rstd;
@@ -337,7 +371,7 @@ __global__ void __launch_bounds__(kBlockThreads, NV == 4 ? 1 : 2) rms_norm_bwd_a
 #pragma unroll
                 for (int i = 0; i < V; ++i) o[i] = 0.0f;
                 if (p.gh != nullptr) unpack16<T>(*slot(turn, 3 * j + 2), o);
-                load_weight<T, true>(p.w, p.w_f32 != 0, col, V, w);
+                load_weight<T, V>(p.w, p.w_f32 != 0, col, V, p.F, w);
 #pragma unroll
                 for (int i = 0; i < V; ++i) o[i] = fmaf(rstd, fmaf(x[i], minus, y[i] * w[i]), o[i]);
                 store_chunk<T, true>(static_cast<T *>(p.gx) + row * p.ldgx + col, V, o);
@@ -376,7 +410,7 @@ __global__ void __launch_bounds__(kWideThreads) rms_norm_bwd_wide_kernel(const B
             float hat[V], g[V], w[V];
             load_chunk<T, VEC>(h + col, valid, hat);
             load_chunk<T, VEC>(gy + col, valid, g);
-            load_weight<T, VEC>(p.w, p.w_f32 != 0, col, valid, w);
+            load_weight<T, VEC ? V : 1>(p.w, p.w_f32 != 0, col, 1, p.F, w);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 hat[i] *= rstd;
@@ -390,7 +424,7 @@ __global__ void __launch_bounds__(kWideThreads) rms_norm_bwd_wide_kernel(const B
             float hat[V], g[V], w[V], gh[V];
             load_chunk<T, VEC>(h + col, valid, hat);
             load_chunk<T, VEC>(gy + col, valid, g);
-            load_weight<T, VEC>(p.w, p.w_f32 != 0, col, valid, w);
+            load_weight<T, VEC ? V : 1>(p.w, p.w_f32 != 0, col, 1, p.F, w);
 #pragma unroll
             for (int i = 0; i < V; ++i) gh[i] = 0.0f;
             if (p.gh != nullptr) load_chunk<T, VEC>(static_cast<const T *>(p.gh) + row * p.ldgh + col, valid, gh);
@@ -449,12 +483,12 @@ int by_type(int type, F32 a, BF16 b, F16 c) {
     return type == kTypeF32 ? a() : type == kTypeBf16 ? b() : c();
 }
 
-template <typename T, bool VEC, bool FP8>
+template <typename T, int P, bool FP8>
 int launch_fwd(const FwdParams &p, cudaStream_t st) {
     const Spread s = spread_of(p.F, (int)sizeof(T));
 #define RMS_WARP(L, NV, R) \
-    rms_norm_fwd_kernel<T, L, NV, R, VEC, FP8><<<(unsigned)div_up(p.rows, kRowThreads / L * R), kRowThreads, 0, st>>>(p)
-#define RMS_BLOCK(NV, THREADS) rms_norm_fwd_kernel<T, 0, NV, 1, VEC, FP8><<<(unsigned)p.rows, THREADS, 0, st>>>(p)
+    rms_norm_fwd_kernel<T, L, NV, R, P, FP8><<<(unsigned)div_up(p.rows, kRowThreads / L * R), kRowThreads, 0, st>>>(p)
+#define RMS_BLOCK(NV, THREADS) rms_norm_fwd_kernel<T, 0, NV, 1, P, FP8><<<(unsigned)p.rows, THREADS, 0, st>>>(p)
     if (s.lanes == 16) RMS_WARP(16, 1, 2);
     else if (s.lanes == 32 && s.nv == 1) RMS_WARP(32, 1, 2);
     else if (s.lanes == 32 && s.nv == 2) RMS_WARP(32, 2, 1);
@@ -469,14 +503,15 @@ int launch_fwd(const FwdParams &p, cudaStream_t st) {
 }
 
 // `blocks`: at most this many; becomes the number of blocks (rows of partial sums).
-template <typename T, bool VEC>
+template <typename T, int P>
 int launch_bwd(const BwdParams &p, int &blocks, cudaStream_t st) {
+    constexpr bool VEC = P == Vec<T>::N;
     const Spread s = spread_of(p.F, (int)sizeof(T));
 #define RMS_LAUNCH(L, NV)                                                                    \
     do {                                                                                     \
-        const int wave = kNumSMs * resident<rms_norm_bwd_kernel<T, L, NV, VEC>>(s.threads);  \
+        const int wave = kNumSMs * resident<rms_norm_bwd_kernel<T, L, NV, P>>(s.threads);  \
         if (blocks > wave) blocks = wave;                                                    \
-        rms_norm_bwd_kernel<T, L, NV, VEC><<<blocks, s.threads, 0, st>>>(p);                 \
+        rms_norm_bwd_kernel<T, L, NV, P><<<blocks, s.threads, 0, st>>>(p);                 \
     } while (0)
 #define RMS_AHEAD(NV)                                                                                            \
     do {                                                                                                         \
@@ -522,8 +557,16 @@ int launch_dw(const float *partial, int blocks, int F, void *dw, cudaStream_t st
     return check_launch("column_sum_kernel");
 }
 
-// 16-byte accesses of rows at p with a stride of ld elements
-bool vec_rows(const void *p, int64_t ld, int size) { return aligned16(p) && (ld * size) % 16 == 0; }
+// How many neighbouring elements all of a call's rows allow one access for.
+struct Together {
+    int F, size;
+    uintptr_t bits = 0;  // of the addresses and strides in bytes, scaled to the rows' element size
+    Together(int F, int size) : F(F), size(size) {}
+    void add(const void *p, int64_t ld, int each) {
+        bits |= reinterpret_cast<uintptr_t>(p) * size / each | (uintptr_t)(ld * size);
+    }
+    bool allow(int n) const { return F % n == 0 && bits % (uintptr_t)(n * size) == 0; }
+};
 
 int check_common(const char *what, int type, int w_type, int64_t rows, int F) {
     if (type_size(type) == 0) return fail(GNNAGG_ERR_ARG, "%s: unknown element type %d", what, type);
@@ -550,14 +593,24 @@ int fwd(const char *what, bool fp8, const void *x, int64_t ldx, const void *resi
     if (fp8 && (!aligned16(y) || ldy % 16 != 0))
         return fail(GNNAGG_ERR_UNSUPPORTED, "%s: code rows start on 16 bytes", what);
     const int size = type_size(type);
-    bool vec = F % (16 / size) == 0 && vec_rows(x, ldx, size) && aligned16(w) && (fp8 || vec_rows(y, ldy, size));
-    if (residual != nullptr) vec = vec && vec_rows(residual, ldr, size) && vec_rows(h, ldh, size);
+    Together rows_of(F, size);
+    rows_of.add(x, ldx, size);
+    rows_of.add(w, 0, w_type == kTypeF32 ? 4 : size);
+    if (!fp8) rows_of.add(y, ldy, size);
+    if (residual != nullptr) {
+        rows_of.add(residual, ldr, size);
+        rows_of.add(h, ldh, size);
+    }
+    const bool vec = rows_of.allow(16 / size), two = size == 2 && rows_of.allow(2);
     const FwdParams p{x, residual, w, h, y, scales, rstd, ldx, ldr, ldh, ldy, lds, rows, F, w_type == kTypeF32, eps};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-#define RMS_TYPE(T)                                                                                       \
-    [&] {                                                                                                 \
-        return fp8 ? (vec ? launch_fwd<T, true, true>(p, st) : launch_fwd<T, false, true>(p, st))         \
-                   : (vec ? launch_fwd<T, true, false>(p, st) : launch_fwd<T, false, false>(p, st));      \
+#define RMS_TYPE(T)                                                                                        \
+    [&] {                                                                                                  \
+        constexpr int V = Vec<T>::N, Two = sizeof(T) == 2 ? 2 : 1;                                         \
+        return fp8 ? (vec ? launch_fwd<T, V, true>(p, st) : two ? launch_fwd<T, Two, true>(p, st)          \
+                                                                : launch_fwd<T, 1, true>(p, st))           \
+                   : (vec ? launch_fwd<T, V, false>(p, st) : two ? launch_fwd<T, Two, false>(p, st)        \
+                                                                 : launch_fwd<T, 1, false>(p, st));        \
     }
     return by_type(type, RMS_TYPE(float), RMS_TYPE(__nv_bfloat16), RMS_TYPE(__half));
 #undef RMS_TYPE
@@ -604,10 +657,20 @@ extern "C" int gnnagg_rms_norm_bwd(const void *gy, int64_t ldgy, const void *gh,
         return fail(GNNAGG_ERR_SCRATCH, "rms_norm_bwd: partial-sum scratch too small");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (rows > 0) {
-        const bool vec = F % (16 / size) == 0 && vec_rows(gy, ldgy, size) && vec_rows(h, ldh, size) &&
-                         vec_rows(gx, ldgx, size) && (gh == nullptr || vec_rows(gh, ldgh, size)) && aligned16(w);
+        Together rows_of(F, size);
+        rows_of.add(gy, ldgy, size);
+        rows_of.add(h, ldh, size);
+        rows_of.add(gx, ldgx, size);
+        if (gh != nullptr) rows_of.add(gh, ldgh, size);
+        rows_of.add(w, 0, w_type == kTypeF32 ? 4 : size);
+        const bool vec = rows_of.allow(16 / size), two = size == 2 && rows_of.allow(2);
         const BwdParams p{gy, gh, h, w, rstd, gx, partial, ldgy, ldgh, ldh, ldgx, rows, F, w_type == kTypeF32};
-#define RMS_TYPE(T) [&] { return vec ? launch_bwd<T, true>(p, blocks, st) : launch_bwd<T, false>(p, blocks, st); }
+#define RMS_TYPE(T)                                                                                  \
+    [&] {                                                                                            \
+        return vec   ? launch_bwd<T, Vec<T>::N>(p, blocks, st)                                       \
+               : two ? launch_bwd<T, sizeof(T) == 2 ? 2 : 1>(p, blocks, st)                          \
+                     : launch_bwd<T, 1>(p, blocks, st);                                              \
+    }
         rc = by_type(type, RMS_TYPE(float), RMS_TYPE(__nv_bfloat16), RMS_TYPE(__half));
 #undef RMS_TYPE
         if (rc != GNNAGG_OK) return rc;
