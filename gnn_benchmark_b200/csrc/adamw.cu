@@ -3,12 +3,14 @@
 //     m = b1 m + (1 - b1) g,   v = b2 v + (1 - b2) g^2
 //     p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
-// A pure stream: 28 bytes an element with 32-bit moments and fp32 parameters, 16 with 8-bit ones, so the kernel
-// is bound by memory, and for a small model by the launch.  The table of tensors (pointers, sizes, the prefix of
-// their block counts) travels in the launch's own parameters: no copy to the device, nothing to keep alive, and a
-// captured graph owns its table.  A warp takes 256 consecutive elements of one tensor: lane l holds elements
-// 4 l .. 4 l + 3 and 128 + 4 l .. 128 + 4 l + 3, so every access of a warp is contiguous, and the block of an
-// 8-bit moment is the warp's own.
+// A pure stream: 28 bytes an element with 32-bit moments and fp32 parameters, 16 with 8-bit ones (22 and 10 for 16-bit
+// parameters), so the kernel is bound by memory, and for a small model by the launch.  90 M elements take 371 us at
+// 6.8 TB/s and 217 us at 6.7 TB/s (293 at 6.8, and 209 at 4.3: at 10 bytes an element its instructions bound it).
+//
+// The table of tensors (pointers, sizes, the prefix of their block counts) travels in the launch's own parameters: no
+// copy to the device, nothing to keep alive, and a captured graph owns its table.  A warp takes 256 consecutive
+// elements of one tensor: lane l holds elements 4 l .. 4 l + 3 and 128 + 4 l .. 128 + 4 l + 3, so every access of a
+// warp is contiguous, and the block of an 8-bit moment is the warp's own.
 //
 // 8-bit moments: m and sqrt(v) are held as e4m3 codes with a scale per 256 elements.  The square root halves the
 // exponent range that v needs; the code of sqrt(v) is at least the type's smallest value where v > 0, so that no
@@ -48,21 +50,65 @@ struct Table {
 constexpr int kSmallCap = 16, kMidCap = 60, kLargeCap = 500;
 static_assert(sizeof(Table<kLargeCap>) <= 32764, "kernel parameters");
 
+// Four elements as they lie in memory, those behind the end as zeros; converted after the last load, in pairs.  With
+// the conversion inside the branch below, a 16-bit type's loads wait for one another: 90 M bf16 parameters took 352 us
+// (274 with 8-bit moments) instead of 293 (209).
 template <typename T>
-__device__ __forceinline__ void load4(const T *p, int64_t at, int64_t n, bool vec, float (&f)[4]) {
+struct Raw4 {
+    uint32_t w[sizeof(T)];
+};
+template <typename T>
+__device__ __forceinline__ Raw4<T> load4(const T *p, int64_t at, int64_t n, bool vec) {
+    Raw4<T> r;
     if (vec && at + 4 <= n) {
         if (sizeof(T) == 4) {
-            const float4 u = __ldcs(reinterpret_cast<const float4 *>(p + at));
-            f[0] = u.x, f[1] = u.y, f[2] = u.z, f[3] = u.w;
+            const uint4 u = __ldcs(reinterpret_cast<const uint4 *>(p + at));
+            r.w[0] = u.x, r.w[1] = u.y, r.w[2 % sizeof(T)] = u.z, r.w[3 % sizeof(T)] = u.w;
         } else {
             const uint2 u = __ldcs(reinterpret_cast<const uint2 *>(p + at));
-            const T *e = reinterpret_cast<const T *>(&u);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) f[i] = to_f32(e[i]);
+            r.w[0] = u.x, r.w[1] = u.y;
         }
+    } else if (sizeof(T) == 4) {
+        const uint32_t *q = reinterpret_cast<const uint32_t *>(p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r.w[i % sizeof(T)] = at + i < n ? q[at + i] : 0;
+    } else {
+        const uint16_t *q = reinterpret_cast<const uint16_t *>(p);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t a = at + 2 * i < n ? q[at + 2 * i] : 0, b = at + 2 * i + 1 < n ? q[at + 2 * i + 1] : 0;
+            r.w[i] = a | (b << 16);
+        }
+    }
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void put(Raw4<float> &to, const Raw4<T> &from) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T); ++i) to.w[i] = from.w[i];
+}
+template <typename T>
+__device__ __forceinline__ Raw4<T> first(const Raw4<float> &from) {
+    Raw4<T> r;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T); ++i) r.w[i] = from.w[i];
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void convert4(const Raw4<T> &r, float (&f)[4]) {
+    if (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(r.w[i % sizeof(T)]);
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = at + i < n ? to_f32(p[at + i]) : 0.0f;
+        for (int i = 0; i < 2; ++i) {
+            if (std::is_same<T, __nv_bfloat16>::value) {  // the upper half of an fp32
+                f[2 * i] = __uint_as_float(r.w[i] << 16), f[2 * i + 1] = __uint_as_float(r.w[i] & 0xFFFF0000u);
+            } else {
+                const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&r.w[i]));
+                f[2 * i] = v.x, f[2 * i + 1] = v.y;
+            }
+        }
     }
 }
 template <typename T>
@@ -71,11 +117,18 @@ __device__ __forceinline__ void store4(T *p, int64_t at, int64_t n, bool vec, co
         if (sizeof(T) == 4) {
             __stcs(reinterpret_cast<float4 *>(p + at), make_float4(f[0], f[1], f[2], f[3]));
         } else {
-            uint2 u;
-            T *e = reinterpret_cast<T *>(&u);
+            uint32_t u[2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) e[i] = from_f32<T>(f[i]);
-            __stcs(reinterpret_cast<uint2 *>(p + at), u);
+            for (int i = 0; i < 2; ++i) {
+                if (std::is_same<T, __nv_bfloat16>::value) {
+                    const __nv_bfloat162 b = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+                    u[i] = *reinterpret_cast<const uint32_t *>(&b);
+                } else {
+                    const __half2 b = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+                    u[i] = *reinterpret_cast<const uint32_t *>(&b);
+                }
+            }
+            __stcs(reinterpret_cast<uint2 *>(p + at), make_uint2(u[0], u[1]));
         }
     } else {
 #pragma unroll
@@ -129,30 +182,41 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
     T *p = static_cast<T *>(e.p);
     const T *g = static_cast<const T *>(e.g);
     const int64_t at[2] = {base + 4 * lane, base + 128 + 4 * lane};
-    float w[2][4], gr[2][4], m[2][4], v[2][4];
+    Raw4<T> raw_g[2];
+    Raw4<float> raw_w[2], raw_m[2], raw_v[2];  // raw_w: the master copy, or in its first words the parameter
     uint32_t mc[2], vc[2];
     float2 sc = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         if (e.master != nullptr)
-            load4<float>(e.master, at[h], n, vec, w[h]);
+            raw_w[h] = load4<float>(e.master, at[h], n, vec);
         else
-            load4<T>(p, at[h], n, vec, w[h]);
-        load4<T>(g, at[h], n, vec, gr[h]);
+            put(raw_w[h], load4<T>(p, at[h], n, vec));
+        raw_g[h] = load4<T>(g, at[h], n, vec);
         if (EIGHT) {
             mc[h] = load_codes(static_cast<const uint8_t *>(e.m), at[h], n, vec);
             vc[h] = load_codes(static_cast<const uint8_t *>(e.v), at[h], n, vec);
         } else {
-            load4<float>(static_cast<const float *>(e.m), at[h], n, vec, m[h]);
-            load4<float>(static_cast<const float *>(e.v), at[h], n, vec, v[h]);
+            raw_m[h] = load4<float>(static_cast<const float *>(e.m), at[h], n, vec);
+            raw_v[h] = load4<float>(static_cast<const float *>(e.v), at[h], n, vec);
         }
     }
     if (EIGHT) sc = *reinterpret_cast<const float2 *>(e.scales + 2 * (base / kWarpElems));
     const Scalars s = t.device_scalars != nullptr ? *t.device_scalars : t.s;
     uint32_t top_m = 0, top_r = 0;
+    float w[2][4], m[2][4], v[2][4];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        if (EIGHT) {
+        float gr[4];
+        if (e.master != nullptr)
+            convert4(raw_w[h], w[h]);
+        else
+            convert4(first<T>(raw_w[h]), w[h]);
+        convert4(raw_g[h], gr);
+        if (!EIGHT) {
+            convert4(raw_m[h], m[h]);
+            convert4(raw_v[h], v[h]);
+        } else {
             const float4 a = from_e4m3x4(mc[h]), b = from_e4m3x4(vc[h]);
             m[h][0] = __fmul_rn(a.x, sc.x), m[h][1] = __fmul_rn(a.y, sc.x);
             m[h][2] = __fmul_rn(a.z, sc.x), m[h][3] = __fmul_rn(a.w, sc.x);
@@ -164,7 +228,7 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             // each step rounded on its own: an 8-bit moment's code then depends on the formula alone
-            const float x = gr[h][i];
+            const float x = gr[i];
             m[h][i] = __fadd_rn(__fmul_rn(m[h][i], s.b1), __fmul_rn(x, s.one_minus_b1));
             v[h][i] = __fadd_rn(__fmul_rn(v[h][i], s.b2), __fmul_rn(__fmul_rn(x, x), s.one_minus_b2));
             const float r = EIGHT ? __fsqrt_rn(v[h][i]) : sqrt_approx(v[h][i]);
