@@ -62,6 +62,11 @@ Tensor empty_scales(int64_t rows, int64_t cols, const Tensor &like) {
 bool wants_grad(const Tensor &t) { return t.requires_grad(); }
 bool wants_grad(const std::optional<Tensor> &t) { return t.has_value() && t->requires_grad(); }
 
+// What torch's own in-place operators leave behind: a graph that kept the old values then raises in its backward.
+void written(const Tensor &t) {
+    if (!t.is_inference()) torch::autograd::impl::bump_version(t);
+}
+
 // ------------------------------------------------------------------------------------------ root-mean-square norm
 
 void check_rms(const char *what, const Tensor &x, const Tensor &w, const std::optional<Tensor> &res) {
@@ -250,6 +255,7 @@ Tensor matmul_fp8(const Tensor &a, const Tensor &sa, const Tensor &b, const Tens
                             bias.has_value() ? type_of(*bias) : 0, accumulate ? 1 : 0, out.data_ptr(), ldc, type_of(out),
                             need > 0 ? ws.data_ptr() : nullptr, need, stream_of(a)),
           "fp8_matmul");
+    if (out_.has_value()) written(out);
     return out;
 }
 
@@ -373,6 +379,13 @@ void adamw_step(const std::vector<Tensor> &params, const std::vector<Tensor> &gr
                             weight_decay, step, device_scalars.has_value() ? device_scalars->data_ptr() : nullptr,
                             stream_of(params[0])),
           "adamw_step");
+    for (size_t i = 0; i < count; ++i) {
+        written(params[i]);
+        written(exp_avgs[i]);
+        written(exp_avg_sqs[i]);
+        if (scales.has_value()) written((*scales)[i]);
+        if (masters.has_value() && (*masters)[i].has_value()) written(*(*masters)[i]);
+    }
 }
 
 }  // namespace

@@ -283,3 +283,23 @@ def test_gpu_refusals():
                 lambda: optim.adamw_step([t.cpu() for t in p], g, m, v, **kw)):
         with pytest.raises(RuntimeError):
             bad()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_graph_of_the_old_values_raises(bits):
+    """A step is a write in place: a graph that kept the parameter from before must not go on with the new one."""
+    from gnn_benchmark_b200 import optim
+
+    p = torch.nn.Parameter(torch.randn(300, device="cuda"))
+    opt = optim.AdamW([p], state_bits=bits)
+    loss = p.square().sum()
+    p.grad = torch.ones_like(p)
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    before = [t._version for t in opt.state[p].values() if isinstance(t, torch.Tensor)]
+    opt.step()
+    assert all(t._version > b for t, b in zip([t for t in opt.state[p].values() if isinstance(t, torch.Tensor)], before))
+    with torch.inference_mode():  # tensors that keep no version
+        p, g, m, v = _tensors([10], torch.float32, 3)
+        optim.adamw_step(p, g, m, v, step=1, lr=1e-3)

@@ -304,3 +304,14 @@ def test_gpu_refusals():
                 lambda: dense.quantize_fp8(out, (1, 64)), lambda: dense.linear_fp8(out, out[:, :39])):
         with pytest.raises(RuntimeError):
             bad()
+
+
+def test_graph_of_an_output_written_over_raises():
+    from gnn_benchmark_b200 import dense
+
+    a, b = dense.quantize_fp8(torch.randn(30, 256, device="cuda")), dense.quantize_fp8(torch.randn(40, 256, device="cuda"))
+    leaf, out = torch.ones(30, 40, device="cuda", requires_grad=True), torch.ones(30, 40, device="cuda")
+    loss = (leaf * out).sum()
+    dense.matmul_fp8(*a, *b, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
