@@ -62,6 +62,25 @@ Tensor empty_scales(int64_t rows, int64_t cols, const Tensor &like) {
 bool wants_grad(const Tensor &t) { return t.requires_grad(); }
 bool wants_grad(const std::optional<Tensor> &t) { return t.has_value() && t->requires_grad(); }
 
+// A captured backward may not reach the default stream, on which the gradients of a leaf are added up when a graph that
+// was made there still holds that leaf: the process would end inside the capture, so the node refuses before.
+void check_capture(const char *what, const Tensor &t) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(static_cast<cudaStream_t>(stream_of(t)), &status) != cudaSuccess ||
+        status == cudaStreamCaptureStatusNone)
+        return;
+    const auto node = torch::autograd::get_current_node();
+    if (!node) return;
+    const c10::Stream other = c10::cuda::getDefaultCUDAStream(t.get_device()).unwrap();
+    for (const auto &edge : node->next_edges()) {
+        if (!edge.function || edge.function->num_outputs() != 0) continue;  // only a leaf's node leads nowhere
+        const auto stream = edge.function->stream();
+        TORCH_CHECK(!stream.has_value() || *stream != other, what,
+                    ": captured backward of a leaf that a graph made on the default stream still holds (delete what that "
+                    "graph computed, its loss for example, before the capture, or compute it on a side stream)");
+    }
+}
+
 // What torch's own in-place operators leave behind: a graph that kept the old values then raises in its backward.
 void written(const Tensor &t) {
     if (!t.is_inference()) torch::autograd::impl::bump_version(t);
@@ -119,6 +138,8 @@ struct RMSNorm : torch::autograd::Function<RMSNorm> {
     }
     static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
         TORCH_CHECK(!at::GradMode::is_enabled(), "rms_norm has no second derivative");
+        for (const Tensor &g : grads)
+            if (g.defined()) check_capture("rms_norm", g);
         const variable_list saved = ctx->get_saved_variables();
         const Tensor &h = saved[0], &w = saved[1], &rstd = saved[2];
         const bool residual = ctx->saved_data["residual"].toBool();
@@ -228,6 +249,8 @@ Tensor matmul_fp8(const Tensor &a, const Tensor &sa, const Tensor &b, const Tens
     const Operand oa = operand("a", a, sa, a), ob = operand("b", b, sb, a);
     const int64_t m = a.size(0), k = a.size(1), n = b.size(0);
     TORCH_CHECK(b.size(1) == k, "matmul_fp8: shape mismatch a=", a.sizes(), " b=", b.sizes());
+    TORCH_CHECK(!at::GradMode::is_enabled() || !(wants_grad(sa) || wants_grad(sb) || wants_grad(bias) || wants_grad(out_)),
+                "matmul_fp8 has no gradient: call it under torch.no_grad(), or use linear_fp8");
     TORCH_CHECK(!bias.has_value() || (type_of(*bias) >= 0 && bias->dim() == 1 && bias->size(0) == n && bias->is_contiguous() &&
                                       bias->device() == a.device()),
                 "matmul_fp8: bias must be a contiguous float32, bfloat16 or float16 vector of N elements on the operands' device");
@@ -289,6 +312,7 @@ struct LinearFP8 : torch::autograd::Function<LinearFP8> {
     }
     static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
         TORCH_CHECK(!at::GradMode::is_enabled(), "linear_fp8 has no second derivative");
+        check_capture("linear_fp8", grads[0]);
         const Tensor kept = ctx->get_saved_variables()[0], g = rows_of(grads[0]);
         const c10::cuda::CUDAGuard guard(g.device());
         const int64_t m = g.size(0), n = g.size(1), k = ctx->saved_data["k"].toInt();
@@ -349,10 +373,20 @@ void adamw_step(const std::vector<Tensor> &params, const std::vector<Tensor> &gr
     TORCH_CHECK(device_scalars.has_value() || step >= 1, "adamw_step: the first step is 1");
     if (count == 0) return;
     require_cuda(params[0]);
+    TORCH_CHECK(!device_scalars.has_value() ||
+                    (device_scalars->scalar_type() == at::kByte && device_scalars->is_contiguous() &&
+                     (size_t)device_scalars->numel() == gnnagg_adamw_scalars_bytes() &&
+                     reinterpret_cast<uintptr_t>(device_scalars->data_ptr()) % 4 == 0 &&
+                     device_scalars->device() == params[0].device()),
+                "adamw_step: device_scalars must be the ", gnnagg_adamw_scalars_bytes(),
+                " bytes that AdamW keeps, on the parameters' device");
     const at::ScalarType type = params[0].scalar_type(), state = scales.has_value() ? at::kFloat8_e4m3fn : at::kFloat;
     TORCH_CHECK(type_of(type) >= 0, "adamw_step: parameters must be float32, bfloat16 or float16, not ", type);
     check_list("parameter", params, params, type, 1, 1);
     check_list("gradient", grads, params, type, 1, 1);
+    for (size_t i = 0; i < count; ++i)
+        TORCH_CHECK(grads[i].sizes() == params[i].sizes(), "adamw_step: gradient ", i, " has the shape ", grads[i].sizes(),
+                    ", its parameter ", params[i].sizes());
     check_list("exp_avg", exp_avgs, params, state, 1, 1);
     check_list("exp_avg_sq", exp_avg_sqs, params, state, 1, 1);
     if (scales.has_value()) check_list("scales", *scales, params, at::kFloat, 256, 2);

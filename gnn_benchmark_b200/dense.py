@@ -322,7 +322,8 @@ def quantize_fp8(x: torch.Tensor, block=(1, 128), transpose: bool = False):
     (1, 128) elements, shape (rows, ceil(cols / 128)), or of (128, 128), shape (ceil(rows / 128), ceil(cols / 128)).
     An element's value is code * scale.  scale = a * (1 / 448) with a the block's largest magnitude (at least 2^-96),
     code = e4m3(x * (448 * (1 / a))).  transpose=True gives the codes and scales of x.T without forming it.  A block
-    that holds a NaN or an infinity reads back as NaN."""
+    that holds a NaN or an infinity reads back as NaN.  Nothing is differentiated through the rounding: the result is
+    detached from x."""
     if tuple(block) not in ((1, 128), (128, 128)):
         raise RuntimeError(f"quantize_fp8: block must be (1, 128) or (128, 128), not {block}")
     return tuple(_lib.ops().quantize_fp8(x, block[0], not transpose, transpose))
@@ -334,7 +335,8 @@ def matmul_fp8(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scale
     """out (M, N) (+)= (a * a_scales) @ (b * b_scales).T (+ bias): a (M, K) and b (N, K) float8_e4m3fn with float32
     scales for each block of 128 along K, one per row, (rows, ceil(K / 128)), or per 128 rows.  out_dtype float32,
     bfloat16 or float16 (out's type when out is given); bias (N,) of one of these; accumulate needs a float32 out.
-    Not differentiable."""
+    out may be a view with contiguous rows; it overlaps no operand.  Not differentiable: with gradients enabled, a bias
+    or out that requires one is refused."""
     out = _lib.ops().matmul_fp8(a, a_scales, b, b_scales, bias, out, out_dtype, accumulate)
     _fp8_devices.add(out.get_device())
     return out

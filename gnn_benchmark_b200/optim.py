@@ -60,8 +60,18 @@ class AdamW(torch.optim.Optimizer):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       master_weights=master_weights, capturable=capturable))
 
+    def add_param_group(self, param_group) -> None:
+        super().add_param_group(param_group)
+        params = self.param_groups[-1]["params"]
+        if len({id(p) for p in params}) != len(params):  # two updates of one tensor in one launch would race
+            self.param_groups.pop()
+            raise ValueError("AdamW: a parameter is listed twice in a group")
+
     def load_state_dict(self, state_dict) -> None:
         """As torch's, but the moments keep the types they were saved in (torch would cast them to the parameter's)."""
+        for group in state_dict["param_groups"]:
+            if not {"state_bits", "master_weights", "capturable"} <= group.keys():
+                raise ValueError("AdamW: the state dict is another optimiser's")
         super().load_state_dict(state_dict)
         saved = state_dict["state"]
         for mine, theirs in zip(self.param_groups, state_dict["param_groups"]):
@@ -131,6 +141,8 @@ class AdamW(torch.optim.Optimizer):
     def _tick(group, device, step):
         """Counts a step on the device and returns its scalars."""
         lib, lr, (b1, b2) = _lib.lib(), group["lr"], group["betas"]
+        if isinstance(lr, torch.Tensor) and lr.device != device:
+            raise RuntimeError(f"AdamW: lr is on {lr.device}, parameters on {device}")
         lr_ptr, host_lr = (lr.data_ptr(), 0.0) if isinstance(lr, torch.Tensor) else (0, float(lr))
         scalars = torch.empty(lib.gnnagg_adamw_scalars_bytes(), dtype=torch.uint8, device=device)
         with _lib.device_of(scalars):

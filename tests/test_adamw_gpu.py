@@ -303,3 +303,18 @@ def test_graph_of_the_old_values_raises(bits):
     with torch.inference_mode():  # tensors that keep no version
         p, g, m, v = _tensors([10], torch.float32, 3)
         optim.adamw_step(p, g, m, v, step=1, lr=1e-3)
+
+
+def test_more_refusals():
+    from gnn_benchmark_b200 import optim
+
+    p, g, m, v = _tensors([12], torch.float32, 1)
+    size = 32  # eight floats
+    for scalars in (torch.zeros(size, dtype=torch.uint8), torch.zeros(size - 4, dtype=torch.uint8, device="cuda"),
+                    torch.zeros(size // 4, device="cuda"), torch.zeros(2 * size, dtype=torch.uint8, device="cuda")[::2],
+                    torch.zeros(size + 1, dtype=torch.uint8, device="cuda")[1:]):
+        with pytest.raises(RuntimeError, match="device_scalars"):
+            optim.adamw_step(p, g, m, v, step=1, lr=1e-3, device_scalars=scalars)
+    square = [p[0].view(3, 4)]
+    with pytest.raises(RuntimeError, match="shape"):  # a transposed gradient has as many elements
+        optim.adamw_step(square, [g[0].view(4, 3)], m, v, step=1, lr=1e-3)

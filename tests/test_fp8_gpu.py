@@ -315,3 +315,16 @@ def test_graph_of_an_output_written_over_raises():
     dense.matmul_fp8(*a, *b, out=out)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+def test_product_refuses_to_drop_a_gradient():
+    from gnn_benchmark_b200 import dense
+
+    a, b = dense.quantize_fp8(torch.randn(30, 256, device="cuda")), dense.quantize_fp8(torch.randn(40, 256, device="cuda"))
+    bias = torch.zeros(40, device="cuda", requires_grad=True)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        dense.matmul_fp8(*a, *b, bias=bias)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        dense.matmul_fp8(*a, *b, out=torch.zeros(30, 40, device="cuda", requires_grad=True))
+    with torch.no_grad():
+        assert torch.equal(dense.matmul_fp8(*a, *b, bias=bias), dense.matmul_fp8(*a, *b))

@@ -150,3 +150,50 @@ def test_training_entry(cuda_lib, monkeypatch, name):
     assert all(l == l and abs(l) < 100 for l in losses)
     assert all(not torch.equal(a, p) and torch.isfinite(p).all() for a, p in zip(old, model.parameters()))
     assert all(s["exp_avg"].dtype == torch.float8_e4m3fn for s in opt.state.values())
+
+
+def test_captured_step_next_to_an_eager_graph():
+    """A step captured while an eager graph of the same leaves lives is refused; without one it is captured and its
+    replays go on from each other's parameters, as eager steps do."""
+    from gnn_benchmark_b200 import dense, norm, optim
+
+    torch.manual_seed(0)
+    x = torch.randn(200, 256, device="cuda")
+    start = [torch.rand(256, device="cuda") + 0.5, torch.randn(128, 256, device="cuda") / 16, torch.zeros(128, device="cuda")]
+
+    def fresh():
+        leaves = [torch.nn.Parameter(t.clone()) for t in start]
+        return leaves, optim.AdamW(leaves, lr=1e-2, capturable=True)
+
+    def loss_of(leaves):
+        return dense.linear_fp8(norm.rms_norm(x, leaves[0]), leaves[1], leaves[2]).square().mean()
+
+    def step(leaves, opt):
+        for p in leaves:
+            p.grad = None
+        loss_of(leaves).backward()
+        opt.step()
+
+    for call in (lambda w, m, b: norm.rms_norm(x, w), lambda w, m, b: dense.linear_fp8(x, m, b)):
+        leaves, _ = fresh()
+        held = call(*leaves)
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="default stream still holds"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call(*leaves).sum().backward()
+        held.sum().backward()  # the eager graph is as it was
+
+    eager, eager_opt = fresh()
+    for _ in range(4):
+        step(eager, eager_opt)
+    leaves, opt = fresh()
+    step(leaves, opt)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(leaves, opt)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    for p, q in zip(leaves, eager):
+        assert torch.equal(p, q)  # the same kernels on the same values, with sums in a fixed order
+    dense.check_status()

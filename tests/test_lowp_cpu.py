@@ -126,3 +126,24 @@ def test_adamw_status_codes(cuda_lib):
     assert call([]) == 0 and call([(None, None, None, None, None, None, 0)]) == 0  # nothing to do, nothing launched
     assert cuda_lib.gnnagg_adamw_tick(None, None, 1e-3, 0.9, 0.999, 1e-8, 0.0, 16, None) == -1
     assert cuda_lib.gnnagg_adamw_tick(16, None, 1e-3, 1.0, 0.999, 1e-8, 0.0, 16, None) == -1
+
+
+def test_missing_front_end_fails_loudly(cuda_lib, monkeypatch, tmp_path):
+    from gnn_benchmark_b200 import _lib
+
+    monkeypatch.setattr(_lib, "_ops", None)
+    monkeypatch.setattr(_lib, "OPS_PATH", str(tmp_path / "nope.so"))
+    with pytest.raises(RuntimeError, match="is missing"):
+        _lib.ops()
+
+
+def test_optimizer_refuses_shared_parameters_and_foreign_state():
+    from gnn_benchmark_b200 import optim
+
+    p = torch.nn.Parameter(torch.ones(4))
+    with pytest.warns(UserWarning, match="duplicate"), pytest.raises(ValueError, match="twice"):
+        optim.AdamW([p, p])
+    opt = optim.AdamW([p])
+    with pytest.raises(ValueError, match="another optimiser"):
+        opt.load_state_dict(torch.optim.AdamW([p]).state_dict())
+    assert opt.param_groups[0]["state_bits"] == 32
