@@ -197,3 +197,53 @@ def test_captured_step_next_to_an_eager_graph():
     for p, q in zip(leaves, eager):
         assert torch.equal(p, q)  # the same kernels on the same values, with sums in a fixed order
     dense.check_status()
+
+
+@pytest.mark.parametrize("what", ["norm", "quantise", "product", "adamw"])
+def test_offsets_past_32_bits(what):
+    """Tensors of more than 2^31 elements: the last rows (for AdamW the last blocks) are what a call on them alone
+    gives, bit for bit; the product's last rows are held to 64 bits."""
+    from gnn_benchmark_b200 import dense, norm, optim
+
+    torch.manual_seed(0)
+    rows, f, tail = 131073 + 128, 16384, 130  # (2^17 + 129) * 2^14 elements
+    if what in ("norm", "quantise"):
+        x = torch.randn(rows, f, device="cuda", dtype=torch.bfloat16)
+        assert x.numel() > 2 ** 31
+        last = x[-tail:].clone()
+    if what == "norm":
+        w = torch.ones(f, device="cuda", requires_grad=True)
+        x.requires_grad_()
+        y = norm.rms_norm(x, w)
+        assert torch.equal(y[-tail:], norm.rms_norm(last, w))
+        y.backward(x.detach())
+        last.requires_grad_()
+        norm.rms_norm(last, w).backward(last.detach())
+        assert torch.equal(x.grad[-tail:], last.grad)
+        del y
+        codes, scales = norm.rms_norm_fp8(x.detach(), w.detach())
+        codes1, scales1 = norm.rms_norm_fp8(last.detach(), w.detach())
+        assert torch.equal(codes[-tail:].view(torch.uint8), codes1.view(torch.uint8)) and torch.equal(scales[-tail:], scales1)
+    elif what == "quantise":
+        codes, scales = dense.quantize_fp8(x)
+        codes1, scales1 = dense.quantize_fp8(last)
+        assert torch.equal(codes[-tail:].view(torch.uint8), codes1.view(torch.uint8)) and torch.equal(scales[-tail:], scales1)
+        codes, scales = dense.quantize_fp8(x, transpose=True)
+        codes1, scales1 = dense.quantize_fp8(x[:, -tail:], transpose=True)  # rows of the transpose
+        assert torch.equal(codes[-tail:].view(torch.uint8), codes1.view(torch.uint8)) and torch.equal(scales[-tail:], scales1)
+    elif what == "product":
+        a, b = dense.quantize_fp8(torch.randn(rows, 128, device="cuda")), dense.quantize_fp8(torch.randn(f, 128, device="cuda"))
+        out = dense.matmul_fp8(*a, *b)
+        assert out.numel() > 2 ** 31
+        _close(out[-tail:], values(*a)[-tail:], values(*b))
+    else:
+        n, cut = 2 ** 31 + 77, 2 ** 31 - 512
+        p, g = (torch.randn(n, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+        m, v = (torch.zeros(n, device="cuda", dtype=torch.uint8).view(torch.float8_e4m3fn) for _ in range(2))
+        s = torch.zeros((n + 255) // 256, 2, device="cuda")
+        p1, g1, m1, v1, s1 = p[cut:].clone(), g[cut:].clone(), m[cut:].clone(), v[cut:].clone(), s[cut // 256:].clone()
+        optim.adamw_step([p], [g], [m], [v], scales=[s], step=1, lr=1e-2)
+        optim.adamw_step([p1], [g1], [m1], [v1], scales=[s1], step=1, lr=1e-2)
+        assert torch.equal(p[cut:], p1) and torch.equal(s[cut // 256:], s1)
+        assert torch.equal(m[cut:].view(torch.uint8), m1.view(torch.uint8)) and torch.equal(v[cut:].view(torch.uint8), v1.view(torch.uint8))
+    dense.check_status()
