@@ -1,7 +1,7 @@
 """AdamW over many tensors at once, with moments in 32 or 8 bits.
 
 The reference trains with torch.optim.Adam (self_benchmark/a64fx/model/utils.py:24), a loop of element-wise passes
-over every parameter.  Here one kernel launch updates up to 500 tensors: `adamw_step` is the plain call on lists of
+over every parameter.  Here one kernel launch updates up to 480 tensors: `adamw_step` is the plain call on lists of
 tensors, `AdamW` the torch.optim.Optimizer around it.
 
 8-bit moments (`state_bits=8`) take 2.03 bytes a parameter instead of 8: e4m3 codes of the first moment and of the
