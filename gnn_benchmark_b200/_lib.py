@@ -90,10 +90,6 @@ SIGNATURES = {
     "gnnagg_adamw_step": (ctypes.c_int, [_vp, _i64, _i32, _i32] + [ctypes.c_double] * 5 + [_i64, _vp, _vp]),
 }
 
-# element types of the low-precision entry points
-F32, BF16, F16 = 0, 1, 2
-TYPES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
-
 
 def lib():
     """The loaded library.  Raises if libgnnagg.so has not been built

@@ -8,8 +8,8 @@
 // shared tile: 8 rows of a column are one 8-byte piece, at piece index XOR (column / V) so that a warp's stores meet
 // different banks, and leave as 16-byte stores.
 // Bound by memory: per element its bytes in and one byte out for each orientation.  What keeps it from the floor is
-// instruction issue: 7 instructions an element with both orientations (15 with a shuffle reduction per row and a
-// reciprocal per thread and column: 195 us at 16384 x 8192 bf16).
+// instruction issue: 16384 x 8192 bf16 in both orientations take 109 us, 4.9 TB/s, at 7 instructions an element (195 us at
+// 15, with a shuffle reduction per row and a reciprocal per thread and column); fp32 161 us, 5.0 TB/s.
 #include "lowp.cuh"
 
 namespace gnnagg {

@@ -6,9 +6,12 @@
 //
 // Forward is one pass: a row stays in registers, as it lies in memory, between the sum of squares and the scaling.  A
 // row of up to 16 16-byte chunks belongs to half a warp, of up to 128 to a warp (short ones two at a time, so that a warp
-// has 1 to 2 KB on their way), a longer one to a block of as many threads as it fills.  Backward reads h and the two gradients once, writes dh
-// once and keeps the column sums of dw in registers over all rows of a persistent block; a second kernel adds the
-// blocks' sums in a fixed order (no atomics).
+// has 1 to 2 KB on their way), a longer one to a block of as many threads as it fills.  Backward reads h and the two gradients
+// once, writes dh once and keeps the column sums of dw in registers over all rows of a persistent block; a second kernel
+// adds the blocks' sums in a fixed order (no atomics).
+//
+// Bound by memory forward: 612500 x 256 bf16 with a residual in 189 us, 6.6 TB/s (codes: 184).  Backward by instruction
+// issue and the two reductions a row: 218 us there, 5.8 TB/s; 8191 x 5000 takes 56 and 79 us.
 //
 // As codes: with t = h w and a = max |t| over 128 columns, code = e4m3(t * (448 / a)) and scale = a / 448 * r.
 // The row's statistic enters the scale alone, so the codes are ready before the sum of squares is, and do not

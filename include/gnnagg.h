@@ -352,7 +352,7 @@ int gnnagg_relu_dropout_bwd(const float *GY, int64_t ldg, const uint8_t *mask, i
  *   F <= 16384; any alignment and strides of at least F elements (16-byte accesses where all rows allow them)
  * gnnagg_rms_norm_fp8 writes e4m3 codes and a scale per row and 128 columns instead of y: with t = h * w and
  * a = max(max |t| of the group, 2^-96), code = e4m3(t * (448 * (1 / a))), scale = a * (1 / 448) * r.  Code rows
- * start on 16 bytes (ldc % 16 == 0; the padding behind column F is overwritten with zeros up to the next 8);
+ * start on 16 bytes (ldc % 16 == 0; the padding behind column F may be overwritten with zeros);
  * the scale of (row, group j) is scales[row + j * lds].
  * gnnagg_rms_norm_bwd: gx = gh + r * (w gy - hat * mean(w gy hat)) with hat = h r (gh may be NULL, gx may alias gy
  * or gh) is the gradient of x and of the residual; dw = sum over the rows of gy * hat, of w's type, added up in a
@@ -437,7 +437,7 @@ int gnnagg_fp8_linear_bwd(const void *g, int64_t ldg, int32_t g_type, int64_t M,
  *   master      fp32 copy that is updated and that `param` is rounded from; NULL: param itself is updated
  *   step        t, from 1; ignored when device_scalars is given
  *   device_scalars  what gnnagg_adamw_tick left: that call adds 1 to *step and writes the step's scalars
- *               (gnnagg_adamw_scalars_bytes bytes, 16-byte aligned) on the device, so that a replayed graph counts
+ *               (gnnagg_adamw_scalars_bytes bytes, 4-byte aligned) on the device, so that a replayed graph counts
  *               its steps; lr (a device fp32) overrides host_lr when not NULL.
  * No two tensors of a call may overlap.
  * ---------------------------------------------------------------------------------- */
