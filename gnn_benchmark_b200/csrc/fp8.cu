@@ -690,7 +690,7 @@ int make_map_f8(CUtensorMap *map, const void *base, int64_t rows, int64_t cols, 
 }
 
 // The output as `splits` matrices of M x N one behind the other, in boxes of 128 bytes x 32 rows; a tile's part
-// outside its matrix is not written.
+// outside its matrix is not written, but for what completes a row's last 16 bytes.
 int make_map_out(CUtensorMap *map, void *base, int type, int splits, int64_t M, int64_t N, int64_t ld) {
     EncodeTiledFn fn = encode_fn();
     const int size = type_size(type);
@@ -844,8 +844,9 @@ extern "C" int gnnagg_fp8_matmul(const uint8_t *A, int64_t lda, const float *sa,
     const int64_t ldo = split ? plan.ldp : ldc;
     void *out = split ? workspace : C;
     const bool vec_out = aligned16(out) && (ldo * type_size(type)) % 16 == 0 && !(accumulate && !split);
-    // wide tiles leave by TMA where it can address the rows
-    const bool tma_out = vec_out && !plan.swap && plan.bn >= 128;
+    // wide tiles leave by TMA where it can address the rows; it ends a row on 16 bytes, so a row that ends between them
+    // would have what lies behind it written over (padding in the workspace, the caller's own in an output)
+    const bool tma_out = vec_out && !plan.swap && plan.bn >= 128 && (split || N * type_size(type) % 16 == 0);
     CUtensorMap map_c = map_p;  // not used without tma_out
     if (tma_out) rc = make_map_out(&map_c, out, type, plan.splits, M, N, ldo);
     if (rc != GNNAGG_OK) return rc;

@@ -328,3 +328,21 @@ def test_product_refuses_to_drop_a_gradient():
         dense.matmul_fp8(*a, *b, out=torch.zeros(30, 40, device="cuda", requires_grad=True))
     with torch.no_grad():
         assert torch.equal(dense.matmul_fp8(*a, *b, bias=bias), dense.matmul_fp8(*a, *b))
+
+
+@pytest.mark.parametrize("n", [185, 322, 567, 1001])
+@pytest.mark.parametrize("m,k", [(300, 200), (70, 9000)])
+def test_columns_behind_an_odd_width_stay(m, n, k):
+    """A row of the output that ends between two 16-byte steps, inside aligned wider rows: what follows is left alone."""
+    from gnn_benchmark_b200 import dense
+
+    qa, qb = dense.quantize_fp8(_matrix(m, k, 1)), dense.quantize_fp8(_matrix(n, k, 2), (128, 128))
+    for dtype in TYPES:
+        want = dense.matmul_fp8(*qa, *qb, out_dtype=dtype)
+        for off in (0, 8):
+            wide = torch.full((m, (n + 8 + off) // 8 * 8), 7.0, device="cuda", dtype=dtype)
+            dense.matmul_fp8(*qa, *qb, out=wide[:, off:off + n])
+            assert torch.equal(wide[:, off:off + n], want)
+            wide[:, off:off + n] = 7.0
+            assert (wide == 7.0).all()
+    dense.check_status()
