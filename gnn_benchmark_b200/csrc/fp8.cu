@@ -21,14 +21,17 @@
 //               lane quarter w % 4 and one half of the columns.
 // What bounds a block is the hand-over and scaling: per scheduler 256 FMAs, 180 cycles of tensor-memory reads and a
 // round trip between the warps of some 400 cycles over two buffers, against 512 cycles of MMA.  So the scaling loop holds
-// nothing that another warp can do.  8192 x 8192 x 8192 takes 515 us alone, 2.1 PFLOP/s, and 589 in a long run at the
+// nothing that another warp can do.  8192 x 8192 x 8192 takes 490 us alone, 2.2 PFLOP/s, and 583 in a long run at the
 // power limit.  Two CTAs that share a tile's operands were slower (the hand-over then takes 1279 cycles instead of 590),
 // and so were tiles 128 wide with two CTAs an SM (644 us where this took 539), and sixteen scaling warps.
 // Where one column of tiles and few k-blocks make up the product (tall activations, a small weight), Q stays in shared
 // memory and only P's blocks go round: a third of the loads, and twice the blocks on their way (612500 x 256 x 100 in
-// 74 us instead of 109; its bytes take 58).
+// 76 us instead of 109; its bytes take 58).
 // Output tiles leave through shared memory by TMA stores, which run under the next tile's MMAs; rows that TMA cannot
 // address, and outputs that are added to, by plain stores.
+// The tiles of a last round that would leave SMs idle are shared out evenly instead: each CTA takes the same number of
+// their k-blocks, a stretch that lies in one tile or two.  Whoever completes a tile (a count per tile and warp, no
+// waiting) adds its parts in the order of k and stores it.
 // A tile's sum may be split along k over several CTAs (few tiles, long sums): each writes an fp32 partial product
 // to the workspace and a second kernel adds them in a fixed order; up to eight small ones (few rows) are CTAs of a
 // cluster, and the first adds the others' from its own shared memory, which saves the second launch (8 x 4096 x 4096:
@@ -112,6 +115,9 @@ struct Params {
     int tma_out;         // the output leaves by TMA
     unsigned long long wait_ns;
     uint32_t tx_excess;
+    float *parts;        // sums of shared tiles' parts, two places a CTA
+    int *counts;         // parts of a shared tile that are there, for each scaling warp
+    int full, tail, per; // tiles that have a CTA of their own, tiles that are shared, k-blocks of these for each CTA
 };
 
 __device__ __forceinline__ void tc_mma_f8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
@@ -178,18 +184,40 @@ __host__ __device__ constexpr uint32_t f8_instr_desc(int n) {
     return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(BP >> 4) << 24);
 }
 
-// A work item: one tile of the output and a range of its k-blocks.
+// A work item: one tile of the output and a range of its k-blocks.  Of a shared tile: its number among them, and the
+// CTAs that have a part of it.
 struct Item {
     int tp, tq, split, kb0, kb1;
+    int shared, cta0, ctas;
 };
+// The shared tiles' k-blocks lie one behind the other, CTA c has [c per, (c + 1) per); per is less than a tile's.
+__device__ __forceinline__ int shared_first(const Params &p, int cta) { return cta * p.per / p.kblocks; }
 // Tiles of one column strip of 16 P-tiles are neighbours, so that concurrent CTAs share operand panels in L2.
+template <bool TAIL>
 __device__ __forceinline__ Item item_of(const Params &p, int i) {
     Item w;
     int t = i;
     w.split = 0, w.tq = 0;
-    if (p.splits > 1) {
+    if (TAIL) w.ctas = 1;
+    w.kb0 = 0, w.kb1 = p.kblocks;
+    if (TAIL && i >= p.full) {
+        const int second = i - p.full >= kNumSMs ? 1 : 0, cta = i - p.full - second * kNumSMs;
+        const int a = cta * p.per, e = min(a + p.per, p.tail * p.kblocks);
+        w.shared = shared_first(p, cta) + second;
+        const int begin = w.shared * p.kblocks;
+        w.kb0 = max(a - begin, 0);
+        w.kb1 = min(e - begin, p.kblocks);  // not above kb0: this CTA has no such part
+        w.cta0 = begin / p.per;
+        w.ctas = (begin + p.kblocks - 1) / p.per - w.cta0 + 1;
+        w.tp = 0;
+        if (w.kb0 >= w.kb1) return w;
+        t = p.full + w.shared;
+    }
+    if (!TAIL && p.splits > 1) {
         t = i / p.splits;
         w.split = i - t * p.splits;
+        w.kb0 = w.split * p.kb_per_split;
+        w.kb1 = min(p.kblocks, w.kb0 + p.kb_per_split);
     }
     w.tp = t;
     if (p.tiles_q > 1) {
@@ -199,8 +227,6 @@ __device__ __forceinline__ Item item_of(const Params &p, int i) {
         w.tq = r / high;
         w.tp = g * kGroup + (r - w.tq * high);
     }
-    w.kb0 = w.split * p.kb_per_split;
-    w.kb1 = min(p.kblocks, w.kb0 + p.kb_per_split);
     return w;
 }
 
@@ -215,12 +241,14 @@ struct Ring {
     }
 };
 
-// SWAP: the output is stored transposed, C[column][lane].  JOIN (with SWAP): the splits of a tile are a cluster.
-template <int BN, bool QROW, bool SWAP, bool JOIN, typename TOut>
+// SWAP: the output is stored transposed, C[column][lane].  SHARE: with SWAP the splits of a tile are a cluster, without
+// the last round's tiles are shared out (a variant of its own: the others lose 2 to 5 % to its code).
+template <int BN, bool QROW, bool SWAP, bool SHARE, typename TOut>
 __global__ void __launch_bounds__((Tile<BN, QROW>::kThreads), 1)
 fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
                   const __grid_constant__ CUtensorMap map_c, const Params p) {
     using S = Tile<BN, QROW>;
+    constexpr bool JOIN = SWAP && SHARE, TAIL = !SWAP && SHARE;
     constexpr int kBufs = S::kBufs, kCols = S::kCols, kWarps = S::kWarps;
     extern __shared__ uint8_t smem_raw[];
     // 1024-byte alignment: the swizzle pattern and the descriptors assume it
@@ -283,7 +311,7 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_consta
             }
             __syncwarp();
             for (int i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
-                const Item w = item_of(p, i);
+                const Item w = item_of<TAIL>(p, i);
                 for (int kb = w.kb0; kb < w.kb1; ++kb, ++it, st.next()) {
                     if (!mbar_wait(bar_empty(st.i), st.phase ^ 1u, abort_flag, &g_status, kErrWaitEmpty, p.wait_ns)) {
                         ok = false;
@@ -319,7 +347,7 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_consta
             Ring ac(kBufs);
             bool ok = !p.keep_q || mbar_wait(bar_q, 0, abort_flag, &g_status, kErrWaitFull, p.wait_ns);
             for (int i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
-                const Item w = item_of(p, i);
+                const Item w = item_of<TAIL>(p, i);
                 for (int kb = w.kb0; kb < w.kb1; ++kb, st.next(), ac.next()) {
                     if (!mbar_wait(bar_full(st.i), st.phase, abort_flag, &g_status, kErrWaitFull, p.wait_ns) ||
                         !mbar_wait(bar_acc_empty(ac.i), ac.phase ^ 1u, abort_flag, &g_status, kErrWaitAccFree, p.wait_ns)) {
@@ -361,7 +389,8 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_consta
             uint32_t it = 0;  // of all blocks; this warp has every second
             bool ok = true;
             for (int i = blockIdx.x; i < p.items && ok; i += gridDim.x) {
-                const Item w = item_of(p, i);
+                const Item w = item_of<TAIL>(p, i);
+                if (TAIL && w.kb0 >= w.kb1) continue;
                 const int64_t row0 = (int64_t)w.tp * BP, col0 = (int64_t)w.tq * BN;
                 const int first = w.kb0 + (int)((it ^ (uint32_t)(warp - 2)) & 1u);
                 auto fetch = [&](int kb) {
@@ -433,7 +462,8 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_consta
         int64_t bias_at = -1;  // first column of the bias that is there
         uint32_t limit = 1u << 22;
         for (int i = blockIdx.x; i < p.items; i += gridDim.x) {
-            const Item w = item_of(p, i);
+            const Item w = item_of<TAIL>(p, i);
+            if (TAIL && w.kb0 >= w.kb1) continue;
             const int64_t row0 = (int64_t)w.tp * BP + q * 32;                    // of P
             const int64_t col0 = (int64_t)w.tq * BN + part * kCols;              // of Q
             float acc[kCols];
@@ -506,6 +536,29 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_consta
                 for (int r = 1; r < p.splits; ++r)
 #pragma unroll
                     for (int j = 0; j < kCols; ++j) acc[j] += sums[((r - 1) * kWarps * kCols + j) * 32];
+            }
+            if (TAIL && w.ctas > 1) {
+                auto place = [&](int cta) {  // of this warp's share of the tile's part
+                    const int second = shared_first(p, cta) != w.shared;
+                    return p.parts + ((int64_t)((cta * 2 + second) * kWarps + (warp - 4)) * kCols) * 32 + lane;
+                };
+                float *own = place((int)blockIdx.x);
+#pragma unroll
+                for (int j = 0; j < kCols; ++j) __stcg(own + j * 32, acc[j]);
+                __threadfence();
+                __syncwarp();
+                int there = 0;
+                if (lane == 0) there = atomicAdd(p.counts + w.shared * kWarps + (warp - 4), 1) + 1;
+                there = __shfl_sync(kFullMask, there, 0);
+                if (there < w.ctas) continue;  // another one completes the tile
+                __threadfence();
+#pragma unroll
+                for (int j = 0; j < kCols; ++j) acc[j] = 0.0f;
+                for (int c = w.cta0; c < w.cta0 + w.ctas; ++c) {
+                    const float *src = place(c);
+#pragma unroll
+                    for (int j = 0; j < kCols; ++j) acc[j] += __ldcg(src + j * 32);
+                }
             }
             if (SWAP) {
                 // lane = column of the output: 32 neighbouring columns of one output row per store
@@ -635,13 +688,21 @@ fp8_join_kernel(const float *__restrict__ partial, int splits, int64_t split_str
     }
 }
 
+constexpr int64_t kSharedOperands = 180000000;  // bytes of both operands, up to which a last round is shared out
+constexpr size_t kCountBytes = 8192;  // counts of shared tiles: fewer than the SMs, eight warps each
+static_assert(kNumSMs * 8 * sizeof(int) <= kCountBytes, "counts of shared tiles");
+
 // What a call of these sizes runs: which operand lies along the lanes, the tile's columns, the splits of the sum.
 struct Plan {
     bool swap;
     int bn, tiles_p, tiles_q, splits, kb_per_split, kblocks;
     int64_t ldp;  // row stride of a partial product
-    size_t bytes() const { return splits > 1 && !join ? (size_t)splits * rows * ldp * sizeof(float) : 0; }
+    size_t bytes() const {
+        if (tail > 0) return kCountBytes + (size_t)2 * kNumSMs * BP * bn * sizeof(float);
+        return splits > 1 && !join ? (size_t)splits * rows * ldp * sizeof(float) : 0;
+    }
     int64_t rows;
+    int tail, per;  // tiles that are shared, k-blocks of these for each CTA
     bool join;    // the splits of a tile are a cluster
 };
 
@@ -672,6 +733,20 @@ Plan plan_of(int64_t M, int64_t N, int64_t K) {
     p.join = p.swap && p.splits > 1 && p.splits <= 8 && (p.splits - 1) * BP * p.bn * 4 <= stage_bytes(p.bn);
     p.rows = M;
     p.ldp = div_up(N, 4) * 4;
+    // A last round of fewer tiles than SMs is shared out where that shortens it by 40 k-blocks or more (a block takes
+    // 0.4 us, 0.8 with row scales on both sides; the parts' way through memory and the cleared counts 12 to 14 us in all).
+    // 2048 x 2560 x 8192: 73 -> 66 us, with row scales 116 -> 91; 4096 x 4096 x 4096, 17 blocks shorter: 80 -> 86.  CTAs
+    // that share a tile are at different k at a time, so the operands have to stay in L2 in the main: at 168 MB (8192 x
+    // 2048 x 16384) 275 -> 262 and 424 -> 391, at 210 MB (1500 x 2000 x 60000) 263 -> 352.  At most nine CTAs have a part
+    // of a tile.
+    p.tail = 0, p.per = 0;
+    const int64_t rest = tiles % kNumSMs;
+    if (!p.swap && p.bn >= 128 && p.splits == 1 && rest > 0 && K > 0 && M + N <= kSharedOperands / K) {
+        int64_t per = div_up(rest * p.kblocks, kNumSMs);
+        if (per < div_up(p.kblocks, 8)) per = div_up(p.kblocks, 8);
+        if (per < 4) per = 4;
+        if (p.kblocks - per >= 40) p.tail = (int)rest, p.per = (int)per;
+    }
     return p;
 }
 
@@ -707,18 +782,18 @@ int make_map_out(CUtensorMap *map, void *base, int type, int splits, int64_t M, 
     return GNNAGG_OK;
 }
 
-template <int BN, bool QROW, bool SWAP, bool JOIN, typename TOut>
+template <int BN, bool QROW, bool SWAP, bool SHARE, typename TOut>
 int launch(const CUtensorMap &mp, const CUtensorMap &mq, const CUtensorMap &mc, Params p, cudaStream_t st) {
     using S = Tile<BN, QROW>;
     static PerDeviceOnce attr_done;
     const cudaError_t e = attr_done.run([] {
         cudaFuncAttributes a;
-        const cudaError_t r = cudaFuncGetAttributes(&a, fp8_matmul_kernel<BN, QROW, SWAP, JOIN, TOut>);
+        const cudaError_t r = cudaFuncGetAttributes(&a, fp8_matmul_kernel<BN, QROW, SWAP, SHARE, TOut>);
         if (r != cudaSuccess) return r;
         // a register split above what the launch allocates would wait forever
         if (S::kSplitRegs && (a.numRegs > kRegsScaling || a.numRegs * S::kThreads < S::kRegsNeeded))
             return cudaErrorInvalidConfiguration;
-        return cudaFuncSetAttribute(fp8_matmul_kernel<BN, QROW, SWAP, JOIN, TOut>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        return cudaFuncSetAttribute(fp8_matmul_kernel<BN, QROW, SWAP, SHARE, TOut>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     S::kSmem);
     });
     if (e != cudaSuccess)
@@ -727,9 +802,9 @@ int launch(const CUtensorMap &mp, const CUtensorMap &mq, const CUtensorMap &mc, 
     const int grid = p.items < kNumSMs ? p.items : kNumSMs;
     // Q stays where every CTA has several tiles of one column, and all of its k-blocks and three of P's fit
     const int left = S::kStages * S::kStageBytes - p.kblocks * BN * BK;
-    p.keep_q = p.tiles_q == 1 && p.splits == 1 && p.items > grid && left >= 3 * P_BYTES;
+    p.keep_q = p.tiles_q == 1 && p.splits == 1 && p.tiles_p > grid && left >= 3 * P_BYTES;
     p.stages = p.keep_q ? (left / P_BYTES < kMaxStages ? left / P_BYTES : kMaxStages) : S::kStages;
-    if (JOIN) {  // one item per CTA: all of them are resident
+    if (SWAP && SHARE) {  // one item per CTA: all of them are resident
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)p.items);
         cfg.blockDim = dim3(S::kThreads);
@@ -742,10 +817,10 @@ int launch(const CUtensorMap &mp, const CUtensorMap &mq, const CUtensorMap &mc, 
         attr[0].val.clusterDim.z = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        const cudaError_t le = cudaLaunchKernelEx(&cfg, fp8_matmul_kernel<BN, QROW, SWAP, JOIN, TOut>, mp, mq, mc, p);
+        const cudaError_t le = cudaLaunchKernelEx(&cfg, fp8_matmul_kernel<BN, QROW, SWAP, SHARE, TOut>, mp, mq, mc, p);
         if (le != cudaSuccess) return fail(GNNAGG_ERR_CUDA, "fp8_matmul_kernel: %s", cudaGetErrorString(le));
     } else {
-        fp8_matmul_kernel<BN, QROW, SWAP, JOIN, TOut><<<grid, S::kThreads, S::kSmem, st>>>(mp, mq, mc, p);
+        fp8_matmul_kernel<BN, QROW, SWAP, SHARE, TOut><<<grid, S::kThreads, S::kSmem, st>>>(mp, mq, mc, p);
     }
     return check_launch("fp8_matmul_kernel");
 }
@@ -761,6 +836,9 @@ int launch_tile(const Plan &plan, const CUtensorMap &mp, const CUtensorMap &mq, 
         return plan.bn == 16   ? launch<16, QROW, true, false, TOut>(mp, mq, mc, p, st)
                : plan.bn == 32 ? launch<32, QROW, true, false, TOut>(mp, mq, mc, p, st)
                                : launch<64, QROW, true, false, TOut>(mp, mq, mc, p, st);
+    if (plan.tail > 0)
+        return plan.bn == 128 ? launch<128, QROW, false, true, TOut>(mp, mq, mc, p, st)
+                              : launch<256, QROW, false, true, TOut>(mp, mq, mc, p, st);
     return plan.bn == 16    ? launch<16, QROW, false, false, TOut>(mp, mq, mc, p, st)
            : plan.bn == 32  ? launch<32, QROW, false, false, TOut>(mp, mq, mc, p, st)
            : plan.bn == 64  ? launch<64, QROW, false, false, TOut>(mp, mq, mc, p, st)
@@ -829,7 +907,7 @@ extern "C" int gnnagg_fp8_matmul(const uint8_t *A, int64_t lda, const float *sa,
     const Plan plan = plan_of(M, N, K);
     if (K == 0) return join_out(out_type, plan, nullptr, 0, M, N, bias, bias_type, accumulate, C, ldc, st);
     const bool split = plan.splits > 1 && !plan.join;  // through the workspace
-    if (split && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < plan.bytes()))
+    if (plan.bytes() > 0 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < plan.bytes()))
         return fail(GNNAGG_ERR_SCRATCH, "fp8_matmul: workspace too small or misaligned (need %zu bytes)", plan.bytes());
     if ((int64_t)plan.tiles_p * plan.tiles_q * plan.splits > 0x7FFFFFFF)
         return fail(GNNAGG_ERR_UNSUPPORTED, "fp8_matmul: too many tiles");
@@ -868,6 +946,14 @@ extern "C" int gnnagg_fp8_matmul(const uint8_t *A, int64_t lda, const float *sa,
     p.tiles_p = plan.tiles_p;
     p.tiles_q = plan.tiles_q;
     p.items = plan.tiles_p * plan.tiles_q * plan.splits;
+    p.tail = plan.tail, p.per = plan.per, p.full = p.items - plan.tail;
+    p.counts = static_cast<int *>(workspace);
+    p.parts = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + (plan.tail > 0 ? kCountBytes : 0));
+    if (plan.tail > 0) {
+        p.items = p.full + 2 * kNumSMs;
+        const cudaError_t e = cudaMemsetAsync(p.counts, 0, kCountBytes, st);
+        if (e != cudaSuccess) return fail(GNNAGG_ERR_CUDA, "fp8_matmul: %s", cudaGetErrorString(e));
+    }
     p.accumulate = split ? 0 : accumulate;
     p.vec_out = vec_out;
     p.tma_out = tma_out;

@@ -346,3 +346,39 @@ def test_columns_behind_an_odd_width_stay(m, n, k):
             wide[:, off:off + n] = 7.0
             assert (wide == 7.0).all()
     dense.check_status()
+
+
+@pytest.mark.parametrize("m,n,k", [(1500, 2000, 14801), (2000, 2600, 6400), (19000, 200, 5900), (18950, 100, 5910),
+                                   (18955, 10, 5950), (19100, 300, 5900), (4096, 4096, 9600)])
+def test_shared_last_round(m, n, k):
+    """Fewer tiles in the last round than SMs: their blocks are shared out, and the parts joined in one order."""
+    from gnn_benchmark_b200 import dense
+
+    qa = dense.quantize_fp8(_matrix(m, k, 1))
+    a64, bias = values(*qa), torch.randn(n, device="cuda")
+    for block in ((1, 128), (128, 128)):
+        qb = dense.quantize_fp8(_matrix(n, k, 2), block)
+        b64 = values(*qb)
+        ref = a64 @ b64.t() + bias.double()
+        room = _room(a64, b64, (k + 127) // 128) + 2 * U * (ref.abs() + bias.double().abs())
+        for dtype in TYPES:
+            out = dense.matmul_fp8(*qa, *qb, bias=bias, out_dtype=dtype)
+            ok = (out.double() - ref).abs() <= room + unit(dtype) * ref.abs() + floor(dtype)
+            # as in test_product: sums reach 1e6 here, and what is above 65504 has no fp16 value to be near to
+            assert (ok | (ref.abs() > torch.finfo(dtype).max)).all()
+            for _ in range(3):
+                assert torch.equal(dense.matmul_fp8(*qa, *qb, bias=bias, out_dtype=dtype), out)
+        base = torch.randn(m, n + 3, device="cuda")
+        got = base.clone()
+        dense.matmul_fp8(*qa, *qb, bias=bias, out=got[:, 1:n + 1], accumulate=True)
+        want = ref + base[:, 1:n + 1].double()
+        assert ((got[:, 1:n + 1].double() - want).abs() <= room + 3 * U * (want.abs() + base[:, 1:n + 1].double().abs() + ref.abs())).all()
+        assert torch.equal(got[:, 0], base[:, 0]) and torch.equal(got[:, n + 1:], base[:, n + 1:])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = dense.matmul_fp8(*qa, *qb, bias=bias, out_dtype=torch.float16)
+    for _ in range(2):
+        held.zero_()
+        graph.replay()
+        assert torch.equal(held, dense.matmul_fp8(*qa, *qb, bias=bias, out_dtype=torch.float16))
+    dense.check_status()
