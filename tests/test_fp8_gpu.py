@@ -261,10 +261,11 @@ def test_linear_without_rows_and_broadcast_gradient():
     assert all(torch.equal(s, t) for s, t in zip(a, c))
 
 
-@pytest.mark.parametrize("m,n,k", [(300, 200, 256), (300, 100, 256), (20000, 200, 200), (5, 2000, 4096), (40, 200, 20000)])
+@pytest.mark.parametrize("m,n,k", [(300, 200, 256), (300, 100, 256), (20000, 200, 200), (5, 2000, 4096), (40, 200, 20000),
+                                   (1500, 2000, 14801)])
 def test_bounded_wait_gives_up_and_reports(m, n, k):
     """A launch that waits for bytes which never come returns by itself, leaves its code, and the next is right: wide and
-    narrow tiles, a weight that stays, a cluster, splits through the workspace."""
+    narrow tiles, a weight that stays, a cluster, splits through the workspace, a shared last round."""
     from gnn_benchmark_b200 import _lib, dense
 
     lib = _lib.lib()
@@ -381,4 +382,22 @@ def test_shared_last_round(m, n, k):
         held.zero_()
         graph.replay()
         assert torch.equal(held, dense.matmul_fp8(*qa, *qb, bias=bias, out_dtype=torch.float16))
+    dense.check_status()
+
+
+def test_shared_rounds_on_two_streams():
+    from gnn_benchmark_b200 import dense
+
+    ops = [(dense.quantize_fp8(_matrix(m, k, i)), dense.quantize_fp8(_matrix(n, k, i + 5), (128, 128)))
+           for i, (m, n, k) in enumerate([(2000, 2600, 6400), (1500, 2000, 14801)])]
+    want = [dense.matmul_fp8(*a, *b, out_dtype=torch.float32) for a, b in ops]
+    streams = [torch.cuda.Stream() for _ in ops]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(dense.matmul_fp8(*ops[i][0], *ops[i][1], out_dtype=torch.float32))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, w) for gs, w in zip(got, want) for g in gs)
     dense.check_status()
