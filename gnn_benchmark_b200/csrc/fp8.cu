@@ -5,8 +5,8 @@
 //
 // Scales are fp32, one per row or one per 128 rows of either operand.  The inner sum of a block is a chain of four
 // MMAs into tensor memory; the outer one is taken in registers, one FMA per element and block, rounded to nearest (two
-// FMAs packed into one instruction are no faster: 258 cycles a block against 262).  Tensor memory holds several blocks' partial products, so the MMAs of the next block run under the FMAs
-// of the last.
+// FMAs packed into one instruction are no faster: 258 cycles a block against 262).  Tensor memory holds several blocks'
+// partial products, so the MMAs of the next block run under the FMAs of the last.
 //
 // One operand lies along the 128 lanes of tensor memory (P), the other along its columns (Q).  P is A and Q is B,
 // except for few rows of A (SWAP): then the weight's rows fill the lanes and the few rows are the columns.
@@ -33,9 +33,9 @@
 // their k-blocks, a stretch that lies in one tile or two.  Whoever completes a tile (a count per tile and warp, no
 // waiting) adds its parts in the order of k and stores it.
 // A tile's sum may be split along k over several CTAs (few tiles, long sums): each writes an fp32 partial product
-// to the workspace and a second kernel adds them in a fixed order; up to eight small ones (few rows) are CTAs of a
-// cluster, and the first adds the others' from its own shared memory, which saves the second launch (8 x 4096 x 4096:
-// 10 us a call, and 256 x 256 x 612500 in 81 us + 9 for the second kernel).
+// to the workspace and a second kernel adds them in a fixed order (256 x 256 x 612500: 81 us and 9 for that kernel); up
+// to eight small ones (few rows) are CTAs of a cluster, and the first adds the others' from its own shared memory, which
+// saves the second launch (8 x 4096 x 4096: 10 us a call).
 // Every wait is bounded (about a second); on a time-out the kernel records a code in the library's status word,
 // drains its own copies and MMAs, frees tensor memory and returns.
 #include "lowp.cuh"
