@@ -374,7 +374,7 @@ gemm_tf32x3_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                         ++nstore;
                         continue;
                     }
-                    // output rows that TMA cannot address (stride not a multiple of 16 bytes): transpose the
+                    // output rows that TMA cannot address (not whole 16-byte steps): transpose the
                     // block through shared memory and store row segments with plain coalesced stores
 #pragma unroll
                     for (int j = 0; j < 32; ++j) tr[lane * kEpiPad + j] = v[j];
@@ -777,8 +777,9 @@ extern "C" int gnnagg_dense_tf32x3_f32(const float *A, int64_t lda, const float 
         return fail(GNNAGG_ERR_CUDA, "dense: cannot reserve %d bytes of shared memory: %s", SMEM_BYTES,
                     cudaGetErrorString(attr_err));
 
-    // C goes out through TMA when its rows are 16-byte addressable, else through plain stores
-    const bool tma_store = aligned16(C) && (ldc % 4) == 0;
+    // C goes out through TMA when its rows start and end on 16 bytes, else through plain stores: TMA completes a row's
+    // last 16 bytes, so a row that ends between them would have up to 12 bytes behind it written over (or added to)
+    const bool tma_store = aligned16(C) && (ldc % 4) == 0 && (N % 4) == 0;
     CUtensorMap map_a, map_bhi, map_blo, map_c;
     int rc = make_map(&map_a, A, M, K, lda, BK, BM);
     const int b_box_rows = n_pad;  // all weight rows of a k-block in one box (rows past N read as zero)

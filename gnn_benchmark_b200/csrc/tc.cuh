@@ -90,7 +90,8 @@ __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap *map, int x, i
     asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
 }
 
-// Shared -> global tile store / add through the tensor map (rows and columns outside the tensor are clipped).
+// Shared -> global tile store / add through the tensor map.  Rows outside the tensor are clipped, and columns in steps of
+// 16 bytes: a row that ends between two steps has its last step written whole.
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, uint32_t src, int x, int y) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(src),
                  "r"(x), "r"(y)

@@ -203,3 +203,28 @@ def test_bounded_waits_give_up_and_report():
     assert ((dw.double() - ref).abs() / scale).max().item() <= 2e-6
     _case(1000, 256, 256, bias=True, accumulate=False, seed=5)
     assert lib.gnnagg_dense_stall_test(-1, 0) != 0 and lib.gnnagg_dense_stall_test(16, 10**7) != 0
+
+
+@pytest.mark.parametrize("N", [1, 45, 46, 47, 253])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_columns_behind_an_odd_width_stay(N, accumulate):
+    """A row of the output that ends between two 16-byte steps, inside 16-byte aligned wider rows: the columns in front of
+    it and behind it keep their values, the last row's too, where the allocation goes on."""
+    from gnn_benchmark_b200 import dense
+
+    g = torch.Generator(device="cuda").manual_seed(N)
+    M, K = 300, 64
+    a, w = torch.randn(M, K, device="cuda", generator=g), torch.randn(N, K, device="cuda", generator=g)
+    bias = torch.randn(N, device="cuda", generator=g)
+    for off in (0, 4):
+        wide = torch.full((M, (N + 3) // 4 * 4 + 8), 7.0, device="cuda")
+        out = wide[:, off:off + N]
+        assert out.data_ptr() % 16 == 0 and out.stride(0) % 4 == 0
+        dense.linear(a, w, bias, out=out, accumulate=accumulate)
+        start = 7.0 if accumulate else 0.0
+        ref = a.double() @ w.double().t() + bias.double() + start
+        scale = a.abs().double() @ w.abs().double().t() + bias.abs().double() + start
+        assert ((out.double() - ref).abs() <= 2e-6 * scale).all()
+        out.fill_(7.0)
+        assert (wide == 7.0).all(), "wrote outside the N output columns"
+    dense.check_status()
