@@ -7,6 +7,8 @@ tensors, `AdamW` the torch.optim.Optimizer around it.
 8-bit moments (`state_bits=8`) take 2.03 bytes a parameter instead of 8: e4m3 codes of the first moment and of the
 second moment's square root, in blocks of 256 elements with an fp32 scale each.
 """
+import weakref
+
 import torch
 
 from . import _lib
@@ -43,7 +45,9 @@ class AdamW(torch.optim.Optimizer):
     state_bits: 32, or 8 for block-quantised moments.  master_weights: keep a float32 copy of 16-bit parameters and
     round the parameter from it at every step.  capturable: the step count lives on the device, so that `step()` can
     be captured into a CUDA graph and replayed; `lr` may then be a 0-dim float32 CUDA tensor that the caller changes
-    between replays.  Parameters are dense float32, bfloat16 or float16 CUDA tensors, and contiguous."""
+    between replays.  Parameters that have always stepped together share a count, and part when one of them has no
+    gradient in a step; a capture, and every step after it, takes all parameters of a count or none.  Parameters are
+    dense float32, bfloat16 or float16 CUDA tensors, and contiguous."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
                  state_bits: int = 32, master_weights: bool = False, capturable: bool = False):
@@ -101,6 +105,29 @@ class AdamW(torch.optim.Optimizer):
         self.state[p] = state
         return state
 
+    def _own_counts(self, members, capturing) -> None:
+        """Device counts for the parameters that step together: one that is also held by a parameter that does not step
+        now stays with that one, and the others go on with a copy.  A count of a captured step is advanced by every
+        replay, so it stays with all of its parameters."""
+        stepping = {id(p) for p, _ in members}
+        idle = {id(s["step"]) for p, s in self.state.items() if s and id(p) not in stepping}
+        known = self.__dict__.setdefault("_captured", {})  # id -> weak reference: counts of captured steps
+        copies = {}
+        for _, state in members:
+            count = state["step"]
+            if id(count) in idle:
+                if capturing:
+                    raise RuntimeError("AdamW: take a step with the gradients of these parameters alone before capturing (they "
+                                       "share their step count with parameters that have no gradient)")
+                if id(count) in known and known[id(count)]() is count:
+                    raise RuntimeError("AdamW: a captured step updates parameters that have no gradient now together with "
+                                       "others that have one: their step count is shared")
+                if id(count) not in copies:
+                    copies[id(count)] = count.clone()
+                state["step"] = copies[id(count)]
+            elif capturing:
+                known[id(count)] = weakref.ref(count)
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
@@ -111,7 +138,7 @@ class AdamW(torch.optim.Optimizer):
         for group in self.param_groups:
             if capturing and not group["capturable"]:
                 raise RuntimeError("AdamW: a step that is captured into a graph needs capturable=True")
-            fresh, calls = {}, {}  # calls: (device, count) -> type -> members
+            fresh, members, calls = {}, [], {}  # calls: (device, count) -> type -> members
             for p in group["params"]:
                 if p.grad is None:
                     continue
@@ -123,6 +150,10 @@ class AdamW(torch.optim.Optimizer):
                     if capturing:
                         raise RuntimeError("AdamW: take one step before capturing (it creates the moments)")
                     state = self._new_state(p, group, fresh)
+                members.append((p, state))
+            if group["capturable"]:
+                self._own_counts(members, capturing)
+            for p, state in members:
                 if group["capturable"]:
                     key = (p.device, id(state["step"]))
                 else:

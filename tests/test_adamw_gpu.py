@@ -318,3 +318,32 @@ def test_more_refusals():
     square = [p[0].view(3, 4)]
     with pytest.raises(RuntimeError, match="shape"):  # a transposed gradient has as many elements
         optim.adamw_step(square, [g[0].view(4, 3)], m, v, step=1, lr=1e-3)
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+def test_a_step_without_a_gradient_is_not_counted(capturable):
+    """A parameter that has no gradient in the middle: its bias corrections are of the steps that it took, from there on
+    and after a state dict's round trip, in both modes."""
+    from gnn_benchmark_b200 import optim
+
+    g = torch.Generator(device="cuda").manual_seed(6)
+    ps = [torch.nn.Parameter(torch.randn(n, device="cuda", generator=g)) for n in (100, 70, 300)]
+    opt = optim.AdamW(ps, lr=1e-2, capturable=capturable)
+    want = [(p.detach().double(), torch.zeros(p.shape, device="cuda", dtype=torch.float64),
+             torch.zeros(p.shape, device="cuda", dtype=torch.float64)) for p in ps]
+    own = [0, 0, 0]
+    for t, which in enumerate(((0, 1, 2), (0, 2), (0,), (0, 1, 2), (1, 2), (0, 1, 2))):
+        for i, p in enumerate(ps):
+            p.grad = torch.randn(p.shape, device="cuda", generator=g) if i in which else None
+            if i in which:
+                own[i] += 1
+                want[i] = _reference(want[i][0], p.grad, *want[i][1:], own[i], 1e-2, 1e-2)[:3]
+        opt.step()
+        if t == 3:
+            other = optim.AdamW(ps, lr=1e-2, capturable=capturable)
+            other.load_state_dict(opt.state_dict())
+            opt = other
+    assert [int(opt.state[p]["step"]) for p in ps] == own
+    for p, (w, _, _) in zip(ps, want):
+        # up to six updates of at most about three rates each, 40 roundings a step
+        assert ((p.double() - w).abs() <= 6 * 40 * U * (w.abs() + 3e-2)).all()

@@ -147,3 +147,71 @@ def test_optimizer_refuses_shared_parameters_and_foreign_state():
     with pytest.raises(ValueError, match="another optimiser"):
         opt.load_state_dict(torch.optim.AdamW([p]).state_dict())
     assert opt.param_groups[0]["state_bits"] == 32
+
+
+def _recorded_optimizer(monkeypatch, n, **kw):
+    """An AdamW over n CPU parameters whose launches are replaced: every update notes the count that it would use."""
+    from gnn_benchmark_b200 import _lib, optim
+
+    used = []
+
+    def tick(group, device, step):
+        step += 1
+        return int(step)
+
+    monkeypatch.setattr(_lib, "require_cuda", lambda *ts: None)
+    monkeypatch.setattr(optim.AdamW, "_tick", staticmethod(tick))
+    monkeypatch.setattr(optim.AdamW, "_update",
+                        staticmethod(lambda group, members, step, scalars: used.extend((p, scalars or step) for p, _ in members)))
+    ps = [torch.nn.Parameter(torch.ones(4)) for _ in range(n)]
+    return ps, optim.AdamW(ps, **kw), used
+
+
+def _stepped(ps, opt, used, which):
+    """One step with gradients for the parameters of these numbers; the count that each of them used."""
+    for i, p in enumerate(ps):
+        p.grad = torch.ones(4) if i in which else None
+    used.clear()
+    opt.step()
+    assert len(used) == len(which)
+    return {next(i for i, q in enumerate(ps) if q is p): t for p, t in used}
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+def test_a_step_without_a_gradient_is_not_counted(monkeypatch, capturable):
+    ps, opt, used = _recorded_optimizer(monkeypatch, 3, capturable=capturable)
+    own = [0, 0, 0]
+    for round in range(2):  # the second time from a state dict, in which equal counts are shared again
+        for which in ((0, 1, 2), (0, 2), (0,), (0, 1, 2), (1,), (1, 2), (0, 1, 2)):
+            for i in which:
+                own[i] += 1
+            assert _stepped(ps, opt, used, which) == {i: own[i] for i in which}
+            assert [int(opt.state[p]["step"]) for p in ps] == own
+        opt.load_state_dict(opt.state_dict())
+
+
+def test_captured_steps_keep_their_counts(monkeypatch):
+    ps, opt, used = _recorded_optimizer(monkeypatch, 2, capturable=True)
+    _stepped(ps, opt, used, (0, 1))
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="before capturing"):  # a count of its own would have to be made inside the graph
+        _stepped(ps, opt, used, (0,))
+    _stepped(ps, opt, used, (0, 1))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    with pytest.raises(RuntimeError, match="captured step"):  # a replay would go on to count for both
+        _stepped(ps, opt, used, (1,))
+    counts = [int(opt.state[p]["step"]) for p in ps]
+    assert counts[0] == counts[1]
+    assert _stepped(ps, opt, used, (0, 1)) == {i: counts[0] + 1 for i in (0, 1)}
+    opt.load_state_dict(opt.state_dict())  # other tensors than the graph's
+    assert _stepped(ps, opt, used, (1,)) == {1: counts[0] + 2}
+
+
+def test_counts_of_parameters_that_change_their_group(monkeypatch):
+    ps, opt, used = _recorded_optimizer(monkeypatch, 2, capturable=True)
+    _stepped(ps, opt, used, (0, 1))
+    first = opt.param_groups[0]
+    opt.param_groups.append(dict(first, params=[first["params"].pop()]))
+    assert _stepped(ps, opt, used, (0, 1)) == {0: 2, 1: 2}
+    assert _stepped(ps, opt, used, (0, 1)) == {0: 3, 1: 3}
