@@ -3,6 +3,7 @@
 //
 // These operators run in few microseconds at small sizes, where the same steps in Python cost five to ten times the
 // kernel (a node's backward in Python 60 us next to 40 us for the engine's own hand-over).
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
@@ -61,6 +62,15 @@ Tensor empty_scales(int64_t rows, int64_t cols, const Tensor &like) {
 
 bool wants_grad(const Tensor &t) { return t.requires_grad(); }
 bool wants_grad(const std::optional<Tensor> &t) { return t.has_value() && t->requires_grad(); }
+
+// The results would be without the tangents that torch.autograd.forward_ad gave the inputs.
+bool has_tangent(const Tensor &t) { return t._fw_grad(/*level=*/0).defined(); }
+bool has_tangent(const std::optional<Tensor> &t) { return t.has_value() && has_tangent(*t); }
+template <typename... Ts>
+void check_tangents(const char *what, const Ts &...ts) {
+    TORCH_CHECK(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !(has_tangent(ts) || ...), what,
+                " has no forward-mode derivative: take the tangents off its inputs (torch.autograd.forward_ad.unpack_dual)");
+}
 
 // A captured backward may not reach the default stream, on which the gradients of a leaf are added up when a graph that
 // was made there still holds that leaf: the process would end inside the capture, so the node refuses before.
@@ -164,6 +174,7 @@ struct RMSNorm : torch::autograd::Function<RMSNorm> {
 
 std::vector<Tensor> rms_norm(const Tensor &x, const Tensor &w, const std::optional<Tensor> &res, double eps) {
     check_rms("rms_norm", x, w, res);
+    check_tangents("rms_norm", x, w, res);
     if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(res))) return RMSNorm::apply(x, w, res, eps);
     Normed n = rms_forward(x, w, res, eps, false);
     return res.has_value() ? std::vector<Tensor>{n.y, n.h} : std::vector<Tensor>{n.y};
@@ -171,6 +182,7 @@ std::vector<Tensor> rms_norm(const Tensor &x, const Tensor &w, const std::option
 
 std::vector<Tensor> rms_norm_fp8(const Tensor &x_, const Tensor &w_, const std::optional<Tensor> &res_, double eps) {
     check_rms("rms_norm_fp8", x_, w_, res_);
+    check_tangents("rms_norm_fp8", x_, w_, res_);
     TORCH_CHECK(!at::GradMode::is_enabled() || !(wants_grad(x_) || wants_grad(w_) || wants_grad(res_)),
                 "rms_norm_fp8 has no gradient: call it under torch.no_grad(), or use rms_norm");
     const Tensor x = rows_of(x_), w = w_.contiguous();
@@ -251,6 +263,7 @@ Tensor matmul_fp8(const Tensor &a, const Tensor &sa, const Tensor &b, const Tens
     TORCH_CHECK(b.size(1) == k, "matmul_fp8: shape mismatch a=", a.sizes(), " b=", b.sizes());
     TORCH_CHECK(!at::GradMode::is_enabled() || !(wants_grad(sa) || wants_grad(sb) || wants_grad(bias) || wants_grad(out_)),
                 "matmul_fp8 has no gradient: call it under torch.no_grad(), or use linear_fp8");
+    check_tangents("matmul_fp8", a, sa, b, sb, bias, out_);
     TORCH_CHECK(!bias.has_value() || (type_of(*bias) >= 0 && bias->dim() == 1 && bias->size(0) == n && bias->is_contiguous() &&
                                       bias->device() == a.device()),
                 "matmul_fp8: bias must be a contiguous float32, bfloat16 or float16 vector of N elements on the operands' device");
@@ -343,6 +356,7 @@ Tensor linear_fp8(const Tensor &x, const Tensor &w, const std::optional<Tensor> 
     TORCH_CHECK(!bias.has_value() || (bias->dim() == 1 && bias->size(0) == w.size(0) && type_of(*bias) >= 0 &&
                                       bias->device() == x.device()),
                 "linear_fp8: bias must be a float32, bfloat16 or float16 vector of N elements on x's device");
+    check_tangents("linear_fp8", x, w, bias);
     const bool grad = at::GradMode::is_enabled();
     return LinearFP8::apply(x, w, bias, grad && wants_grad(x), grad && wants_grad(w));
 }

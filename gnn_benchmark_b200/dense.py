@@ -336,7 +336,7 @@ def matmul_fp8(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scale
     scales for each block of 128 along K, one per row, (rows, ceil(K / 128)), or per 128 rows.  out_dtype float32,
     bfloat16 or float16 (out's type when out is given); bias (N,) of one of these; accumulate needs a float32 out.
     out may be a view with contiguous rows; it overlaps no operand.  Not differentiable: with gradients enabled, a bias
-    or out that requires one is refused."""
+    or out that requires one is refused, and one with a forward-mode tangent always."""
     out = _lib.ops().matmul_fp8(a, a_scales, b, b_scales, bias, out, out_dtype, accumulate)
     _fp8_devices.add(out.get_device())
     return out
@@ -347,7 +347,7 @@ def linear_fp8(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor = None)
     both gradients; sums in float32, the output in x's type.  float32, bfloat16 or float16.
 
     x and the output's gradient are rounded in blocks of 1 x 128 along the sum they enter, the weight in blocks of
-    128 x 128.  What is kept for the backward is 8-bit.  Differentiable once."""
+    128 x 128.  What is kept for the backward is 8-bit.  Differentiable once, in reverse mode."""
     y = _lib.ops().linear_fp8(x, weight, bias)
     _fp8_devices.add(y.get_device())
     return y

@@ -144,7 +144,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor = Non
 
     x and residual (rows, F) float32, bfloat16 or float16, F at most 16384; weight (F,) of the same type or float32.
     With a residual the result is (y, h): h, rounded to x's type, is the stream that the next layer adds to, and the
-    norm is of that rounded h.  Without one it is y alone.  Differentiable (once) in x, weight and residual."""
+    norm is of that rounded h.  Without one it is y alone.  Differentiable (once, in reverse mode) in x, weight and
+    residual."""
     r = _lib.ops().rms_norm(x, weight, residual, eps)
     return r[0] if residual is None else tuple(r)
 

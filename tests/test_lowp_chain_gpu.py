@@ -247,3 +247,34 @@ def test_offsets_past_32_bits(what):
         assert torch.equal(p[cut:], p1) and torch.equal(s[cut // 256:], s1)
         assert torch.equal(m[cut:].view(torch.uint8), m1.view(torch.uint8)) and torch.equal(v[cut:].view(torch.uint8), v1.view(torch.uint8))
     dense.check_status()
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(grad):
+    """No operator hands over an output without the tangent that its input has; in a call that is no part of forward-mode
+    differentiation, a tangent of the same tensor does not count."""
+    from torch.autograd import forward_ad
+
+    from gnn_benchmark_b200 import dense, norm
+
+    x, w = torch.randn(40, 256, device="cuda"), torch.randn(50, 256, device="cuda")
+    scale, bias, res = torch.ones(256, device="cuda"), torch.zeros(50, device="cuda"), torch.randn(40, 256, device="cuda")
+    a, b = dense.quantize_fp8(x), dense.quantize_fp8(w)
+    out = torch.zeros(40, 50, device="cuda")
+    calls = {
+        "rms_norm": (norm.rms_norm, [x, scale, res]),
+        "rms_norm_fp8": (norm.rms_norm_fp8, [x, scale, res]),
+        "linear_fp8": (dense.linear_fp8, [x, w, bias]),
+        "matmul_fp8": (lambda sa, sb, bias, out: dense.matmul_fp8(a[0], sa, b[0], sb, bias, out), [a[1], b[1], bias, out]),
+    }
+    with torch.set_grad_enabled(grad):
+        for name, (call, inputs) in calls.items():
+            call(*inputs)
+            for i, t in enumerate(inputs):
+                with forward_ad.dual_level():
+                    dual = forward_ad.make_dual(t, torch.ones_like(t))
+                    with pytest.raises(RuntimeError, match=name + " has no forward-mode derivative"):
+                        call(*inputs[:i], dual, *inputs[i + 1:])
+                    call(*inputs[:i], forward_ad.unpack_dual(dual).primal, *inputs[i + 1:])
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            torch.func.jvp(lambda x: norm.rms_norm(x, scale), (x,), (x,))
