@@ -261,7 +261,8 @@ Tensor matmul_fp8(const Tensor &a, const Tensor &sa, const Tensor &b, const Tens
     const Operand oa = operand("a", a, sa, a), ob = operand("b", b, sb, a);
     const int64_t m = a.size(0), k = a.size(1), n = b.size(0);
     TORCH_CHECK(b.size(1) == k, "matmul_fp8: shape mismatch a=", a.sizes(), " b=", b.sizes());
-    TORCH_CHECK(!at::GradMode::is_enabled() || !(wants_grad(sa) || wants_grad(sb) || wants_grad(bias) || wants_grad(out_)),
+    TORCH_CHECK(!at::GradMode::is_enabled() || !(wants_grad(a) || wants_grad(sa) || wants_grad(b) || wants_grad(sb) ||
+                                                 wants_grad(bias) || wants_grad(out_)),
                 "matmul_fp8 has no gradient: call it under torch.no_grad(), or use linear_fp8");
     check_tangents("matmul_fp8", a, sa, b, sb, bias, out_);
     TORCH_CHECK(!bias.has_value() || (type_of(*bias) >= 0 && bias->dim() == 1 && bias->size(0) == n && bias->is_contiguous() &&

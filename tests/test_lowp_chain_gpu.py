@@ -278,3 +278,16 @@ def test_forward_mode_is_refused(grad):
                     call(*inputs[:i], forward_ad.unpack_dual(dual).primal, *inputs[i + 1:])
         with pytest.raises(RuntimeError, match="no forward-mode derivative"):
             torch.func.jvp(lambda x: norm.rms_norm(x, scale), (x,), (x,))
+
+
+def test_product_refuses_codes_that_require_a_gradient():
+    from gnn_benchmark_b200 import dense
+
+    a, b = dense.quantize_fp8(torch.randn(30, 256, device="cuda")), dense.quantize_fp8(torch.randn(40, 256, device="cuda"))
+    leaf = a[0].detach().requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        dense.matmul_fp8(leaf, a[1], *b)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        dense.matmul_fp8(*b, leaf, a[1])
+    with torch.no_grad():
+        assert torch.equal(dense.matmul_fp8(leaf, a[1], *b), dense.matmul_fp8(*a, *b))
