@@ -417,6 +417,7 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_consta
                         ok = false;
                         break;
                     }
+                    __syncwarp();  // other lanes' copies are read: each lane has waited for its own, the barrier orders them
                     const float *src = mine + (kb - first) / 2 % kRing * S::kRaw;
                     float *dst = slots + ac.i * S::kSlot;
                     const float4 a = *reinterpret_cast<const float4 *>(src + 4 * lane);

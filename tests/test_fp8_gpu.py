@@ -401,3 +401,19 @@ def test_shared_rounds_on_two_streams():
     torch.cuda.synchronize()
     assert all(torch.equal(g, w) for gs, w in zip(got, want) for g in gs)
     dense.check_status()
+
+
+@pytest.mark.parametrize("m,n,k", [(300, 260, 9000), (5, 2000, 4100), (129, 16, 1290)])
+@pytest.mark.parametrize("block", [(1, 128), (128, 128)])
+def test_scales_brought_in_4_bytes(m, n, k, block):
+    """Scales that lie row by row are copied element by element, by other lanes than those that read them: the same bits
+    as from scales that lie column by column, at every one of many blocks."""
+    from gnn_benchmark_b200 import dense
+
+    qa, qb = dense.quantize_fp8(_matrix(m, k, 1)), dense.quantize_fp8(_matrix(n, k, 2), block)
+    want = dense.matmul_fp8(*qa, *qb, out_dtype=torch.float32)
+    sa, sb = qa[1].contiguous(), qb[1].contiguous()
+    assert sa.stride(1) == 1 and torch.equal(sa, qa[1])
+    for _ in range(20):
+        assert torch.equal(dense.matmul_fp8(qa[0], sa, qb[0], sb, out_dtype=torch.float32), want)
+    dense.check_status()
