@@ -168,7 +168,7 @@ __device__ __forceinline__ void fetch_scales(uint32_t dst, const Scales &s, int6
         for (int j = 0; j < N; j += 128) {
             const int64_t r = row0 + j + 4 * lane;
             const int left = (int)(rows - r < 4 ? (rows - r < 0 ? 0 : rows - r) : 4);
-            if (j + 4 * lane < N) cp_async_16_or_less(dst + (j + 4 * lane) * 4, left > 0 ? base + r : s.p, 4 * left);
+            if (j + 4 * lane < N) cp_async_16_or_less(dst + (j + 4 * lane) * 4, left > 0 ? base + r : base, 4 * left);
         }
     } else {
 #pragma unroll 1

@@ -417,3 +417,24 @@ def test_scales_brought_in_4_bytes(m, n, k, block):
     for _ in range(20):
         assert torch.equal(dense.matmul_fp8(qa[0], sa, qb[0], sb, out_dtype=torch.float32), want)
     dense.check_status()
+
+
+@pytest.mark.parametrize("m,n,k", [(301, 190, 700), (6, 1000, 2100), (130, 20, 300)])
+@pytest.mark.parametrize("first", [1, 2, 3])
+def test_scales_whose_columns_start_off_16_bytes(m, n, k, first):
+    """Columns of scales cut out of a matrix of odd column stride: some start on 16 bytes and are copied in such pieces, the
+    first one does not.  The tile's last rows have no scale."""
+    from gnn_benchmark_b200 import dense
+
+    def cut(scales):
+        rows, cols = scales.shape
+        wide = torch.full((cols + 4, (rows + 3) // 4 * 4 + 1), float("nan"), device="cuda")
+        wide[first:first + cols, :rows] = scales.t()
+        view = wide[first:first + cols, :rows].t()
+        assert view.stride(0) == 1 and view.stride(1) % 2 == 1 and view.data_ptr() % 16 != 0
+        return view
+
+    qa, qb = dense.quantize_fp8(_matrix(m, k, 1)), dense.quantize_fp8(_matrix(n, k, 2))
+    want = dense.matmul_fp8(*qa, *qb, out_dtype=torch.float32)
+    assert torch.equal(dense.matmul_fp8(qa[0], cut(qa[1]), qb[0], cut(qb[1]), out_dtype=torch.float32), want)
+    dense.check_status()
