@@ -783,6 +783,16 @@ int make_map_out(CUtensorMap *map, void *base, int type, int splits, int64_t M, 
     return GNNAGG_OK;
 }
 
+// Stages of P alone that `bytes` hold beside all of Q's k-blocks, 0 for fewer than three.  In 64 bits: Q may be long.
+constexpr int stages_beside_q(int64_t kblocks, int bn, int64_t bytes) {
+    const int64_t left = bytes - kblocks * bn * BK;
+    return left < 3 * P_BYTES ? 0 : left / P_BYTES < kMaxStages ? (int)(left / P_BYTES) : kMaxStages;
+}
+static_assert(stages_beside_q(1, 256, 5 * P_BYTES) == 3 && stages_beside_q(1, 16, 64 * P_BYTES) == kMaxStages, "Q that stays");
+static_assert(stages_beside_q(2, 256, 5 * P_BYTES) == 0 && stages_beside_q(1 << 16, 256, 5 * P_BYTES) == 0 &&
+                  stages_beside_q(1 << 17, 256, 5 * P_BYTES) == 0 && stages_beside_q((1 << 24) - 2, 256, 5 * P_BYTES) == 0,
+              "Q that does not fit, up to the longest sum");
+
 template <int BN, bool QROW, bool SWAP, bool SHARE, typename TOut>
 int launch(const CUtensorMap &mp, const CUtensorMap &mq, const CUtensorMap &mc, Params p, cudaStream_t st) {
     using S = Tile<BN, QROW>;
@@ -802,9 +812,9 @@ int launch(const CUtensorMap &mp, const CUtensorMap &mq, const CUtensorMap &mc, 
                     cudaGetErrorString(e));
     const int grid = p.items < kNumSMs ? p.items : kNumSMs;
     // Q stays where every CTA has several tiles of one column, and all of its k-blocks and three of P's fit
-    const int left = S::kStages * S::kStageBytes - p.kblocks * BN * BK;
-    p.keep_q = p.tiles_q == 1 && p.splits == 1 && p.tiles_p > grid && left >= 3 * P_BYTES;
-    p.stages = p.keep_q ? (left / P_BYTES < kMaxStages ? left / P_BYTES : kMaxStages) : S::kStages;
+    const int beside = stages_beside_q(p.kblocks, BN, S::kStages * S::kStageBytes);
+    p.keep_q = p.tiles_q == 1 && p.splits == 1 && p.tiles_p > grid && beside > 0;
+    p.stages = p.keep_q ? beside : S::kStages;
     if (SWAP && SHARE) {  // one item per CTA: all of them are resident
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)p.items);
