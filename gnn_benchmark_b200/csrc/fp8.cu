@@ -471,11 +471,11 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_consta
 #pragma unroll
             for (int j = 0; j < kCols; ++j) acc[j] = 0.0f;
             for (int kb = w.kb0; kb < w.kb1; ++kb, ac.next()) {
-                // a wait that is counted in polls (up to about a second) and leaves the loop alone: after a time-out the
-                // sums are not used, and no later wait polls more than once
+                // a wait that is counted in polls (up to about a second) and leaves the loop alone (a vote of the warp to
+                // leave it costs 1 % of the time): after a time-out the sums are not used, and later waits poll once
                 uint32_t polls = 0;
                 while (!mbar_try_wait(bar_acc_full(ac.i), ac.phase))
-                    if ((++polls & 1023u) == 0 && (polls > limit || *abort_flag != 0)) {
+                    if (limit == 0 || ((++polls & 1023u) == 0 && (polls > limit || *abort_flag != 0))) {
                         limit = 0;
                         break;
                     }

@@ -438,3 +438,32 @@ def test_scales_whose_columns_start_off_16_bytes(m, n, k, first):
     want = dense.matmul_fp8(*qa, *qb, out_dtype=torch.float32)
     assert torch.equal(dense.matmul_fp8(qa[0], cut(qa[1]), qb[0], cut(qb[1]), out_dtype=torch.float32), want)
     dense.check_status()
+
+
+def test_a_long_sum_gives_up_at_once():
+    """After a wait has run out (3 ms here) the blocks that are left are not waited for one by one: a tile of 2048 blocks
+    ends as soon as one of two."""
+    from gnn_benchmark_b200 import _lib, dense
+
+    m, n, k = 149 * 128, 16, 2048 * 128  # a tile for every SM and one more: nothing is split
+    a, b = torch.zeros(m, k, device="cuda", dtype=torch.uint8).view(F8), torch.zeros(n, k, device="cuda", dtype=torch.uint8).view(F8)
+    sa, sb = torch.ones(149, 2048, device="cuda"), torch.ones(1, 2048, device="cuda")
+    lib = _lib.lib()
+    dense.matmul_fp8(a, sa, b, sb)
+    dense.check_status()
+    begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    _lib.check(lib.gnnagg_dense_stall_test(16, 3000), "stall_test")
+    try:
+        begin.record()
+        dense.matmul_fp8(a, sa, b, sb)
+        end.record()
+        torch.cuda.synchronize()
+    finally:
+        _lib.check(lib.gnnagg_dense_stall_test(0, 0), "stall_test")
+    with pytest.raises(RuntimeError, match=r"reported status"):
+        dense.check_status()
+    dense.clear_status()
+    took = begin.elapsed_time(end)
+    assert took < 50.0, f"{took:.1f} ms"
+    assert not dense.matmul_fp8(a, sa, b, sb).any()
+    dense.check_status()
