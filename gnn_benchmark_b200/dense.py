@@ -27,10 +27,19 @@ MAX_N = 256
 # "tf32x3": the tensor-core kernels wherever `supported()`.  "fp8": the same transforms with operands rounded to
 # e4m3 in blocks of 128 (any width).  Tests and the epoch benchmark set "cublas" (torch's fp32 matmul) to have the
 # library call the kernels replace measured beside them.
+MODES = ("tf32x3", "fp8", "cublas")
 MODE = "tf32x3"
 
 _workspaces = {}
 _fp8_devices = set()  # devices that have run an 8-bit product, whose status check_status reads
+
+
+def set_mode(mode: str) -> None:
+    """Sets MODE for the transforms that follow; another name than those of MODES is refused."""
+    global MODE
+    if mode not in MODES:
+        raise ValueError(f"unknown dense mode {mode!r}: one of {', '.join(MODES)}")
+    MODE = mode
 
 
 def enabled() -> bool:

@@ -87,13 +87,13 @@ def main():
         config = yaml.safe_load(f)
     config["num_bits"] = args.num_bits
     config["is_pre_delay"] = args.is_pre_delay == "true"
+    dense.set_mode(config.get("dense_mode", dense.MODE))  # "fp8": the layers' transforms with 8-bit operands
 
     Communicator(config["num_bits"], config.get("is_async", True))
     rank, world_size = Communicator.ctx.init_dist_group()
     Quantizer_for_all_procs(world_size, config["num_bits"])
     config["input_dir"] += "{}_{}_part/".format(config["graph_name"], world_size)
     device = torch.device("cuda", torch.cuda.current_device())
-    dense.MODE = config.get("dense_mode", dense.MODE)  # "fp8": the layers' transforms with 8-bit operands
     set_random_seed(config["random_seed"])
     model, optimizer = create_model_and_optimizer(config, device)
     data = load_data(config)

@@ -215,3 +215,21 @@ def test_counts_of_parameters_that_change_their_group(monkeypatch):
     opt.param_groups.append(dict(first, params=[first["params"].pop()]))
     assert _stepped(ps, opt, used, (0, 1)) == {0: 2, 1: 2}
     assert _stepped(ps, opt, used, (0, 1)) == {0: 3, 1: 3}
+
+
+def test_an_unknown_dense_mode_is_refused(monkeypatch, tmp_path):
+    """A misspelt name must not turn the tensor-core kernels off without a word."""
+    from gnn_benchmark_b200 import dense, train
+
+    monkeypatch.setattr(dense, "MODE", dense.MODE)  # put back at the end
+    for mode in dense.MODES:
+        dense.set_mode(mode)
+        assert dense.MODE == mode and dense.enabled() == (mode != "cublas")
+    for mode in ("FP8", "fp16", "", None, 8):
+        with pytest.raises(ValueError, match="unknown dense mode"):
+            dense.set_mode(mode)
+    path = tmp_path / "config.yaml"
+    path.write_text("dense_mode: tf32\n")
+    monkeypatch.setattr("sys.argv", ["train", "--config", str(path)])
+    with pytest.raises(ValueError, match="unknown dense mode 'tf32'"):
+        train.main()
