@@ -1,6 +1,8 @@
 import os
 import sys
+import threading
 
+import numpy as np
 import pytest
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -26,3 +28,19 @@ def cuda_lib():
 
     build.build()
     return _lib.lib()
+
+
+@pytest.fixture(scope="session", autouse=True)
+def npz_arrays_are_read_one_at_a_time():
+    """Ranks that run as threads read their arrays from one open .npz archive, whose zip file has a single position: two
+    reads at a time fail now and then.  So an array is read under a lock."""
+    archive, lock = type(np.load(os.path.join(GOLDEN, "quant_v1.npz"))), threading.Lock()
+    read = archive.__getitem__
+
+    def read_alone(self, key):
+        with lock:
+            return read(self, key)
+
+    archive.__getitem__ = read_alone
+    yield
+    archive.__getitem__ = read
