@@ -82,8 +82,10 @@ void check_capture(const char *what, const Tensor &t) {
     const auto node = torch::autograd::get_current_node();
     if (!node) return;
     const c10::Stream other = c10::cuda::getDefaultCUDAStream(t.get_device()).unwrap();
-    for (const auto &edge : node->next_edges()) {
-        if (!edge.function || edge.function->num_outputs() != 0) continue;  // only a leaf's node leads nowhere
+    for (uint32_t i = 0; i < node->num_outputs(); ++i) {
+        const auto &edge = node->next_edge(i);
+        // only a leaf's node leads nowhere; one whose gradient this pass does not compute is not reached
+        if (!edge.function || edge.function->num_outputs() != 0 || !node->task_should_compute_output(i)) continue;
         const auto stream = edge.function->stream();
         TORCH_CHECK(!stream.has_value() || *stream != other, what,
                     ": captured backward of a leaf that a graph made on the default stream still holds (delete what that "

@@ -291,3 +291,27 @@ def test_product_refuses_codes_that_require_a_gradient():
         dense.matmul_fp8(*b, leaf, a[1])
     with torch.no_grad():
         assert torch.equal(dense.matmul_fp8(leaf, a[1], *b), dense.matmul_fp8(*a, *b))
+
+
+def test_captured_gradients_beside_an_eager_graph():
+    """What a captured pass does not compute does not keep it: the gradient of x alone, while an eager graph holds the
+    weight."""
+    from gnn_benchmark_b200 import dense, norm
+
+    x = torch.randn(16, 64, device="cuda", requires_grad=True)
+    w, m = torch.ones(64, device="cuda", requires_grad=True), torch.randn(48, 64, device="cuda", requires_grad=True)
+    gy, gz = torch.randn(16, 64, device="cuda"), torch.randn(16, 48, device="cuda")
+    calls = [lambda: torch.autograd.grad(norm.rms_norm(x, w), [x], gy), lambda: torch.autograd.grad(dense.linear_fp8(x, m), [x], gz)]
+    want = [call()[0] for call in calls]
+    held = (w * 2).sum() + (m * 2).sum()
+    torch.cuda.synchronize()
+    for call, expected in zip(calls, want):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            (got,) = call()
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, expected)
+    held.backward()
+    assert torch.equal(w.grad, torch.full_like(w, 2.0))
