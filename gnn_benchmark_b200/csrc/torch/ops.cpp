@@ -9,6 +9,7 @@
 #include <torch/extension.h>
 
 #include <optional>
+#include <unordered_set>
 #include <vector>
 
 #include "gnnagg.h"
@@ -72,8 +73,9 @@ void check_tangents(const char *what, const Ts &...ts) {
                 " has no forward-mode derivative: take the tangents off its inputs (torch.autograd.forward_ad.unpack_dual)");
 }
 
-// A captured backward may not reach the default stream, on which the gradients of a leaf are added up when a graph that
-// was made there still holds that leaf: the process would end inside the capture, so the node refuses before.
+// A captured backward may not reach the default stream: a forward's node goes on where the forward ran, and the gradients
+// of a leaf are added up there when a graph that was made there still holds that leaf.  The process would end inside the
+// capture, so the node refuses before.
 void check_capture(const char *what, const Tensor &t) {
     cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
     if (cudaStreamIsCapturing(static_cast<cudaStream_t>(stream_of(t)), &status) != cudaSuccess ||
@@ -82,14 +84,24 @@ void check_capture(const char *what, const Tensor &t) {
     const auto node = torch::autograd::get_current_node();
     if (!node) return;
     const c10::Stream other = c10::cuda::getDefaultCUDAStream(t.get_device()).unwrap();
-    for (uint32_t i = 0; i < node->num_outputs(); ++i) {
-        const auto &edge = node->next_edge(i);
-        // only a leaf's node leads nowhere; one whose gradient this pass does not compute is not reached
-        if (!edge.function || edge.function->num_outputs() != 0 || !node->task_should_compute_output(i)) continue;
-        const auto stream = edge.function->stream();
-        TORCH_CHECK(!stream.has_value() || *stream != other, what,
-                    ": captured backward of a leaf that a graph made on the default stream still holds (delete what that "
-                    "graph computed, its loss for example, before the capture, or compute it on a side stream)");
+    // all nodes that this pass goes on to: those behind a view of the leaf, and only those whose gradient it computes
+    std::vector<torch::autograd::Node *> todo{node.get()};
+    std::unordered_set<torch::autograd::Node *> seen;
+    while (!todo.empty()) {
+        torch::autograd::Node *at = todo.back();
+        todo.pop_back();
+        for (uint32_t i = 0; i < at->num_outputs(); ++i) {
+            torch::autograd::Node *next = at->next_edge(i).function.get();
+            if (next == nullptr || !at->task_should_compute_output(i) || !seen.insert(next).second) continue;
+            const auto stream = next->stream();
+            const bool leaf = next->num_outputs() == 0;  // a leaf's node leads nowhere
+            TORCH_CHECK(!stream.has_value() || *stream != other || !leaf, what,
+                        ": captured backward of a leaf that a graph made on the default stream still holds (delete what that "
+                        "graph computed, its loss for example, before the capture, or compute it on a side stream)");
+            TORCH_CHECK(!stream.has_value() || *stream != other, what, ": captured backward reaches ", next->name(),
+                        ", whose forward ran on the default stream (capture that too, or run it on a side stream)");
+            todo.push_back(next);
+        }
     }
 }
 

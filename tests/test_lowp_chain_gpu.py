@@ -295,7 +295,7 @@ def test_product_refuses_codes_that_require_a_gradient():
 
 def test_captured_gradients_beside_an_eager_graph():
     """What a captured pass does not compute does not keep it: the gradient of x alone, while an eager graph holds the
-    weight."""
+    weight.  What it does reach, it reaches through views and other operators too."""
     from gnn_benchmark_b200 import dense, norm
 
     x = torch.randn(16, 64, device="cuda", requires_grad=True)
@@ -313,5 +313,12 @@ def test_captured_gradients_beside_an_eager_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, expected)
+    early = w * 1.0  # its node belongs to the default stream
+    for call, message in ((lambda: torch.autograd.grad(norm.rms_norm(x, w.view(64)), [w], gy), "still holds"),
+                          (lambda: torch.autograd.grad(dense.linear_fp8(x.detach(), m.view(48, 64)), [m], gz), "still holds"),
+                          (lambda: norm.rms_norm(x, early).sum().backward(), "forward ran on the default stream")):
+        with pytest.raises(RuntimeError, match=message):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
     held.backward()
     assert torch.equal(w.grad, torch.full_like(w, 2.0))
