@@ -4,8 +4,9 @@
 //     p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
 // A pure stream: 28 bytes an element with 32-bit moments and fp32 parameters, 16 with 8-bit ones (22 and 10 for 16-bit
-// parameters), so the kernel is bound by memory, and for a small model by the launch.  90 M elements take 371 us at
-// 6.8 TB/s and 217 us at 6.7 TB/s (293 at 6.8, and 209 at 4.3: at 10 bytes an element its instructions bound it).
+// parameters), so the kernel is bound by memory, and for a small model by the launch.  90 M elements take 374 us at
+// 6.7 TB/s and 235 at 6.2 TB/s (295 at 6.7, and 232 at 3.9: at 10 bytes an element its instructions bound it, the schedulers
+// issue in 90 % of the cycles).
 //
 // The table of tensors (pointers, sizes, the prefix of their block counts) travels in the launch's own parameters: no
 // copy to the device, nothing to keep alive, and a captured graph owns its table.  A warp takes 256 consecutive
@@ -52,7 +53,7 @@ static_assert(sizeof(Table<kLargeCap>) <= 32764, "kernel parameters");
 
 // Four elements as they lie in memory, those behind the end as zeros; converted after the last load, in pairs.  With
 // the conversion inside the branch below, a 16-bit type's loads wait for one another: 90 M bf16 parameters took 352 us
-// (274 with 8-bit moments) instead of 293 (209).
+// instead of 293, and with 8-bit moments a third longer.
 template <typename T>
 struct Raw4 {
     uint32_t w[sizeof(T)];

@@ -19,21 +19,25 @@
 //               hands over both;
 //   warps 4-11  read a block's product, scale and add it; after the last block, convert and store.  Warp w reads
 //               lane quarter w % 4 and one half of the columns.
-// What bounds a block is the hand-over and scaling: per scheduler 256 FMAs, 180 cycles of tensor-memory reads and a
-// round trip between the warps of some 400 cycles over two buffers, against 512 cycles of MMA.  So the scaling loop holds
-// nothing that another warp can do.  8192 x 8192 x 8192 takes 490 us alone, 2.2 PFLOP/s, and 583 in a long run at the
-// power limit.  Two CTAs that share a tile's operands were slower (the hand-over then takes 1279 cycles instead of 590),
-// and so were tiles 128 wide with two CTAs an SM (644 us where this took 539), and sixteen scaling warps.
+// What bounds a block is the scaling warps' chain: the wait, the tensor-memory reads, the FMAs, the release, over two
+// partial products.  At 4096 x 4096 x 4096 a block takes 985 cycles, of which the MMAs fill 512; the schedulers issue in 55 %
+// of them and the FMA pipe is busy in 31 %.  With row scales on both sides it takes 1525 (512, 60 %, 38 %).  No unit is
+// full, so the scaling loop holds nothing that another warp can do.  8192 x 8192 x 8192 takes 500 us alone, 2.2 PFLOP/s, and
+// 580 in a long run, where the power limit takes the clock from 1965 to about 1490 MHz (780 and 830 with row scales).
+// Two CTAs that share a tile's operands were slower (the hand-over then goes through both), and so were tiles 128 wide
+// with two CTAs an SM (644 us where this took 539 at the time), and sixteen scaling warps.
 // Where one column of tiles and few k-blocks make up the product (tall activations, a small weight), Q stays in shared
 // memory and only P's blocks go round: a third of the loads, and twice the blocks on their way (612500 x 256 x 100 in
-// 76 us instead of 109; its bytes take 58).
+// 82 us instead of 109; its bytes take 58).  A tile of one block then takes 3900 cycles, most of them in the chain from the
+// product over the conversion to the stores: DRAM is at half its rate, the schedulers issue in 43 %.
 // Output tiles leave through shared memory by TMA stores, which run under the next tile's MMAs; rows that TMA cannot
-// address, and outputs that are added to, by plain stores.
+// address, and outputs that are added to, by plain stores (four bytes at a time: 612500 x 256 x 256 in fp32 takes 900 us
+// with the addition and 141 without).
 // The tiles of a last round that would leave SMs idle are shared out evenly instead: each CTA takes the same number of
 // their k-blocks, a stretch that lies in one tile or two.  Whoever completes a tile (a count per tile and warp, no
 // waiting) adds its parts in the order of k and stores it.
 // A tile's sum may be split along k over several CTAs (few tiles, long sums): each writes an fp32 partial product
-// to the workspace and a second kernel adds them in a fixed order (256 x 256 x 612500: 81 us and 9 for that kernel); up
+// to the workspace and a second kernel adds them in a fixed order (256 x 256 x 612500: 94 us, 19 of them that kernel); up
 // to eight small ones (few rows) are CTAs of a cluster, and the first adds the others' from its own shared memory, which
 // saves the second launch (8 x 4096 x 4096: 10 us a call).
 // Every wait is bounded (about a second); on a time-out the kernel records a code in the library's status word,
@@ -735,7 +739,7 @@ Plan plan_of(int64_t M, int64_t N, int64_t K) {
     p.rows = M;
     p.ldp = div_up(N, 4) * 4;
     // A last round of fewer tiles than SMs is shared out where that shortens it by 40 k-blocks or more (a block takes
-    // 0.4 us, 0.8 with row scales on both sides; the parts' way through memory and the cleared counts 12 to 14 us in all).
+    // 0.5 us, 0.8 with row scales on both sides; the parts' way through memory and the cleared counts 12 to 14 us in all).
     // 2048 x 2560 x 8192: 73 -> 66 us, with row scales 116 -> 91; 4096 x 4096 x 4096, 17 blocks shorter: 80 -> 86.  CTAs
     // that share a tile are at different k at a time, so the operands have to stay in L2 in the main: at 168 MB (8192 x
     // 2048 x 16384) 275 -> 262 and 424 -> 391, at 210 MB (1500 x 2000 x 60000) 263 -> 352.  At most nine CTAs have a part

@@ -7,9 +7,11 @@
 // reciprocal is taken once, and columns through a shared table of the runs' maxima.  Transposed codes go through a 16 KB
 // shared tile: 8 rows of a column are one 8-byte piece, at piece index XOR (column / V) so that a warp's stores meet
 // different banks, and leave as 16-byte stores.
-// Bound by memory: per element its bytes in and one byte out for each orientation.  What keeps it from the floor is
-// instruction issue: 16384 x 8192 bf16 in both orientations take 109 us, 4.9 TB/s, at 7 instructions an element (195 us at
-// 15, with a shuffle reduction per row and a reciprocal per thread and column); fp32 161 us, 5.0 TB/s.
+// Its floor is memory: per element its bytes in and one byte out for each orientation.  16384 x 8192 bf16 in both
+// orientations take 106 us, 5.1 TB/s, at 16 instructions an element (195 us with a shuffle reduction per row and a reciprocal
+// per thread and column); the schedulers issue in 62 % of the cycles, and the 24 warps that the registers allow an SM wait
+// for loads in most of the others.  fp32 158 us, 5.1 TB/s.  Rows off 16 bytes are loaded element by element: 612500 x 100 bf16
+// take 117 us, 2.1 TB/s, and 30000 x 1501 78 us.
 #include "lowp.cuh"
 
 namespace gnnagg {

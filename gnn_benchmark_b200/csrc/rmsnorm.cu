@@ -10,8 +10,10 @@
 // once, writes dh once and keeps the column sums of dw in registers over all rows of a persistent block; a second kernel
 // adds the blocks' sums in a fixed order (no atomics).
 //
-// Bound by memory forward: 612500 x 256 bf16 with a residual in 189 us, 6.6 TB/s (codes: 184).  Backward by instruction
-// issue and the two reductions a row: 218 us there, 5.8 TB/s; 8191 x 5000 takes 56 and 79 us.
+// Bound by memory forward: 612500 x 256 bf16 with a residual in 192 us, 6.5 TB/s (codes: 195, 5.7 TB/s); 8191 x 5000 in 56.
+// Backward 227 us, 5.5 TB/s, and 84 us, column sums included (9 of them each).  In the wide one nothing is full: the
+// schedulers issue in 56 % of the cycles, DRAM reads at 51 % of its rate; a block waits for its row, reduces it and waits at
+// the barrier, with the next row on its way and three blocks an SM to fill the gaps.
 //
 // As codes: with t = h w and a = max |t| over 128 columns, code = e4m3(t * (448 / a)) and scale = a / 448 * r.
 // The row's statistic enters the scale alone, so the codes are ready before the sum of squares is, and do not
@@ -309,7 +311,7 @@ rms_norm_bwd_kernel(const BwdParams p) {
 
 // The block-per-row form on 16-byte rows: the next row's chunks are copied to shared memory (cp.async, every thread its
 // own, so that no barrier is needed for them) while the block works on this one.  Without, a block's three loads, its
-// reduction and its store follow one another: 16384 x 4096 bf16 in 116 us instead of 104.
+// reduction and its store follow one another: 16384 x 4096 bf16 in 116 us instead of 104 (109 with cold caches).
 template <typename T, int NV>
 __global__ void __launch_bounds__(kBlockThreads) rms_norm_bwd_ahead_kernel(const BwdParams p) {
     constexpr int V = Vec<T>::N;
