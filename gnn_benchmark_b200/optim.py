@@ -112,21 +112,20 @@ class AdamW(torch.optim.Optimizer):
         stepping = {id(p) for p, _ in members}
         idle = {id(s["step"]) for p, s in self.state.items() if s and id(p) not in stepping}
         known = self.__dict__.setdefault("_captured", {})  # id -> weak reference: counts of captured steps
-        copies = {}
+        counts = {id(s["step"]): s["step"] for _, s in members}
+        shared = {k: c for k, c in counts.items() if k in idle}
+        if shared and capturing:
+            raise RuntimeError("AdamW: take a step with the gradients of these parameters alone before capturing (they share "
+                               "their step count with parameters that have no gradient)")
+        if any(k in known and known[k]() is c for k, c in shared.items()):
+            raise RuntimeError("AdamW: a captured step updates parameters that have no gradient now together with others that "
+                               "have one: their step count is shared (once the graph is not replayed any more, "
+                               "load_state_dict(state_dict()) gives them other counts)")
+        if capturing:
+            known.update((k, weakref.ref(c)) for k, c in counts.items())
+        copies = {k: c.clone() for k, c in shared.items()}
         for _, state in members:
-            count = state["step"]
-            if id(count) in idle:
-                if capturing:
-                    raise RuntimeError("AdamW: take a step with the gradients of these parameters alone before capturing (they "
-                                       "share their step count with parameters that have no gradient)")
-                if id(count) in known and known[id(count)]() is count:
-                    raise RuntimeError("AdamW: a captured step updates parameters that have no gradient now together with "
-                                       "others that have one: their step count is shared")
-                if id(count) not in copies:
-                    copies[id(count)] = count.clone()
-                state["step"] = copies[id(count)]
-            elif capturing:
-                known[id(count)] = weakref.ref(count)
+            state["step"] = copies.get(id(state["step"]), state["step"])
 
     @torch.no_grad()
     def step(self, closure=None):

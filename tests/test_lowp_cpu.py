@@ -233,3 +233,17 @@ def test_an_unknown_dense_mode_is_refused(monkeypatch, tmp_path):
     monkeypatch.setattr("sys.argv", ["train", "--config", str(path)])
     with pytest.raises(ValueError, match="unknown dense mode 'tf32'"):
         train.main()
+
+
+def test_a_refused_capture_leaves_no_trace(monkeypatch):
+    """Counts of a step whose capture is refused are not those of a captured step."""
+    ps, opt, used = _recorded_optimizer(monkeypatch, 4, capturable=True)
+    _stepped(ps, opt, used, (0, 1))
+    _stepped(ps, opt, used, (2, 3))
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="before capturing"):
+        _stepped(ps, opt, used, (0, 1, 2))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    assert _stepped(ps, opt, used, (0, 2)) == {0: 2, 2: 2}
+    assert _stepped(ps, opt, used, (0, 1, 2, 3)) == {0: 3, 1: 2, 2: 3, 3: 2}
