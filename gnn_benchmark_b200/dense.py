@@ -344,6 +344,7 @@ def matmul_fp8(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scale
     """out (M, N) (+)= (a * a_scales) @ (b * b_scales).T (+ bias): a (M, K) and b (N, K) float8_e4m3fn with float32
     scales for each block of 128 along K, one per row, (rows, ceil(K / 128)), or per 128 rows.  out_dtype float32,
     bfloat16 or float16 (out's type when out is given); bias (N,) of one of these; accumulate needs a float32 out.
+    A block's two scales are multiplied first: where that product leaves float32's range, so does the block's sum.
     out may be a view with contiguous rows; it overlaps no operand.  Not differentiable: with gradients enabled, an input
     or out that requires one is refused, and one with a forward-mode tangent always."""
     out = _lib.ops().matmul_fp8(a, a_scales, b, b_scales, bias, out, out_dtype, accumulate)

@@ -387,7 +387,7 @@ int gnnagg_rms_norm_bwd(const void *gy, int64_t ldgy, const void *gh, int64_t ld
  *   workspace gnnagg_fp8_matmul_workspace_bytes(M, N, K) bytes, 16-byte aligned; NULL when that is 0.  Its contents
  *             mean nothing between calls.
  * Sums are fp32: chains of 128 elements in tensor memory, their scaled sum in registers; a sum that is split over
- * CTAs is joined in a fixed order.
+ * CTAs is joined in a fixed order.  A block's two scales are multiplied first, and their product is in fp32's range.
  * gnnagg_fp8_matmul_status synchronises the stream and returns 0, or the positive code of the first wait that ran
  * out inside a kernel on the current device (codes as for gnnagg_dense_status; the output is then undefined);
  * gnnagg_fp8_matmul_status_clear resets it.  gnnagg_dense_stall_test covers these launches too.
