@@ -181,7 +181,7 @@ def _stepped(ps, opt, used, which):
 def test_a_step_without_a_gradient_is_not_counted(monkeypatch, capturable):
     ps, opt, used = _recorded_optimizer(monkeypatch, 3, capturable=capturable)
     own = [0, 0, 0]
-    for round in range(2):  # the second time from a state dict, in which equal counts are shared again
+    for _ in range(2):  # the second time from a state dict, in which equal counts are shared again
         for which in ((0, 1, 2), (0, 2), (0,), (0, 1, 2), (1,), (1, 2), (0, 1, 2)):
             for i in which:
                 own[i] += 1
