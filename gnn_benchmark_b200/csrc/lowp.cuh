@@ -62,6 +62,12 @@ __device__ __forceinline__ float load_as_f32(const void *p, int type, int64_t i)
                                : to_f32(static_cast<const __half *>(p)[i]);
 }
 
+// 16 bytes global -> shared; completed as the copies of 4 bytes are (common.cuh).
+__device__ __forceinline__ void cp_async_16(void *smem, const void *gmem) {
+    const uint32_t s = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s), "l"(gmem) : "memory");
+}
+
 template <typename T>
 struct Vec {
     static constexpr int N = 16 / (int)sizeof(T);  // elements of one 16-byte access
